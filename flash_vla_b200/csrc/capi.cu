@@ -108,7 +108,7 @@ static void gemm_ws(void* ws, size_t ws_bytes, int M, int K, void** p, size_t* n
 // Device status word written by kernels whose bounded waits ran out (0 = healthy).
 __device__ int g_device_status;
 
-static int* device_status_ptr() {
+int* device_status_ptr() {
     static thread_local int cached_dev = -1;
     static thread_local int* cached_ptr = nullptr;
     int dev = 0;
@@ -249,7 +249,7 @@ using namespace fvla;
 extern "C" {
 
 const char* fvla_last_error(void) { return g_error; }
-int fvla_abi_version(void) { return 5; }
+int fvla_abi_version(void) { return 6; }
 unsigned long long fvla_launch_count(void) { return g_launches.load(std::memory_order_relaxed); }
 
 int fvla_device_status(void* stream) {

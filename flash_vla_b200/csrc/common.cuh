@@ -166,6 +166,8 @@ bool plan_lookup(int M, int N, int K, int kind, PlanChoice* out);
 // Host-side: record the message of the last failing call on this thread.
 void set_error(const char* fmt, ...);
 int check_launch(const char* what);
+// Health word of the current device, written by kernels (0 = healthy).
+int* device_status_ptr();
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

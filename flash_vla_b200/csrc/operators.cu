@@ -1,0 +1,141 @@
+// extern "C" entries of masked attention and of the 8-bit KV cache: argument validation and launches. Nothing here allocates, frees or synchronises.
+#include "common.cuh"
+#include "masked_attention.cuh"
+#include "quantized_cache.cuh"
+
+namespace fvla {
+
+static inline cudaStream_t S(void* s) { return reinterpret_cast<cudaStream_t>(s); }
+
+#define FVLA_REQUIRE(cond, ...)            \
+    do {                                   \
+        if (!(cond)) {                     \
+            set_error(__VA_ARGS__);        \
+            return FVLA_ERR_ARG;           \
+        }                                  \
+    } while (0)
+
+template <typename... KArgs, typename... Args>
+static int launch(const char* what, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
+    const cudaError_t e = launch_pdl(kern, grid, block, smem, st, args...);
+    if (e != cudaSuccess) { set_error("%s: %s", what, cudaGetErrorString(e)); return FVLA_ERR_LAUNCH; }
+    return check_launch(what);
+}
+
+static bool block_ok(int block) { return block == 16 || block == 32 || block == 64 || block == 128; }
+// Element strides such that every row starts on 16 bytes.
+static bool strides_ok(const long long (&s)[3], int multiple) { return s[0] % multiple == 0 && s[1] % multiple == 0 && s[2] % multiple == 0; }
+
+static int check_attention(const struct fvla_attention* a) {
+    FVLA_REQUIRE(a != nullptr, "attention: null arguments");
+    FVLA_REQUIRE(a->episodes > 0 && a->tokens > 0 && a->keys >= 0 && a->heads > 0 && a->kv_heads > 0, "attention: empty shape");
+    FVLA_REQUIRE(a->heads % a->kv_heads == 0 && a->heads / a->kv_heads <= 128, "attention: %d heads over %d K/V heads", a->heads, a->kv_heads);
+    const bool q8 = a->k_scale != nullptr;
+    const int multiple = q8 ? 16 : 8;
+    FVLA_REQUIRE(a->head_dim > 0 && a->head_dim <= 256 && a->head_dim % multiple == 0, "attention: head_dim %d (a multiple of %d up to 256)", a->head_dim, multiple);
+    FVLA_REQUIRE(a->q != nullptr && a->out != nullptr && (a->keys == 0 || (a->k != nullptr && a->v != nullptr)), "attention: null pointer");
+    FVLA_REQUIRE((a->v_scale != nullptr) == q8, "attention: scales of both K and V, or of neither");
+    FVLA_REQUIRE(aligned16(a->q) && aligned16(a->k) && aligned16(a->v) && aligned16(a->out), "attention: every tensor must be 16-byte aligned");
+    FVLA_REQUIRE(strides_ok(a->q_stride, 8) && strides_ok(a->out_stride, 8) && strides_ok(a->k_stride, multiple) && strides_ok(a->v_stride, multiple),
+                 "attention: every row must start on 16 bytes");
+    FVLA_REQUIRE(!q8 || (block_ok(a->block) && a->keys % a->block == 0), "attention: blocks of %d rows in %d", a->block, a->keys);
+    FVLA_REQUIRE((a->q_docs != nullptr) == (a->k_docs != nullptr), "attention: documents of queries and keys, or of neither");
+    FVLA_REQUIRE(a->prefix == nullptr || a->causal, "attention: a prefix without the causal mask");
+    FVLA_REQUIRE(a->weights == nullptr || (a->lse != nullptr && a->k_docs == nullptr), "attention: weights need the log-sum-exp, and no documents");
+    FVLA_REQUIRE(a->cap >= 0.f && a->scale == a->scale, "attention: scale and cap");
+    FVLA_REQUIRE((long long)a->tokens * a->heads < (1ll << 31) && (long long)a->episodes * a->kv_heads < 65536, "attention: too many rows");
+    return FVLA_OK;
+}
+
+static mattn::Args attention_args(const struct fvla_attention* a) {
+    mattn::Args p;
+    p.q = a->q; p.k = a->k; p.v = a->v; p.k_scale = static_cast<const float*>(a->k_scale); p.v_scale = static_cast<const float*>(a->v_scale);
+    p.out = static_cast<bf16*>(a->out); p.lse = static_cast<float*>(a->lse);
+    p.prefix = a->prefix; p.q_lens = a->q_lens; p.k_lens = a->k_lens; p.q_start = a->q_start; p.q_docs = a->q_docs; p.k_docs = a->k_docs; p.k_pos = a->k_pos;
+    p.slopes = a->slopes; p.weights = static_cast<float*>(a->weights);
+    for (int i = 0; i < 3; ++i) { p.qs[i] = a->q_stride[i]; p.ks[i] = a->k_stride[i]; p.vs[i] = a->v_stride[i]; p.os[i] = a->out_stride[i]; }
+    p.scale = a->scale; p.cap = a->cap; p.decay = a->decay;
+    p.episodes = a->episodes; p.tokens = a->tokens; p.keys = a->keys; p.heads = a->heads; p.kv_heads = a->kv_heads; p.dim = a->head_dim;
+    p.block = a->block; p.causal = a->causal;
+    return p;
+}
+
+}  // namespace fvla
+
+using namespace fvla;
+
+extern "C" {
+
+size_t fvla_attention_workspace_bytes(const struct fvla_attention* a) {
+    (void)a;
+    return 0;
+}
+
+int fvla_attention_run(const struct fvla_attention* a, void* stream) {
+    int rc = check_attention(a);
+    if (rc) return rc;
+    const mattn::Args p = attention_args(a);
+    const bool q8 = p.k_scale != nullptr;
+    const dim3 rows((unsigned)(((long long)p.episodes * p.tokens * p.heads + 3) / 4)), keys((unsigned)(((long long)p.episodes * p.keys + 3) / 4));
+    rc = launch("attention_rows_kernel", q8 ? mattn::attention_rows_kernel<true> : mattn::attention_rows_kernel<false>, rows, dim3(128), 0, S(stream), p);
+    if (rc || p.weights == nullptr || p.keys == 0) return rc;
+    return launch("key_weights_kernel", q8 ? mattn::key_weights_kernel<true> : mattn::key_weights_kernel<false>, keys, dim3(128), 0, S(stream), p);
+}
+
+int fvla_cache_append(const struct fvla_cache_append_args* a, void* stream) {
+    FVLA_REQUIRE(a != nullptr, "cache_append: null arguments");
+    FVLA_REQUIRE(a->episodes > 0 && a->episodes < 65536 && a->tokens > 0 && a->rows > 0 && a->kv_heads > 0, "cache_append: empty shape");
+    FVLA_REQUIRE(a->head_dim > 0 && a->head_dim <= 256 && a->head_dim % 16 == 0, "cache_append: head_dim %d (a multiple of 16 up to 256)", a->head_dim);
+    FVLA_REQUIRE(block_ok(a->block) && a->rows % a->block == 0, "cache_append: blocks of %d rows in %d", a->block, a->rows);
+    FVLA_REQUIRE(a->tokens <= a->rows, "cache_append: %d rows into a cache of %d", a->tokens, a->rows);
+    FVLA_REQUIRE(a->k && a->v && a->k_held && a->v_held && a->k_scale && a->v_scale && a->starts, "cache_append: null pointer");
+    FVLA_REQUIRE(aligned16(a->k) && aligned16(a->v) && aligned16(a->k_held) && aligned16(a->v_held), "cache_append: every tensor must be 16-byte aligned");
+    FVLA_REQUIRE(strides_ok(a->k_stride, 8) && strides_ok(a->v_stride, 8) && strides_ok(a->k_held_stride, 16) && strides_ok(a->v_held_stride, 16),
+                 "cache_append: every row must start on 16 bytes");
+    q8::AppendArgs p;
+    p.x[0] = static_cast<const bf16*>(a->k); p.x[1] = static_cast<const bf16*>(a->v);
+    p.held[0] = static_cast<uint8_t*>(a->k_held); p.held[1] = static_cast<uint8_t*>(a->v_held);
+    p.scale[0] = static_cast<float*>(a->k_scale); p.scale[1] = static_cast<float*>(a->v_scale);
+    for (int i = 0; i < 3; ++i) { p.xs[0][i] = a->k_stride[i]; p.xs[1][i] = a->v_stride[i]; p.hs[0][i] = a->k_held_stride[i]; p.hs[1][i] = a->v_held_stride[i]; }
+    p.starts = a->starts; p.counts = a->counts; p.status = device_status_ptr();
+    p.tokens = a->tokens; p.rows = a->rows; p.blocks = a->rows / a->block; p.block = a->block; p.kv_heads = a->kv_heads; p.dim = a->head_dim;
+    const int windows = (a->tokens + a->block - 2) / a->block + 1;           // blocks that a run of so many rows can touch
+    return launch("cache_append_kernel", q8::cache_append_kernel, dim3(windows * a->kv_heads, 2, a->episodes), dim3(q8::APPEND_THREADS), 0, S(stream), p);
+}
+
+size_t fvla_cache_evict_workspace_bytes(int episodes, int keep) { return episodes > 0 && keep > 0 ? (size_t)episodes * keep * sizeof(int) : 0; }
+
+int fvla_cache_evict(const struct fvla_cache_evict_args* a, void* stream) {
+    FVLA_REQUIRE(a != nullptr, "cache_evict: null arguments");
+    FVLA_REQUIRE(a->episodes > 0 && a->episodes < 65536 && a->rows > 0 && a->out_rows > 0 && a->kv_heads > 0 && a->keep > 0, "cache_evict: empty shape");
+    FVLA_REQUIRE(a->keep <= a->out_rows, "cache_evict: %d rows to keep in a cache of %d", a->keep, a->out_rows);
+    FVLA_REQUIRE(a->sinks >= 0 && a->recent >= 0 && (long long)a->sinks + a->recent <= a->keep, "cache_evict: %d first and %d last rows in %d", a->sinks, a->recent, a->keep);
+    FVLA_REQUIRE(a->head_dim > 0 && a->head_dim <= 256 && a->head_dim % 16 == 0, "cache_evict: head_dim %d (a multiple of 16 up to 256)", a->head_dim);
+    FVLA_REQUIRE(block_ok(a->block) && a->rows % a->block == 0 && block_ok(a->out_block) && a->out_rows % a->out_block == 0, "cache_evict: blocks of %d rows in %d, %d in %d",
+                 a->block, a->rows, a->out_block, a->out_rows);
+    FVLA_REQUIRE(a->k && a->v && a->k_scale && a->v_scale && a->out_k && a->out_v && a->out_k_scale && a->out_v_scale && a->weights && a->lengths && a->out_lengths,
+                 "cache_evict: null pointer");
+    FVLA_REQUIRE(aligned16(a->k) && aligned16(a->v) && aligned16(a->out_k) && aligned16(a->out_v), "cache_evict: every tensor must be 16-byte aligned");
+    FVLA_REQUIRE(strides_ok(a->k_stride, 16) && strides_ok(a->v_stride, 16) && strides_ok(a->out_k_stride, 16) && strides_ok(a->out_v_stride, 16),
+                 "cache_evict: every row must start on 16 bytes");
+    if (a->ws == nullptr || a->ws_bytes < fvla_cache_evict_workspace_bytes(a->episodes, a->keep)) {
+        set_error("cache_evict: workspace of %zu bytes needed", fvla_cache_evict_workspace_bytes(a->episodes, a->keep));
+        return FVLA_ERR_WORKSPACE;
+    }
+    q8::EvictArgs p;
+    p.held[0] = static_cast<const uint8_t*>(a->k); p.held[1] = static_cast<const uint8_t*>(a->v);
+    p.scale[0] = static_cast<const float*>(a->k_scale); p.scale[1] = static_cast<const float*>(a->v_scale);
+    p.out[0] = static_cast<uint8_t*>(a->out_k); p.out[1] = static_cast<uint8_t*>(a->out_v);
+    p.out_scale[0] = static_cast<float*>(a->out_k_scale); p.out_scale[1] = static_cast<float*>(a->out_v_scale);
+    for (int i = 0; i < 3; ++i) { p.hs[0][i] = a->k_stride[i]; p.hs[1][i] = a->v_stride[i]; p.os[0][i] = a->out_k_stride[i]; p.os[1][i] = a->out_v_stride[i]; }
+    p.weights = static_cast<const float*>(a->weights); p.out_weights = static_cast<float*>(a->out_weights);
+    p.lengths = a->lengths; p.positions = a->positions; p.out_lengths = a->out_lengths; p.out_positions = a->out_positions;
+    p.source = static_cast<int*>(a->ws);
+    p.rows = a->rows; p.blocks = a->rows / a->block; p.out_rows = a->out_rows; p.out_blocks = a->out_rows / a->out_block; p.block = a->block; p.out_block = a->out_block;
+    p.kv_heads = a->kv_heads; p.dim = a->head_dim; p.keep = a->keep; p.sinks = a->sinks; p.recent = a->recent;
+    int rc = launch("evict_select_kernel", q8::evict_select_kernel, dim3(a->episodes), dim3(q8::SELECT_THREADS), 0, S(stream), p);
+    if (rc) return rc;
+    return launch("evict_move_kernel", q8::evict_move_kernel, dim3((a->keep + a->out_block - 1) / a->out_block * a->kv_heads, 2, a->episodes), dim3(q8::MOVE_THREADS), 0, S(stream), p);
+}
+
+}  // extern "C"

@@ -1,0 +1,257 @@
+// The 8-bit KV cache: e4m3 values with one power-of-two scale per block of rows and K/V head.
+//
+//   value = e4m3 * scale,   scale = the smallest power of two s with amax(block) <= 448 s   (at least 2^-120)
+//
+// e4m3 is a floating format: a power-of-two scale loses none of its precision (it only moves the exponents), and division by it is exact, so a value
+// is rounded once, to e4m3, and a block whose scale has to grow later moves its old values by a power of two, exact down to the subnormals.
+// Values that are not finite are held as NaN and do not take part in amax.
+#pragma once
+
+#include "common.cuh"
+
+namespace fvla {
+namespace q8 {
+
+constexpr int kMinExponent = -120;
+
+// Bits of the scale for a block whose largest finite |bf16 value| has the bits `amax` (bf16, sign cleared).
+// 448 = 1.75 * 2^8: an amax of m * 2^x (1 <= m < 2) needs 2^(x-8) up to m = 1.75 and 2^(x-7) above it.
+__device__ __forceinline__ float scale_of(uint32_t amax) {
+    const int x = (int)(amax >> 7) - 127;                       // a subnormal amax lands far below the smallest scale
+    const int e = x - ((amax & 0x7fu) <= 0x60u ? 8 : 7);
+    return __int_as_float((max(e, kMinExponent) + 127) << 23);
+}
+// 1 / s of a power of two s within [2^-120, 2^121].
+__device__ __forceinline__ float inverse_pow2(float s) { return __int_as_float((254 << 23) - __float_as_int(s)); }
+
+__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float2 from_e4m3x2(uint32_t pair) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)pair));
+    float2 f;
+    asm("{.reg .f16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;}" : "=f"(f.x), "=f"(f.y) : "r"(h));
+    return f;
+}
+// Two bf16 values over a power of two -> e4m3 pair; what is not finite becomes NaN (0x7f).
+__device__ __forceinline__ uint32_t quantize_pair(uint32_t bf, float inv) {
+    const float2 f = unpack_bf16x2(bf);
+    uint32_t r = to_e4m3x2(f.x * inv, f.y * inv);
+    if ((bf & 0x7f80u) == 0x7f80u) r = (r & 0xff00u) | 0x7fu;
+    if ((bf & 0x7f800000u) == 0x7f800000u) r = (r & 0x00ffu) | 0x7f00u;
+    return r;
+}
+// Four e4m3 values times a power of two, rounded again.
+__device__ __forceinline__ uint32_t rescale4(uint32_t v, float ratio) {
+    const float2 a = from_e4m3x2(v & 0xffffu), b = from_e4m3x2(v >> 16);
+    return to_e4m3x2(a.x * ratio, a.y * ratio) | (to_e4m3x2(b.x * ratio, b.y * ratio) << 16);
+}
+__device__ __forceinline__ uint32_t amax_pair(uint32_t amax, uint32_t bf) {
+    const uint32_t lo = bf & 0x7fffu, hi = (bf >> 16) & 0x7fffu;
+    if (lo < 0x7f80u) amax = max(amax, lo);
+    if (hi < 0x7f80u) amax = max(amax, hi);
+    return amax;
+}
+
+struct AppendArgs {
+    const bf16* x[2];                 // new K, V rows (episodes, tokens, kv_heads, dim)
+    uint8_t* held[2];                 // cache
+    float* scale[2];                  // (episodes, blocks, kv_heads)
+    long long xs[2][3], hs[2][3];     // strides in elements: episode, row, head
+    const int *starts, *counts;
+    int* status;
+    int tokens, rows, blocks, block, kv_heads, dim;
+};
+
+constexpr int APPEND_THREADS = 128;
+
+// One CTA per (block that a run of new rows can touch and head, K or V, episode): its new rows' amax, the scale, then old rows moved to that scale
+// and new rows rounded. A thread takes 16 values at a time (32 bytes in, 16 out).
+__global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const AppendArgs p) {
+    __shared__ uint32_t warp_max[APPEND_THREADS / 32];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int e = blockIdx.z, kv = blockIdx.y, head = blockIdx.x % p.kv_heads, w = blockIdx.x / p.kv_heads;
+    const long long start = p.starts[e];
+    const int count = p.counts ? min(max(p.counts[e], 0), p.tokens) : p.tokens;
+    if (count > 0 && (start < 0 || start + count > p.rows) && threadIdx.x == 0 && blockIdx.x == 0 && kv == 0 && p.status) atomicExch(p.status, 8);
+    const long long from = max(start, 0ll), to = min(start + count, (long long)p.rows);      // rows outside the cache are left out
+    if (from >= to) return;
+    const long long b = from / p.block + w, row0 = b * p.block;
+    if (row0 >= to) return;
+    const int first = (int)(max(from, row0) - row0), last = (int)(min(to, row0 + p.block) - row0);     // new rows of this block
+    const int old = from > row0 ? first : 0;                                                           // rows that were there before
+    const int chunks = p.dim / 16;
+    const bf16* x = p.x[kv] + e * p.xs[kv][0] + (row0 - start) * p.xs[kv][1] + head * p.xs[kv][2];
+    uint8_t* held = p.held[kv] + e * p.hs[kv][0] + row0 * p.hs[kv][1] + head * p.hs[kv][2];
+    float* scale = p.scale[kv] + ((size_t)e * p.blocks + b) * p.kv_heads + head;
+
+    uint32_t amax = 0;
+    for (int i = first * chunks + threadIdx.x; i < last * chunks; i += APPEND_THREADS) {
+        const uint4* src = reinterpret_cast<const uint4*>(x + (long long)(i / chunks) * p.xs[kv][1] + (i % chunks) * 16);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint4 u = __ldg(src + h);
+            amax = amax_pair(amax_pair(amax_pair(amax_pair(amax, u.x), u.y), u.z), u.w);
+        }
+    }
+    amax = __reduce_max_sync(0xffffffffu, amax);
+    if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = amax;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < APPEND_THREADS / 32; ++i) amax = max(amax, warp_max[i]);
+    const float needed = scale_of(amax), was = old > 0 ? *scale : 0.f, now = fmaxf(was, needed);
+    __syncthreads();                                             // every thread has read the old scale
+    if (threadIdx.x == 0) *scale = now;
+    if (now != was) {
+        const float ratio = was * inverse_pow2(now);
+        for (int i = threadIdx.x; i < old * chunks; i += APPEND_THREADS) {
+            uint4* at = reinterpret_cast<uint4*>(held + (long long)(i / chunks) * p.hs[kv][1] + (i % chunks) * 16);
+            uint4 u = *at;
+            *at = make_uint4(rescale4(u.x, ratio), rescale4(u.y, ratio), rescale4(u.z, ratio), rescale4(u.w, ratio));
+        }
+    }
+    const float inv = inverse_pow2(now);
+    for (int i = first * chunks + threadIdx.x; i < last * chunks; i += APPEND_THREADS) {
+        const uint4* src = reinterpret_cast<const uint4*>(x + (long long)(i / chunks) * p.xs[kv][1] + (i % chunks) * 16);
+        uint32_t o[4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint4 u = __ldg(src + h);
+            o[2 * h] = quantize_pair(u.x, inv) | (quantize_pair(u.y, inv) << 16);
+            o[2 * h + 1] = quantize_pair(u.z, inv) | (quantize_pair(u.w, inv) << 16);
+        }
+        *reinterpret_cast<uint4*>(held + (long long)(i / chunks) * p.hs[kv][1] + (i % chunks) * 16) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ eviction
+struct EvictArgs {
+    const uint8_t* held[2];
+    const float* scale[2];
+    uint8_t* out[2];
+    float* out_scale[2];
+    long long hs[2][3], os[2][3];     // strides in elements: episode, row, head
+    const float* weights;             // (episodes, rows)
+    float* out_weights;               // (episodes, out_rows), may be null
+    const int *lengths, *positions;   // positions (episodes, rows), may be null: row numbers
+    int *out_lengths, *out_positions; // (episodes), (episodes, out_rows; may be null)
+    int* source;                      // scratch (episodes, keep): the rows that stay, in order
+    int rows, blocks, out_rows, out_blocks, block, out_block, kv_heads, dim, keep, sinks, recent;
+};
+
+constexpr int SELECT_THREADS = 1024;
+
+// Order of weights as unsigned integers: larger is kept first. NaN counts as -infinity, -0 as 0.
+__device__ __forceinline__ uint32_t order_of(float w) {
+    if (w != w) w = -INFINITY;
+    const uint32_t u = __float_as_uint(w + 0.f);                // -0 + 0 = +0
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// One CTA per episode: the threshold by a radix select of 8 bits at a time, then one ordered pass that writes the rows which stay.
+__global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const EvictArgs p) {
+    __shared__ uint32_t hist[256];
+    __shared__ uint32_t s_prefix, s_left;
+    __shared__ int warp_sum[2][SELECT_THREADS / 32];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int e = blockIdx.x, tid = threadIdx.x;
+    const int L = min(max(p.lengths[e], 0), p.rows);
+    const int n = min(L, p.keep);
+    const float* w = p.weights + (size_t)e * p.rows;
+    const int low = min(p.sinks, L), high = max(low, L - p.recent);       // rows [low, high) compete
+    const int wanted = n - low - (L - high);                              // and so many of them stay (sinks + recent <= keep)
+    uint32_t threshold = 0, ties = 0;
+    if (L > p.keep && wanted > 0) {
+        uint32_t prefix = 0, left = wanted;
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            for (int i = tid; i < 256; i += SELECT_THREADS) hist[i] = 0;
+            __syncthreads();
+            for (int j = low + tid; j < high; j += SELECT_THREADS) {
+                const uint32_t u = order_of(w[j]);
+                if (shift == 24 || (u >> (shift + 8)) == prefix) atomicAdd(&hist[(u >> shift) & 255u], 1u);
+            }
+            __syncthreads();
+            if (tid == 0) {
+                uint32_t d = 255, above = 0;
+                while (d > 0 && above + hist[d] < left) above += hist[d--];
+                s_prefix = (prefix << 8) | d;
+                s_left = left - above;
+            }
+            __syncthreads();
+            prefix = s_prefix;
+            left = s_left;
+        }
+        threshold = prefix;
+        ties = left;                                                      // so many rows of exactly this weight stay, the first ones
+    }
+    int kept = 0, equal = 0;                                              // before this round of rows
+    for (int j0 = 0; j0 < L; j0 += SELECT_THREADS) {
+        const int j = j0 + tid;
+        const bool inside = j < L, free = inside && j >= low && j < high && L > p.keep;
+        const uint32_t u = free ? order_of(w[j]) : 0;
+        const bool tie = free && wanted > 0 && u == threshold;
+        const uint32_t tie_mask = __ballot_sync(0xffffffffu, tie);
+        if ((tid & 31) == 0) warp_sum[0][tid >> 5] = __popc(tie_mask);
+        __syncthreads();
+        int tie_rank = equal + __popc(tie_mask & ((1u << (tid & 31)) - 1)), tie_all = 0;
+        for (int i = 0; i < SELECT_THREADS / 32; ++i) { if (i < (tid >> 5)) tie_rank += warp_sum[0][i]; tie_all += warp_sum[0][i]; }
+        const bool stays = inside && (!free || (wanted > 0 && (u > threshold || (tie && tie_rank < (int)ties))));
+        const uint32_t mask = __ballot_sync(0xffffffffu, stays);
+        if ((tid & 31) == 0) warp_sum[1][tid >> 5] = __popc(mask);
+        __syncthreads();
+        int rank = kept + __popc(mask & ((1u << (tid & 31)) - 1)), all = 0;
+        for (int i = 0; i < SELECT_THREADS / 32; ++i) { if (i < (tid >> 5)) rank += warp_sum[1][i]; all += warp_sum[1][i]; }
+        if (stays) {
+            p.source[(size_t)e * p.keep + rank] = j;
+            if (p.out_weights) p.out_weights[(size_t)e * p.out_rows + rank] = w[j];
+            if (p.out_positions) p.out_positions[(size_t)e * p.out_rows + rank] = p.positions ? p.positions[(size_t)e * p.rows + j] : j;
+        }
+        kept += all;
+        equal += tie_all;
+        __syncthreads();
+    }
+    if (tid == 0) p.out_lengths[e] = n;
+}
+
+constexpr int MOVE_THREADS = 128;
+
+// One CTA per (block of the result and head, K or V, episode): its scale is the largest of its rows' source scales; rows of another scale
+// are moved to it by a power of two.
+__global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const EvictArgs p) {
+    __shared__ int row_of[128];
+    __shared__ float scale_of_row[128];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int e = blockIdx.z, kv = blockIdx.y, head = blockIdx.x % p.kv_heads, b = blockIdx.x / p.kv_heads, tid = threadIdx.x;
+    const int n = min(min(max(p.lengths[e], 0), p.rows), p.keep);
+    const int row0 = b * p.out_block, have = min(p.out_block, n - row0);
+    if (have <= 0) return;
+    for (int i = tid; i < have; i += MOVE_THREADS) {
+        const int j = p.source[(size_t)e * p.keep + row0 + i];
+        row_of[i] = j;
+        scale_of_row[i] = p.scale[kv][((size_t)e * p.blocks + j / p.block) * p.kv_heads + head];
+    }
+    __syncthreads();
+    float now = 0.f;
+    for (int i = 0; i < have; ++i) now = fmaxf(now, scale_of_row[i]);
+    if (tid == 0) p.out_scale[kv][((size_t)e * p.out_blocks + b) * p.kv_heads + head] = now;
+    const float inv = inverse_pow2(now);
+    const int chunks = p.dim / 16;
+    const uint8_t* held = p.held[kv] + e * p.hs[kv][0] + head * p.hs[kv][2];
+    uint8_t* out = p.out[kv] + e * p.os[kv][0] + (long long)row0 * p.os[kv][1] + head * p.os[kv][2];
+    for (int i = tid; i < have * chunks; i += MOVE_THREADS) {
+        const int r = i / chunks, c = i % chunks;
+        uint4 u = __ldg(reinterpret_cast<const uint4*>(held + row_of[r] * p.hs[kv][1] + c * 16));
+        const float ratio = scale_of_row[r] * inv;
+        if (ratio != 1.f) u = make_uint4(rescale4(u.x, ratio), rescale4(u.y, ratio), rescale4(u.z, ratio), rescale4(u.w, ratio));
+        *reinterpret_cast<uint4*>(out + r * p.os[kv][1] + c * 16) = u;
+    }
+}
+
+}  // namespace q8
+}  // namespace fvla

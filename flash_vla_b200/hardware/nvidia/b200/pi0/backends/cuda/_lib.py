@@ -50,7 +50,33 @@ class DecoderBatchLayers(ctypes.Structure):
                 [(n, _I) for n in ("episodes", "tokens", "prefix", "first", "last", "layers")])
 
 
-# name -> argument ctypes (every function returns int except the three queries below)
+_L3 = ctypes.c_longlong * 3
+
+
+class Attention(ctypes.Structure):
+    """`struct fvla_attention` of the header."""
+    _fields_ = ([(n, _P) for n in ("q", "k", "v", "k_scale", "v_scale", "out", "lse", "weights", "ws", "prefix", "q_lens", "k_lens", "q_start",
+                                   "q_docs", "k_docs", "k_pos", "slopes")] + [("ws_bytes", _Z)] +
+                [(n, _L3) for n in ("q_stride", "k_stride", "v_stride", "out_stride")] + [(n, _F) for n in ("scale", "cap", "decay")] +
+                [(n, _I) for n in ("episodes", "tokens", "keys", "heads", "kv_heads", "head_dim", "block", "causal")])
+
+
+class CacheAppend(ctypes.Structure):
+    """`struct fvla_cache_append_args` of the header."""
+    _fields_ = ([(n, _P) for n in ("k", "v", "k_held", "v_held", "k_scale", "v_scale", "starts", "counts")] +
+                [(n, _L3) for n in ("k_stride", "v_stride", "k_held_stride", "v_held_stride")] +
+                [(n, _I) for n in ("episodes", "tokens", "rows", "kv_heads", "head_dim", "block")])
+
+
+class CacheEvict(ctypes.Structure):
+    """`struct fvla_cache_evict_args` of the header."""
+    _fields_ = ([(n, _P) for n in ("k", "v", "k_scale", "v_scale", "weights", "out_k", "out_v", "out_k_scale", "out_v_scale", "out_weights", "ws",
+                                   "lengths", "positions", "out_lengths", "out_positions")] + [("ws_bytes", _Z)] +
+                [(n, _L3) for n in ("k_stride", "v_stride", "out_k_stride", "out_v_stride")] +
+                [(n, _I) for n in ("episodes", "rows", "out_rows", "kv_heads", "head_dim", "block", "out_block", "keep", "sinks", "recent")])
+
+
+# name -> argument ctypes (every function returns int except the queries below)
 SIGNATURES: dict[str, list] = {
     "fvla_vision_patch_embed": [_P, _P, _P, _P, _P, _I, _P, _Z, _P],
     "fvla_vision_patch_embed_noalloc": [_P, _P, _P, _P, _P, _I, _P],
@@ -77,6 +103,9 @@ SIGNATURES: dict[str, list] = {
     "fvla_encoder_layers_run": [ctypes.POINTER(EncoderLayers), _P],
     "fvla_embed_rows": [_P, _P, _P, _I, _I, ctypes.c_longlong, _P],
     "fvla_convert_copy": [_P, _I, _P, _I, _P, _Z, _P],
+    "fvla_attention_run": [ctypes.POINTER(Attention), _P],
+    "fvla_cache_append": [ctypes.POINTER(CacheAppend), _P],
+    "fvla_cache_evict": [ctypes.POINTER(CacheEvict), _P],
     "fvla_selftest_wait_timeout": [_P, _P, _P, _I, _I, _I, ctypes.c_uint, _P],
     "fvla_gemm_plan_set": [_I, _I, _I, _I, _I, _I, _I],
     "fvla_gemm_plan_clear": [],
@@ -94,6 +123,8 @@ QUERIES: dict[str, tuple] = {
     "fvla_decoder_attention_workspace_bytes": ([_I, _I], c_size_t),
     "fvla_encoder_attention_workspace_bytes": ([_I, _I], c_size_t),
     "fvla_patch_embed_workspace_bytes": ([_I], c_size_t),
+    "fvla_attention_workspace_bytes": ([ctypes.POINTER(Attention)], c_size_t),
+    "fvla_cache_evict_workspace_bytes": ([_I, _I], c_size_t),
 }
 
 _lib = None

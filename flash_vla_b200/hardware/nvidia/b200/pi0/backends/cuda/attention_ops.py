@@ -1,0 +1,307 @@
+"""Attention with masks, caps and biases, and the 8-bit KV cache: call sites without a counterpart in the reference.
+
+The reference's attentions (`kernels/attention.py:20-34`, `fused_wrappers.py:88-115`) have one shape and one mask each. These take batches of
+episodes of different lengths, grouped heads and the masks and score functions of other language backbones, and read the cache
+either in bf16 or as e4m3 values with a power-of-two scale for each block of rows and K/V head (`QuantizedCache`). A server's step is
+`cache_append`, then `cache_attention`; `cache_attention(..., weights=w)` adds up what weight each key received, by which
+`cache_evict` later picks the rows that stay.
+
+Conventions of `wrappers.py`: torch tensors in, destinations passed in and written in place, checks on the host, one call into
+libfvla_b200 on torch's current stream. Tensors are (episodes, tokens, heads, head_dim) with a contiguous last axis and otherwise any strides that
+start every row on 16 bytes; lengths, starts, positions and document ids are int32 on the device, contiguous. They are not read on the host: lengths
+outside a tensor are clamped on the device. Scratch comes from the active `ScratchPool` of a program that installed one (`use_pool`, `set_pool`),
+whose captured graph then owns it; without one it is allocated for the call, from a graph's own memory during a capture.
+"""
+from __future__ import annotations
+
+import ctypes
+import functools
+import math
+
+import torch
+
+from . import _lib
+from . import wrappers as _w
+
+BLOCKS = (16, 32, 64, 128)      # rows per scale of an 8-bit cache
+_INT32, _F32 = torch.int32, torch.float32
+
+
+def _rows(name, shape, stride, dtype, want, multiple, overlap_ok=True):
+    """Element strides (episode, token, head) of a 4-D operand; an axis of one element gets a stride that any layout may have."""
+    if dtype != want:
+        raise ValueError(f"{name}: expected {want}, got {dtype}")
+    if len(shape) != 4:
+        raise ValueError(f"{name}: expected (episodes, tokens, heads, head_dim), got shape {tuple(shape)}")
+    if shape[3] > 1 and stride[3] != 1:
+        raise ValueError(f"{name}: the head dimension must be contiguous, got strides {tuple(stride)}")
+    out = []
+    for size, s in zip(shape[:3], stride[:3]):
+        if size <= 1:
+            s = 256
+        if s % multiple:
+            raise ValueError(f"{name}: rows must start on 16 bytes, got strides {tuple(stride)}")
+        if s == 0 and not overlap_ok:
+            raise ValueError(f"{name}: a destination whose rows share memory, strides {tuple(stride)}")
+        out.append(s)
+    return out
+
+
+def _cache_shapes(name, shapes, strides, dtypes):
+    """Block size of a QuantizedCache whose four tensors have these shapes, strides and types."""
+    k, v, ks, vs = shapes
+    if tuple(k) != tuple(v) or tuple(ks) != tuple(vs):
+        raise ValueError(f"{name}: K and V must have one shape, got {tuple(k)} {tuple(v)}, scales {tuple(ks)} {tuple(vs)}")
+    if len(k) != 4 or len(ks) != 3 or ks[0] != k[0] or ks[2] != k[2]:
+        raise ValueError(f"{name}: expected K (episodes, rows, kv_heads, head_dim) and scales (episodes, blocks, kv_heads), got {tuple(k)} and {tuple(ks)}")
+    if ks[1] == 0 or k[1] % ks[1] or k[1] // ks[1] not in BLOCKS:
+        raise ValueError(f"{name}: {k[1]} rows in {ks[1]} blocks (blocks of {BLOCKS} rows)")
+    for t, dt in zip(("K_scale", "V_scale"), dtypes[2:]):
+        if dt != _F32:
+            raise ValueError(f"{name}.{t}: expected {_F32}, got {dt}")
+    for t, s in zip(("K_scale", "V_scale"), strides[2:]):
+        if any(n > 1 and a != b for n, a, b in zip(ks, s, (ks[1] * ks[2], ks[2], 1))):
+            raise ValueError(f"{name}.{t}: expected a contiguous tensor, got strides {tuple(s)}")
+    if k[3] % 16 or not 0 < k[3] <= 256:
+        raise ValueError(f"{name}: head_dim {k[3]} (a multiple of 16 up to 256)")
+    return k[1] // ks[1]
+
+
+def _layout(t):
+    return t.shape, t.stride(), t.dtype
+
+
+def _cache_layout(c):
+    return tuple(t.shape for t in c), tuple(t.stride() for t in c), tuple(t.dtype for t in c)
+
+
+@functools.lru_cache(maxsize=1024)
+def _attention_plan(q, k, v, out, cache):
+    """(argument block without addresses, scratch bytes) of an attention with operands of these layouts; `cache`: layout of a QuantizedCache, or None."""
+    a = _lib.Attention()
+    if cache is None:
+        multiple, want, dim_multiple = 8, torch.bfloat16, 8
+    else:
+        a.block = _cache_shapes("cache", *cache)
+        multiple, want, dim_multiple = 16, torch.float8_e4m3fn, 16
+        k, v = ((cache[0][i], cache[1][i], cache[2][i]) for i in (0, 1))
+    a.q_stride[:] = _rows("Q", *q, torch.bfloat16, 8)
+    a.k_stride[:] = _rows("K", *k, want, multiple)
+    a.v_stride[:] = _rows("V", *v, want, multiple)
+    a.out_stride[:] = _rows("out", *out, torch.bfloat16, 8, overlap_ok=False)
+    (E, T, H, D), (_, S, HK, _) = q[0], k[0]
+    if tuple(k[0]) != (E, S, HK, D) or tuple(v[0]) != (E, S, HK, D) or tuple(out[0]) != (E, T, H, D):
+        raise ValueError(f"attention: shapes do not fit: Q {tuple(q[0])}, K {tuple(k[0])}, V {tuple(v[0])}, out {tuple(out[0])}")
+    if D % dim_multiple or not 0 < D <= 256:
+        raise ValueError(f"attention: head_dim {D} (a multiple of {dim_multiple} up to 256)")
+    if HK == 0 or H % HK or not 0 < H // HK <= 128:
+        raise ValueError(f"attention: {H} query heads over {HK} K/V heads")
+    if T * H >= 1 << 31 or E * HK >= 1 << 16 or S >= 1 << 31 or E >= 1 << 16:
+        raise ValueError(f"attention: {E} episodes of {T} queries of {H} heads over {S} keys: too many")
+    a.episodes, a.tokens, a.keys, a.heads, a.kv_heads, a.head_dim = E, T, S, H, HK, D
+    return a, _lib.load().fvla_attention_workspace_bytes(ctypes.byref(a)) if E and T else 0
+
+
+def _vector(name, t, shape, dtype, device):
+    """Address of an optional small operand. (Without a GPU the large operands, which come last, are the ones refused for their device.)"""
+    if t is None:
+        return None
+    if t.dtype != dtype:
+        raise ValueError(f"{name}: expected {dtype}, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous tensor, got strides {t.stride()}")
+    if t.get_device() != device and device >= 0:
+        raise ValueError(f"{name}: expected a tensor on the current CUDA device, got {t.device}")
+    return t.data_ptr()
+
+
+def _address(name, t, device):
+    """Address of an operand whose layout has been checked."""
+    if t.get_device() != device:
+        raise ValueError(f"{name}: expected a CUDA tensor on the current device, got {t.device}")
+    p = t.data_ptr()
+    if p & 15:
+        raise ValueError(f"{name}: expected 16-byte alignment")
+    return p
+
+
+def _device():
+    return torch._C._cuda_getDevice() if torch.cuda.is_available() else -2      # -1 is the CPU's number
+
+
+def _scratch(role, nbytes, like):
+    if not nbytes:
+        return None
+    if _w.default_pool():
+        return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+    return _w.scratch(role, (nbytes,), torch.uint8, like.device)
+
+
+def _copy(struct):
+    return type(struct).from_buffer_copy(struct)
+
+
+def _attend(Q, K, V, cache, scale, out, causal, prefix, q_lens, k_lens, q_start, q_docs, k_docs, k_pos, cap, slopes, lse, weights, decay):
+    plan, nbytes = _attention_plan(_layout(Q), None if cache else _layout(K), None if cache else _layout(V), _layout(out), _cache_layout(cache) if cache else None)
+    E, T, S, H = plan.episodes, plan.tokens, plan.keys, plan.heads
+    scale, cap, decay = float(scale), float(cap or 0.0), float(decay)
+    if not math.isfinite(scale) or not (0.0 <= cap < math.inf) or not math.isfinite(decay):
+        raise ValueError(f"attention: scale {scale}, cap {cap}, decay {decay}: finite numbers, the cap not negative")
+    if prefix is not None and not causal:
+        raise ValueError("attention: a prefix without the causal mask")
+    if (q_docs is None) != (k_docs is None):
+        raise ValueError("attention: documents of queries and keys, or of neither")
+    device, a = _device(), _copy(plan)
+    a.prefix, a.q_lens = _vector("prefix", prefix, (E,), _INT32, device), _vector("q_lens", q_lens, (E,), _INT32, device)
+    a.k_lens, a.q_start = _vector("k_lens", k_lens, (E,), _INT32, device), _vector("q_start", q_start, (E,), _INT32, device)
+    a.q_docs, a.k_docs = _vector("q_docs", q_docs, (E, T), _INT32, device), _vector("k_docs", k_docs, (E, S), _INT32, device)
+    a.k_pos, a.slopes = _vector("k_pos", k_pos, (E, S), _INT32, device), _vector("slopes", slopes, (H,), _F32, device)
+    a.lse, a.weights = _vector("lse", lse, (E, H, T), _F32, device), _vector("weights", weights, (E, S), _F32, device)
+    a.scale, a.cap, a.decay, a.causal = scale, cap, decay, int(bool(causal))
+    a.q, a.out = _address("Q", Q, device), _address("out", out, device)
+    if cache:
+        a.k, a.v = _address("cache.K", cache[0], device), _address("cache.V", cache[1], device)
+        a.k_scale, a.v_scale = _vector("cache.K_scale", cache[2], cache[2].shape, _F32, device), _vector("cache.V_scale", cache[3], cache[3].shape, _F32, device)
+    else:
+        a.k, a.v = _address("K", K, device), _address("V", V, device)
+    if E == 0 or T == 0:
+        return out
+    if weights is not None:
+        if a.out == a.q:
+            raise ValueError("attention: the weights are taken from Q, which out would overwrite")
+        if lse is None:
+            held = _scratch("attention_lse", 4 * E * H * T, Q)
+            a.lse = held.data_ptr()
+    ws = _scratch("attention_ws", nbytes, Q)
+    if ws is not None:
+        a.ws, a.ws_bytes = ws.data_ptr(), nbytes
+    _lib.call("fvla_attention_run", ctypes.byref(a), _w._stream())
+    return out
+
+
+def masked_attention(Q, K, V, scale, out, causal=False, prefix=None, q_lens=None, k_lens=None, q_docs=None, k_docs=None, cap=0.0, slopes=None,
+                     lse=None):
+    """out = softmax(bias(cap(scale * Q K^T))) V over the keys that each query sees.
+
+    Q, out (E, T, H, D); K, V (E, S, HK, D), H a multiple of HK; bf16, D a multiple of 8 up to 256. `out` may be Q.
+    cap > 0: scores become cap * tanh(score / cap). slopes (H,) fp32: slope * |distance| is taken off them.
+    k_lens, q_lens (E,): keys and queries of each episode, all by default; rows of `out` (and of `lse`) behind q_lens stay as they were. The queries are the
+    last tokens of their episode: token t stands at k_lens - q_lens + t.
+    causal: a query sees keys up to its own position; prefix (E,): and all of the first `prefix` keys.
+    q_docs (E, T), k_docs (E, S): a query sees the keys of its own document; negative ids are padding.
+    A query that sees no key gets zeros. lse (E, H, T) fp32 receives the natural log-sum-exp of the scores, -inf for such a query.
+    One new token per episode (T = 1) is the same call. K and V behind k_lens, or under a negative document id, may hold anything."""
+    return _attend(Q, K, V, None, scale, out, causal, prefix, q_lens, k_lens, None, q_docs, k_docs, None, cap, slopes, lse, None, 1.0)
+
+
+def cache_attention(Q, cache, lengths, scale, out, causal=False, prefix=None, q_lens=None, q_start=None, k_pos=None, cap=0.0, slopes=None, lse=None,
+                    weights=None, decay=1.0):
+    """`masked_attention` over a `QuantizedCache` of which each episode has `lengths` (E,) rows, the queries' own among them.
+
+    q_start (E,): position of each episode's first query, by default lengths - q_lens. k_pos (E, rows): position of each cached row, by default its
+    number; a cache that `cache_evict` has thinned out needs both for `causal`, `prefix` (then positions below `prefix`) and `slopes`.
+    weights (E, rows) fp32: weights = decay * weights + the probability mass that each row received from all queries and heads; rows
+    behind `lengths` stay as they were. decay = 0 overwrites. `out` may be Q, unless weights are asked for."""
+    cache = tuple(cache)
+    return _attend(Q, None, None, cache, scale, out, causal, prefix, q_lens, lengths, q_start, None, None, k_pos, cap, slopes, lse, weights, decay)
+
+
+@functools.lru_cache(maxsize=1024)
+def _append_plan(k, v, cache):
+    a = _lib.CacheAppend()
+    a.block = _cache_shapes("cache", *cache)
+    a.k_stride[:] = _rows("K", *k, torch.bfloat16, 8)
+    a.v_stride[:] = _rows("V", *v, torch.bfloat16, 8)
+    for field, i in (("k_held_stride", 0), ("v_held_stride", 1)):
+        getattr(a, field)[:] = _rows("cache", cache[0][i], cache[1][i], cache[2][i], torch.float8_e4m3fn, 16, overlap_ok=False)
+    E, rows, HK, D = cache[0][0]
+    T = k[0][1]
+    if tuple(k[0]) != (E, T, HK, D) or tuple(v[0]) != (E, T, HK, D):
+        raise ValueError(f"cache_append: K {tuple(k[0])} and V {tuple(v[0])} do not fit a cache of {tuple(cache[0][0])}")
+    if T > rows:
+        raise ValueError(f"cache_append: {T} rows into a cache of {rows}")
+    if E >= 1 << 16 or rows >= 1 << 31 or HK == 0:
+        raise ValueError(f"cache_append: a cache of {tuple(cache[0][0])}")
+    a.episodes, a.tokens, a.rows, a.kv_heads, a.head_dim = E, T, rows, HK, D
+    return a
+
+
+def cache_append(K, V, cache, starts, counts=None):
+    """New rows K, V (E, T, kv_heads, head_dim) bf16 into rows starts[e] .. starts[e] + T - 1 of each episode's cache (counts[e] <= T of them).
+
+    The scale of a block is the smallest power of two that brings its new values into e4m3's range, or the block's own where that is larger and the
+    block holds rows before starts[e]; where it has grown, those rows are moved to it. Rows behind the new ones are taken to be unused. Values
+    that are not finite become NaN and leave the scale alone. Rows that would lie outside the cache are left out (device status 8)."""
+    cache = tuple(cache)
+    plan = _append_plan(_layout(K), _layout(V), _cache_layout(cache))
+    device, a = _device(), _copy(plan)
+    a.starts, a.counts = _vector("starts", starts, (plan.episodes,), _INT32, device), _vector("counts", counts, (plan.episodes,), _INT32, device)
+    a.k, a.v = _address("K", K, device), _address("V", V, device)
+    a.k_held, a.v_held = _address("cache.K", cache[0], device), _address("cache.V", cache[1], device)
+    a.k_scale, a.v_scale = _vector("cache.K_scale", cache[2], cache[2].shape, _F32, device), _vector("cache.V_scale", cache[3], cache[3].shape, _F32, device)
+    if plan.episodes and plan.tokens:
+        _lib.call("fvla_cache_append", ctypes.byref(a), _w._stream())
+
+
+@functools.lru_cache(maxsize=1024)
+def _evict_plan(cache, out, keep, sinks, recent):
+    a = _lib.CacheEvict()
+    a.block, a.out_block = _cache_shapes("cache", *cache), _cache_shapes("out_cache", *out)
+    for name, layout, fields in (("cache", cache, ("k_stride", "v_stride")), ("out_cache", out, ("out_k_stride", "out_v_stride"))):
+        for i, field in enumerate(fields):
+            getattr(a, field)[:] = _rows(name, layout[0][i], layout[1][i], layout[2][i], torch.float8_e4m3fn, 16, overlap_ok=name == "cache")
+    E, rows, HK, D = cache[0][0]
+    out_rows = out[0][0][1]
+    if tuple(out[0][0]) != (E, out_rows, HK, D):
+        raise ValueError(f"cache_evict: rows of {tuple(cache[0][0])} into {tuple(out[0][0])}")
+    if not 0 < keep <= out_rows:
+        raise ValueError(f"cache_evict: {keep} rows to keep in a cache of {out_rows}")
+    if sinks < 0 or recent < 0 or sinks + recent > keep:
+        raise ValueError(f"cache_evict: the first {sinks} and the last {recent} rows in {keep}")
+    if E >= 1 << 16 or rows >= 1 << 31 or HK == 0:
+        raise ValueError(f"cache_evict: a cache of {tuple(cache[0][0])}")
+    a.episodes, a.rows, a.out_rows, a.kv_heads, a.head_dim, a.keep, a.sinks, a.recent = E, rows, out_rows, HK, D, keep, sinks, recent
+    return a, _lib.load().fvla_cache_evict_workspace_bytes(E, keep)
+
+
+def _span(t):
+    """First and last byte of a tensor's memory."""
+    return t.data_ptr(), t.data_ptr() + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) * t.element_size()
+
+
+def cache_evict(cache, lengths, weights, keep, out_cache, out_lengths, out_weights=None, positions=None, out_positions=None, sinks=0, recent=0):
+    """The rows of each episode that stay, in their order, into `out_cache` (another cache of at least `keep` rows).
+
+    min(lengths[e], keep) rows stay: the first `sinks`, the last `recent` and of the others those of the largest weight (weights (E, rows) fp32 as
+    `cache_attention` adds them up; equal weights: the first rows; NaN: as -inf). out_lengths (E,) receives their number; out_weights
+    (E, out rows) fp32 and out_positions (E, out rows) int32 what weight and position each had (positions (E, rows), or the row numbers). A block's
+    scale is the largest among its rows', and values are rounded again where theirs was smaller. What lies behind the last row stays as it was."""
+    cache, out_cache = tuple(cache), tuple(out_cache)
+    plan, nbytes = _evict_plan(_cache_layout(cache), _cache_layout(out_cache), int(keep), int(sinks), int(recent))
+    E, rows, out_rows = plan.episodes, plan.rows, plan.out_rows
+    device, a = _device(), _copy(plan)
+    a.lengths, a.out_lengths = _vector("lengths", lengths, (E,), _INT32, device), _vector("out_lengths", out_lengths, (E,), _INT32, device)
+    a.weights, a.out_weights = _vector("weights", weights, (E, rows), _F32, device), _vector("out_weights", out_weights, (E, out_rows), _F32, device)
+    a.positions, a.out_positions = _vector("positions", positions, (E, rows), _INT32, device), _vector("out_positions", out_positions, (E, out_rows), _INT32, device)
+    a.k, a.v = _address("cache.K", cache[0], device), _address("cache.V", cache[1], device)
+    a.out_k, a.out_v = _address("out_cache.K", out_cache[0], device), _address("out_cache.V", out_cache[1], device)
+    a.k_scale, a.v_scale = _vector("cache.K_scale", cache[2], cache[2].shape, _F32, device), _vector("cache.V_scale", cache[3], cache[3].shape, _F32, device)
+    a.out_k_scale = _vector("out_cache.K_scale", out_cache[2], out_cache[2].shape, _F32, device)
+    a.out_v_scale = _vector("out_cache.V_scale", out_cache[3], out_cache[3].shape, _F32, device)
+    if E == 0:
+        return
+    reads = [cache[0], cache[1], cache[2], cache[3], weights, lengths] + ([positions] if positions is not None else [])
+    writes = [*out_cache, out_lengths] + [t for t in (out_weights, out_positions) if t is not None]
+    spans = [_span(t) for t in reads]
+    for t in writes:
+        low, high = _span(t)
+        if any(low <= b and a_ <= high for a_, b in spans):
+            raise ValueError("cache_evict: a destination lies over what it is made of")
+    ws = _scratch("evict_ws", nbytes, weights)
+    a.ws, a.ws_bytes = ws.data_ptr(), nbytes
+    _lib.call("fvla_cache_evict", ctypes.byref(a), _w._stream())
+
+
+OPERATORS = {f.__name__: f for f in (masked_attention, cache_append, cache_attention, cache_evict)}

@@ -19,7 +19,7 @@ from flash_vla_b200.runtime.cuda import ScratchPool
 
 from . import _lib
 
-_POOL = ScratchPool()
+_POOL = _DEFAULT_POOL = ScratchPool()
 
 DECODER_HEADS = 8
 VISION_TOKENS = 256
@@ -121,6 +121,11 @@ def embed_prompt(table: torch.Tensor, ids: torch.Tensor, out: torch.Tensor) -> t
     if rows:
         _lib.call("fvla_embed_rows", _chk("table", table), ids.data_ptr(), _chk("out", out), rows, dim, vocab, _stream())
     return out
+
+
+def default_pool() -> bool:
+    """Whether no program has installed a pool of its own."""
+    return _POOL is _DEFAULT_POOL
 
 
 def scratch(role: str, shape, dtype, device) -> torch.Tensor:

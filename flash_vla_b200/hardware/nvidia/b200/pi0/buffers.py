@@ -18,8 +18,13 @@ shapes and bf16 dtype (`.../h100/pi0/buffers.py:26-64`) and adds what the B200 k
 
 RoPE tables: row r holds interleaved (cos, sin) of (offset + r) * 10000^(-2p/256), rounded
 to bf16 (`buffers.py:15-23`); the decoder's positions continue after the prefix.
+
+`QuantizedCache` is the 8-bit form of a K/V cache, for programs that keep long histories of many
+episodes; no buffer of the plan above has it.
 """
 from __future__ import annotations
+
+from typing import NamedTuple
 
 import torch
 
@@ -182,3 +187,24 @@ def allocate_static_buffers(num_views: int, chunk_size: int, prompt_len: int,
     buffers["encoder_rope_weights"].copy_(rope_table(S, 0, HEAD_DIM, device))
     buffers["decoder_rope_weights"].copy_(rope_table(D, S, HEAD_DIM, device))
     return buffers, S
+
+
+class QuantizedCache(NamedTuple):
+    """K/V cache of e4m3 values: row r of head h is K[e, r, h] * K_scale[e, r // block, h], scales powers of two. The block size is the number of rows
+    over the number of scales."""
+    K: torch.Tensor             # (episodes, rows, kv_heads, head_dim) float8_e4m3fn
+    V: torch.Tensor
+    K_scale: torch.Tensor       # (episodes, rows / block, kv_heads) fp32
+    V_scale: torch.Tensor
+
+
+def allocate_quantized_cache(episodes: int, rows: int, kv_heads: int, head_dim: int, device, block: int = 64) -> QuantizedCache:
+    """An empty cache with room for at least `rows` rows of each episode (whole blocks of 16, 32, 64 or 128 rows)."""
+    if block not in (16, 32, 64, 128):
+        raise ValueError(f"allocate_quantized_cache: blocks of {block} rows (16, 32, 64 or 128)")
+    if head_dim % 16 or not 0 < head_dim <= 256:
+        raise ValueError(f"allocate_quantized_cache: head_dim {head_dim} (a multiple of 16 up to 256)")
+    blocks = (rows + block - 1) // block
+    held = [torch.zeros(episodes, blocks * block, kv_heads, head_dim, dtype=torch.float8_e4m3fn, device=device) for _ in range(2)]
+    scales = [torch.ones(episodes, blocks, kv_heads, dtype=torch.float32, device=device) for _ in range(2)]
+    return QuantizedCache(*held, *scales)

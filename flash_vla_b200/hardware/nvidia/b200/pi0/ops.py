@@ -28,6 +28,8 @@ def op_table(fused: bool = True, backend: str = "cuda",
             table[name] = module.FUSED_WRAPPERS[name]
         elif name in module.ALL_WRAPPERS:
             table[name] = module.ALL_WRAPPERS[name]
+        elif name in module.OPERATORS:
+            table[name] = module.OPERATORS[name]
     if fused and set(plan.values()) <= {backend}:      # a stage stands for ops of one backend only
         table.update(BACKENDS[backend].STAGES)
     return SimpleNamespace(**table)
@@ -35,7 +37,7 @@ def op_table(fused: bool = True, backend: str = "cuda",
 
 def _op_names(backend: str) -> list[str]:
     module = BACKENDS[backend]
-    return sorted(set(module.ALL_WRAPPERS) | set(module.FUSED_WRAPPERS))
+    return sorted(set(module.ALL_WRAPPERS) | set(module.FUSED_WRAPPERS) | set(module.OPERATORS))
 
 
 def op_names(fused: bool = True, backend: str = "cuda") -> list[str]:

@@ -42,8 +42,8 @@ int fvla_abi_version(void);
  * count once, at capture time). Lets a caller report how much of a pass ran in these kernels. */
 unsigned long long fvla_launch_count(void);
 /* Health word of the current device: 0, or a small positive code once a kernel gave up on one of its
- * bounded waits (1..6: which kernel; its output is then invalid) or met a bad token id (7). Reading
- * clears the word. Negative: error code. This one call synchronises `stream`. */
+ * bounded waits (1..6 and 9: which kernel; its output is then invalid), met a bad token id (7) or rows that
+ * do not fit a cache (8). Reading clears the word. Negative: error code. This one call synchronises `stream`. */
 int fvla_device_status(void* stream);
 /* No counterpart in the reference (which has no device-side error reporting, only Python exceptions).
  * Failure-detection self-test: runs the decoder's cluster GEMM (out += x(M,K) @ W(K,N), all bf16, a
@@ -300,6 +300,61 @@ int fvla_convert_copy(const void* src, int src_is_f32, void* dst, int dst_is_f32
  * outside [0, vocab) gives a zero row and makes fvla_device_status report 7. */
 int fvla_embed_rows(const void* table, const long long* ids, void* out, int rows, int dim,
                     long long vocab, void* stream);
+
+/* ---- Attention with masks, caps and biases; the 8-bit KV cache (no counterpart in the reference) -----------------
+ * Strides are in elements and in the order episode, token (row), head; the head dimension is contiguous. Every row has to
+ * start on 16 bytes. Optional pointers are NULL where they do not apply. Lengths are clamped to the tensors on the device.
+ *
+ *   s = scale q.k;  cap > 0: s = cap tanh(s / cap);  slopes: s -= slopes[head] |p - kp|;  out = softmax(s) v
+ *
+ * Token t of an episode stands at p = q_start[e] + t, or k_lens[e] - q_lens[e] + t; key j at kp = k_pos[e][j], or j. A query sees key
+ * j < k_lens[e]; with `causal` only where kp <= max(p, prefix[e] - 1); with documents only where q_docs[e][t] == k_docs[e][j] >= 0. A query that
+ * sees nothing gets zeros and a log-sum-exp of -infinity; rows behind q_lens[e] stay as they were. With k_scale / v_scale (fp32 powers of two,
+ * (episodes, keys / block, kv_heads) contiguous; block 16, 32, 64 or 128) k and v hold e4m3 values, else bf16. lse: (episodes, heads,
+ * tokens) fp32. weights: (episodes, keys) fp32, weights[e][j] = decay * weights[e][j] + the probabilities that key j < k_lens[e] got from all queries;
+ * needs lse. What a query does not see may hold any bits, infinities and NaN among them, where no query of its 128-row tile sees it: rows behind
+ * k_lens, and rows of a negative document. head_dim: a multiple of 8 (e4m3: 16) up to 256; up to 128 query heads per K/V head. */
+struct fvla_attention {
+    const void *q, *k, *v, *k_scale, *v_scale;
+    void *out, *lse, *weights, *ws;
+    const int *prefix, *q_lens, *k_lens, *q_start, *q_docs, *k_docs, *k_pos;
+    const float* slopes;
+    size_t ws_bytes;
+    long long q_stride[3], k_stride[3], v_stride[3], out_stride[3];
+    float scale, cap, decay;
+    int episodes, tokens, keys, heads, kv_heads, head_dim, block, causal;
+};
+size_t fvla_attention_workspace_bytes(const struct fvla_attention* args);
+int fvla_attention_run(const struct fvla_attention* args, void* stream);
+
+/* Rows [0, counts[e]) (NULL: all) of k and v (episodes, tokens, kv_heads, head_dim) bf16 into rows starts[e].. of the cache. A block's scale is the
+ * smallest power of two s, at least 2^-120, with |new values| <= 448 s, or the block's own scale where that is larger and the block holds rows
+ * before starts[e]; those rows move to a scale that has grown. Values that are not finite are held as NaN and have no part in the
+ * scale. Rows that do not fit the cache are left out, and fvla_device_status reports 8. */
+struct fvla_cache_append_args {
+    const void *k, *v;
+    void *k_held, *v_held, *k_scale, *v_scale;
+    const int *starts, *counts;
+    long long k_stride[3], v_stride[3], k_held_stride[3], v_held_stride[3];
+    int episodes, tokens, rows, kv_heads, head_dim, block;
+};
+int fvla_cache_append(const struct fvla_cache_append_args* args, void* stream);
+
+/* The rows of each episode that stay, in their order, into another cache: min(lengths[e], keep) of them, the first `sinks`, the last `recent` and of
+ * the others those of the largest weight (ties: the first rows; NaN counts as -infinity). Scale of a block of the result: the largest of its rows'.
+ * out_weights and out_positions (episodes, out_rows) get the rows' weights and positions (positions, or the row numbers); both may be NULL. ws:
+ * fvla_cache_evict_workspace_bytes, any contents. The two caches must not overlap. */
+struct fvla_cache_evict_args {
+    const void *k, *v, *k_scale, *v_scale, *weights;
+    void *out_k, *out_v, *out_k_scale, *out_v_scale, *out_weights, *ws;
+    const int *lengths, *positions;
+    int *out_lengths, *out_positions;
+    size_t ws_bytes;
+    long long k_stride[3], v_stride[3], out_k_stride[3], out_v_stride[3];
+    int episodes, rows, out_rows, kv_heads, head_dim, block, out_block, keep, sinks, recent;
+};
+size_t fvla_cache_evict_workspace_bytes(int episodes, int keep);
+int fvla_cache_evict(const struct fvla_cache_evict_args* args, void* stream);
 
 #ifdef __cplusplus
 }

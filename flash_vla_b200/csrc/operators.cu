@@ -38,10 +38,13 @@ static int check_attention(const struct fvla_attention* a) {
     FVLA_REQUIRE(aligned16(a->q) && aligned16(a->k) && aligned16(a->v) && aligned16(a->out), "attention: every tensor must be 16-byte aligned");
     FVLA_REQUIRE(strides_ok(a->q_stride, 8) && strides_ok(a->out_stride, 8) && strides_ok(a->k_stride, multiple) && strides_ok(a->v_stride, multiple),
                  "attention: every row must start on 16 bytes");
+    FVLA_REQUIRE((a->tokens == 1 || a->q_stride[1] > 0) && (a->heads == 1 || a->q_stride[2] > 0) && (a->keys <= 1 || (a->k_stride[1] > 0 && a->v_stride[1] > 0)),
+                 "attention: tokens or query heads that share their memory");
+    for (int i = 0; i < 3; ++i) FVLA_REQUIRE(a->q_stride[i] >= 0 && a->k_stride[i] >= 0 && a->v_stride[i] >= 0 && a->out_stride[i] >= 0, "attention: negative strides");
     FVLA_REQUIRE(!q8 || (block_ok(a->block) && a->keys % a->block == 0), "attention: blocks of %d rows in %d", a->block, a->keys);
     FVLA_REQUIRE((a->q_docs != nullptr) == (a->k_docs != nullptr), "attention: documents of queries and keys, or of neither");
     FVLA_REQUIRE(a->prefix == nullptr || a->causal, "attention: a prefix without the causal mask");
-    FVLA_REQUIRE(a->weights == nullptr || (a->lse != nullptr && a->k_docs == nullptr), "attention: weights need the log-sum-exp, and no documents");
+    FVLA_REQUIRE(a->weights == nullptr || (a->lse != nullptr && q8), "attention: weights need the 8-bit cache and the log-sum-exp");
     FVLA_REQUIRE(a->cap >= 0.f && a->scale == a->scale, "attention: scale and cap");
     FVLA_REQUIRE((long long)a->tokens * a->heads < (1ll << 31) && (long long)a->episodes * a->kv_heads < 65536, "attention: too many rows");
     return FVLA_OK;
@@ -67,19 +70,17 @@ using namespace fvla;
 extern "C" {
 
 size_t fvla_attention_workspace_bytes(const struct fvla_attention* a) {
-    (void)a;
-    return 0;
+    return check_attention(a) ? 0 : mattn::workspace_bytes(attention_args(a));
 }
 
 int fvla_attention_run(const struct fvla_attention* a, void* stream) {
     int rc = check_attention(a);
     if (rc) return rc;
     const mattn::Args p = attention_args(a);
-    const bool q8 = p.k_scale != nullptr;
-    const dim3 rows((unsigned)(((long long)p.episodes * p.tokens * p.heads + 3) / 4)), keys((unsigned)(((long long)p.episodes * p.keys + 3) / 4));
-    rc = launch("attention_rows_kernel", q8 ? mattn::attention_rows_kernel<true> : mattn::attention_rows_kernel<false>, rows, dim3(128), 0, S(stream), p);
-    if (rc || p.weights == nullptr || p.keys == 0) return rc;
-    return launch("key_weights_kernel", q8 ? mattn::key_weights_kernel<true> : mattn::key_weights_kernel<false>, keys, dim3(128), 0, S(stream), p);
+    const size_t need = mattn::workspace_bytes(p);
+    if (need > 0 && (a->ws == nullptr || a->ws_bytes < need)) { set_error("attention: workspace of %zu bytes needed", need); return FVLA_ERR_WORKSPACE; }
+    FVLA_REQUIRE(aligned16(a->ws), "attention: the workspace must be 16-byte aligned");
+    return mattn::launch_attention(p, a->ws, device_status_ptr(), S(stream));
 }
 
 int fvla_cache_append(const struct fvla_cache_append_args* a, void* stream) {

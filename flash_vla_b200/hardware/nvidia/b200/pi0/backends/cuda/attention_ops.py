@@ -27,8 +27,9 @@ BLOCKS = (16, 32, 64, 128)      # rows per scale of an 8-bit cache
 _INT32, _F32 = torch.int32, torch.float32
 
 
-def _rows(name, shape, stride, dtype, want, multiple, overlap_ok=True):
-    """Element strides (episode, token, head) of a 4-D operand; an axis of one element gets a stride that any layout may have."""
+def _rows(name, shape, stride, dtype, want, multiple, shared=()):
+    """Element strides (episode, token, head) of a 4-D operand; an axis of one element gets a stride that any layout may have. `shared`: axes whose
+    elements may share their memory (stride 0)."""
     if dtype != want:
         raise ValueError(f"{name}: expected {want}, got {dtype}")
     if len(shape) != 4:
@@ -36,13 +37,13 @@ def _rows(name, shape, stride, dtype, want, multiple, overlap_ok=True):
     if shape[3] > 1 and stride[3] != 1:
         raise ValueError(f"{name}: the head dimension must be contiguous, got strides {tuple(stride)}")
     out = []
-    for size, s in zip(shape[:3], stride[:3]):
+    for axis, (size, s) in enumerate(zip(shape[:3], stride[:3])):
         if size <= 1:
             s = 256
         if s % multiple:
             raise ValueError(f"{name}: rows must start on 16 bytes, got strides {tuple(stride)}")
-        if s == 0 and not overlap_ok:
-            raise ValueError(f"{name}: a destination whose rows share memory, strides {tuple(stride)}")
+        if s == 0 and axis not in shared:
+            raise ValueError(f"{name}: rows that share memory, strides {tuple(stride)}")
         out.append(s)
     return out
 
@@ -77,7 +78,7 @@ def _cache_layout(c):
 
 @functools.lru_cache(maxsize=1024)
 def _attention_plan(q, k, v, out, cache):
-    """(argument block without addresses, scratch bytes) of an attention with operands of these layouts; `cache`: layout of a QuantizedCache, or None."""
+    """(argument block without addresses, scratch bytes without and with documents or weights) of an attention with operands of these layouts; `cache`: layout of a QuantizedCache, or None."""
     a = _lib.Attention()
     if cache is None:
         multiple, want, dim_multiple = 8, torch.bfloat16, 8
@@ -85,10 +86,10 @@ def _attention_plan(q, k, v, out, cache):
         a.block = _cache_shapes("cache", *cache)
         multiple, want, dim_multiple = 16, torch.float8_e4m3fn, 16
         k, v = ((cache[0][i], cache[1][i], cache[2][i]) for i in (0, 1))
-    a.q_stride[:] = _rows("Q", *q, torch.bfloat16, 8)
-    a.k_stride[:] = _rows("K", *k, want, multiple)
-    a.v_stride[:] = _rows("V", *v, want, multiple)
-    a.out_stride[:] = _rows("out", *out, torch.bfloat16, 8, overlap_ok=False)
+    a.q_stride[:] = _rows("Q", *q, torch.bfloat16, 8, shared=(0,))
+    a.k_stride[:] = _rows("K", *k, want, multiple, shared=(0, 2))
+    a.v_stride[:] = _rows("V", *v, want, multiple, shared=(0, 2))
+    a.out_stride[:] = _rows("out", *out, torch.bfloat16, 8)
     (E, T, H, D), (_, S, HK, _) = q[0], k[0]
     if tuple(k[0]) != (E, S, HK, D) or tuple(v[0]) != (E, S, HK, D) or tuple(out[0]) != (E, T, H, D):
         raise ValueError(f"attention: shapes do not fit: Q {tuple(q[0])}, K {tuple(k[0])}, V {tuple(v[0])}, out {tuple(out[0])}")
@@ -99,7 +100,14 @@ def _attention_plan(q, k, v, out, cache):
     if T * H >= 1 << 31 or E * HK >= 1 << 16 or S >= 1 << 31 or E >= 1 << 16:
         raise ValueError(f"attention: {E} episodes of {T} queries of {H} heads over {S} keys: too many")
     a.episodes, a.tokens, a.keys, a.heads, a.kv_heads, a.head_dim = E, T, S, H, HK, D
-    return a, _lib.load().fvla_attention_workspace_bytes(ctypes.byref(a)) if E and T else 0
+    nbytes = [0, 0]
+    for i, extra in enumerate(((), ("q_docs", "k_docs") if cache is None else ("weights", "lse"))):
+        b = _copy(a)
+        for name in ("q", "out", "k", "v", *(("k_scale", "v_scale") if cache is not None else ()), *extra):
+            setattr(b, name, 16)                # an address that only says that there is a tensor
+        if E and T:
+            nbytes[i] = _lib.load().fvla_attention_workspace_bytes(ctypes.byref(b))
+    return a, nbytes
 
 
 def _vector(name, t, shape, dtype, device):
@@ -174,9 +182,9 @@ def _attend(Q, K, V, cache, scale, out, causal, prefix, q_lens, k_lens, q_start,
         if lse is None:
             held = _scratch("attention_lse", 4 * E * H * T, Q)
             a.lse = held.data_ptr()
-    ws = _scratch("attention_ws", nbytes, Q)
+    ws = _scratch("attention_ws", nbytes[q_docs is not None or weights is not None], Q)
     if ws is not None:
-        a.ws, a.ws_bytes = ws.data_ptr(), nbytes
+        a.ws, a.ws_bytes = ws.data_ptr(), ws.numel()
     _lib.call("fvla_attention_run", ctypes.byref(a), _w._stream())
     return out
 
@@ -212,10 +220,10 @@ def cache_attention(Q, cache, lengths, scale, out, causal=False, prefix=None, q_
 def _append_plan(k, v, cache):
     a = _lib.CacheAppend()
     a.block = _cache_shapes("cache", *cache)
-    a.k_stride[:] = _rows("K", *k, torch.bfloat16, 8)
-    a.v_stride[:] = _rows("V", *v, torch.bfloat16, 8)
+    a.k_stride[:] = _rows("K", *k, torch.bfloat16, 8, shared=(0, 1, 2))
+    a.v_stride[:] = _rows("V", *v, torch.bfloat16, 8, shared=(0, 1, 2))
     for field, i in (("k_held_stride", 0), ("v_held_stride", 1)):
-        getattr(a, field)[:] = _rows("cache", cache[0][i], cache[1][i], cache[2][i], torch.float8_e4m3fn, 16, overlap_ok=False)
+        getattr(a, field)[:] = _rows("cache", cache[0][i], cache[1][i], cache[2][i], torch.float8_e4m3fn, 16)
     E, rows, HK, D = cache[0][0]
     T = k[0][1]
     if tuple(k[0]) != (E, T, HK, D) or tuple(v[0]) != (E, T, HK, D):
@@ -251,7 +259,7 @@ def _evict_plan(cache, out, keep, sinks, recent):
     a.block, a.out_block = _cache_shapes("cache", *cache), _cache_shapes("out_cache", *out)
     for name, layout, fields in (("cache", cache, ("k_stride", "v_stride")), ("out_cache", out, ("out_k_stride", "out_v_stride"))):
         for i, field in enumerate(fields):
-            getattr(a, field)[:] = _rows(name, layout[0][i], layout[1][i], layout[2][i], torch.float8_e4m3fn, 16, overlap_ok=name == "cache")
+            getattr(a, field)[:] = _rows(name, layout[0][i], layout[1][i], layout[2][i], torch.float8_e4m3fn, 16, shared=(0, 1, 2) if name == "cache" else ())
     E, rows, HK, D = cache[0][0]
     out_rows = out[0][0][1]
     if tuple(out[0][0]) != (E, out_rows, HK, D):

@@ -263,11 +263,9 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
 
     const bool any = walk.next(0) < walk.count;
 
-    // 640 threads start with 96 registers each: 472 of 480 for a thread of every warpgroup
-    if (Q8) {
-        if (warp < SOFTMAX0) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-        else if (warp < CONVERT0) asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
-    }
+    // (8-bit cache) 640 threads start with 96 registers each: 40 + 2 x 120 + 2 x 96 = 472 of 480 for a thread of every warpgroup
+    if (warp < SOFTMAX0) {
+    if (Q8) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 0) {
         if (lane == 0 && any) {
             tc5::prefetch_tensormap(&tmQ);
@@ -340,7 +338,9 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                 tc5::umma_commit(o_done);
             }
         }
-    } else if (warp >= SOFTMAX0 && warp < CONVERT0) {
+    }
+    } else if (warp < CONVERT0) {
+        if (Q8) asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
         // Softmax. Every thread runs every iteration and every named barrier even after a wait has given up (`ok` false), so nobody is left behind.
         const int quad = warp & 3, half = (warp - SOFTMAX0) >> 2;      // TMEM lane group this warp may access; which 64 keys of a block
         const int row = quad * 32 + lane;
@@ -607,7 +607,7 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                 }
             }
         }
-    } else if (Q8 && warp >= CONVERT0) {
+    } else if (Q8) {
         // e4m3 -> fp16 operands: warps 12-15 the keys, 16-19 the values
         const bool values = warp >= CONVERT0 + 4;
         const int ct = tid - 32 * (values ? CONVERT0 + 4 : CONVERT0);

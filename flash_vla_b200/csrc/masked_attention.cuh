@@ -429,10 +429,12 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
             if (walk.range != nullptr) tail = tail || __ldg(walk.range + walk.first + i).x < 0;
             if (busy) {
                 float (&v)[64] = reinterpret_cast<float (&)[64]>(r);
+                if (capped) {
 #pragma unroll
-                for (int c = 0; c < 64; ++c) {
-                    v[c] = v[c] * kf[c >> 4];
-                    if (capped) v[c] = cap2 * tanh_f(v[c]);
+                    for (int c = 0; c < 64; ++c) v[c] = cap2 * tanh_f(v[c] * kf[c >> 4]);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 64; ++c) v[c] *= kf[c >> 4];
                 }
                 if (a.slopes) {
                     const float d0 = (float)(pos - key0);
@@ -463,29 +465,20 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                     see[0] &= seen[0];
                     see[1] &= seen[1];
                 }
+                // what is hidden becomes -infinity, and 2^-infinity is 0
+                if (!__all_sync(0xffffffffu, (see[0] & see[1]) == 0xffffffffu)) {
+#pragma unroll
+                    for (int c = 0; c < 64; ++c) v[c] = see[c >> 5] & (1u << (c & 31)) ? v[c] : -INFINITY;
+                }
                 if (Q8 && p.scores != nullptr && mine) {
                     float4* dst = reinterpret_cast<float4*>(p.scores + (((size_t)e * a.heads + h) * a.tokens + t0 + t) * p.pitch + key0);
 #pragma unroll
-                    for (int c = 0; c < 64; c += 4) {
-                        float4 x = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
-                        const uint32_t bits = see[c >> 5] >> (c & 31);
-                        if (!(bits & 1u)) x.x = -INFINITY;
-                        if (!(bits & 2u)) x.y = -INFINITY;
-                        if (!(bits & 4u)) x.z = -INFINITY;
-                        if (!(bits & 8u)) x.w = -INFINITY;
-                        dst[c / 4] = x;
-                    }
+                    for (int c = 0; c < 64; c += 4) dst[c / 4] = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
                 }
-                float mx = -INFINITY;
-                const bool all = (see[0] & see[1]) == 0xffffffffu;
-                if (all) {
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int c = 0; c < 64; ++c) mx = fmaxf(mx, v[c] + lv[c >> 4]);
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 64; ++c)
-                        if (see[c >> 5] >> (c & 31) & 1u) mx = fmaxf(mx, v[c] + lv[c >> 4]);
-                }
+                for (int c = 0; c < 64; ++c) top[c >> 4] = fmaxf(top[c >> 4], v[c]);
+                float mx = fmaxf(fmaxf(top[0] + lv[0], top[1] + lv[1]), fmaxf(top[2] + lv[2], top[3] + lv[3]));
                 if (n > 0) pair_barrier();                             // the maxima of the block before have been read
                 xch[half * BQ + row] = mx;
                 pair_barrier();
@@ -518,7 +511,6 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
 #pragma unroll
                     for (int c = g * 16; c < g * 16 + 16; ++c) {
                         v[c] = fast_exp2(v[c] + off);
-                        if (!all) v[c] = see[c >> 5] >> (c & 31) & 1u ? v[c] : 0.f;
                         sum += v[c];
                     }
                     l += Q8 ? sum * fast_exp2(-lv[g]) : sum;

@@ -1,0 +1,466 @@
+// Attention of few rows: a decoding step of at most 32 rows (tokens x the query heads of a K/V head), bound by the bytes of the cache.
+//
+// The keys are the 128-row operand of both products, so that every thread of the softmax has one key and all rows of it:
+//   S^T (128 keys x rows) = K Q^T,      O^T (128 dims x rows, one or two halves) += V^T P^T
+// K and V tiles go from TMA straight to the tensor cores, also the 8-bit ones (kind::f8f6f4): nothing is converted. Instead the few rows are split
+// into e4m3 terms, each a row of the other operand. A bf16 q brought to 2^7..2^8 by its row's power of two is the sum of two terms of 4 bits
+// (the second times 2^5; what falls below the subnormals is under 2^-22 of the row's largest element), a probability the sum of three (times 2^4 and
+// 2^8: 12 bits). Probabilities stand against the running maximum at 2^4, which leaves 2^-22 of it above the last term's half step.
+//   warp 0      TMA: K and V tiles of 128 keys in turn through a ring of SLOTS
+//   warp 1      one lane issues the MMAs, S^T a block ahead
+//   warps 2-5   softmax: thread = key. The rows' maxima by redux and through shared memory, sums kept per thread until the end.
+// Each CTA has a share of an episode's blocks of one K/V head and leaves unnormalised sums; attention_join_kernel adds them up.
+#pragma once
+
+namespace fvla {
+namespace mattn {
+
+__device__ __forceinline__ float redux_max(float x) {
+    float r;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// N consecutive columns (a multiple of 16) of this thread's TMEM lane.
+template <int N>
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[N]) {
+    uint32_t r[N];
+    int c = 0;
+#pragma unroll
+    for (; c + 32 <= N; c += 32) ld32_nowait(taddr + c, r + c);
+    if (c < N)
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+            : "=r"(r[N - 16]), "=r"(r[N - 15]), "=r"(r[N - 14]), "=r"(r[N - 13]), "=r"(r[N - 12]), "=r"(r[N - 11]), "=r"(r[N - 10]), "=r"(r[N - 9]),
+              "=r"(r[N - 8]), "=r"(r[N - 7]), "=r"(r[N - 6]), "=r"(r[N - 5]), "=r"(r[N - 4]), "=r"(r[N - 3]), "=r"(r[N - 2]), "=r"(r[N - 1])
+            : "r"(taddr + N - 16) : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void st16(uint32_t taddr, const float* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(taddr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]),
+          "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]) : "memory");
+}
+
+constexpr int FEW_THREADS = 192;
+
+template <int HDP, bool Q8, int NR>
+struct FewCfg {
+    static constexpr int round16(int n) { return (n + 15) / 16 * 16; }
+    static constexpr int QT = Q8 ? 2 : 1, PT = Q8 ? 3 : 1;               // terms of Q and of P
+    static constexpr int NS = round16(NR * QT), NO = round16(NR * PT);   // columns of S^T and of a half of O^T
+    static constexpr int HALVES = HDP / 128, ELEM = Q8 ? 1 : 2;
+    static constexpr int ATOMS = HDP * ELEM / 128;                       // 128-byte columns of a tile
+    static constexpr int TILE = ATOMS * 16384;
+    static constexpr int KEY_ATOMS = 128 * ELEM / 128;                   // of P
+    static constexpr int Q_BYTES = ATOMS * NS * 128, P_BYTES = KEY_ATOMS * NO * 128;
+    // tiles in flight: three CTAs per SM with four tiles of 16 KB, two with three of 32 KB, one with three of 64 KB (32 rows: two, one, one)
+    static constexpr int SLOTS = TILE == 16384 ? 4 : 3;
+    static constexpr int PER_SM = NR == 32 ? (TILE == 16384 ? 2 : 1) : (TILE == 16384 ? 3 : (TILE == 32768 ? 2 : 1));
+    static constexpr int OFF_Q = 0, OFF_P = OFF_Q + Q_BYTES, OFF_T = OFF_P + P_BYTES;
+    static constexpr int OFF_F = OFF_T + SLOTS * TILE;                   // per row: factor, slope (floats), position, limit (ints)
+    static constexpr int OFF_M = OFF_F + 4 * NR * 4;                     // maxima of the four warps, twice
+    static constexpr int OFF_W = OFF_M + 2 * 4 * NR * 4;                 // of each warp, per row: the maximum in use, the factor of what is accumulated
+    static constexpr int OFF_BAR = OFF_W + 4 * 2 * NR * 4;
+    static constexpr int SMEM = 1024 + OFF_BAR + 160;
+    static constexpr int S_COL = 0, O_COL = 2 * NS;
+    static constexpr int USED = 2 * NS + HALVES * NO;
+    static constexpr uint32_t COLS = USED <= 64 ? 64 : (USED <= 128 ? 128 : (USED <= 256 ? 256 : 512));
+    static constexpr float SHIFT = Q8 ? 4.f : 0.f, THRESHOLD = Q8 ? 4.f : RESCALE_THRESHOLD;
+};
+
+template <int HDP, bool Q8, int NR>
+__global__ void __launch_bounds__(FEW_THREADS, (FewCfg<HDP, Q8, NR>::PER_SM))
+attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV) {
+    using C = FewCfg<HDP, Q8, NR>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t bars = base + C::OFF_BAR;
+    const uint32_t q_ready = bars, p_full = bars + 8, o_done = bars + 16;
+    auto s_full = [&](int b) { return bars + 24 + b * 8; };
+    auto s_empty = [&](int b) { return bars + 40 + b * 8; };
+    auto full = [&](int s) { return bars + 56 + s * 8; };
+    auto empty = [&](int s) { return bars + 88 + s * 8; };
+    volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(gen + C::OFF_BAR + 120);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + C::OFF_BAR + 124);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const Args& a = p.a;
+    const int e = blockIdx.z, kv = blockIdx.y, split = blockIdx.x;
+
+    if (tid == 0) {
+        mbar_init(q_ready, 4); mbar_init(p_full, 4); mbar_init(o_done, 1);
+        for (int b = 0; b < 2; ++b) { mbar_init(s_full(b), 1); mbar_init(s_empty(b), 4); }
+        for (int s = 0; s < C::SLOTS; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        tc5::tmem_alloc(bars + 120, C::COLS);
+        tc5::tmem_relinquish();
+    }
+    tc5::tc_fence_before();
+    __syncthreads();
+    tc5::tc_fence_after();
+    const uint32_t tmem = *tmem_slot_ptr;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    const Episode s = episode_of(a, e);
+    int most = s.n > 0 ? s.L : 0;
+    if (a.causal && a.k_pos == nullptr) most = max(0, min(most, max(s.start + s.n, s.prefix)));
+    const int blocks = (most + BKEY - 1) / BKEY, share = (blocks + p.splits - 1) / p.splits;
+    const int first = split * share, count = max(0, min(share, blocks - first));
+
+    if (warp == 0) {
+        if (lane == 0) {
+            tc5::prefetch_tensormap(&tmK);
+            tc5::prefetch_tensormap(&tmV);
+            for (int i = 0; i < 2 * count; ++i) {
+                const int st = i % C::SLOTS;
+                const CUtensorMap* map = i & 1 ? &tmV : &tmK;
+                const int* mul = i & 1 ? p.v_mul : p.k_mul;
+                if (!mbar_wait(empty(st), (uint32_t)((i / C::SLOTS) & 1) ^ 1u, abort_flag)) break;
+                mbar_expect_tx(full(st), C::TILE);
+#pragma unroll
+                for (int c = 0; c < C::ATOMS; ++c)
+                    tma_load_4d(base + C::OFF_T + st * C::TILE + c * 16384, map, full(st), c * (128 / C::ELEM), (first + (i >> 1)) * BKEY, kv * mul[0], e * mul[1]);
+            }
+        }
+    } else if (warp == 1) {
+        if (tc5::elect_one() && count > 0) {
+            constexpr uint32_t type = Q8 ? 0u : 1u;                      // e4m3 or bf16
+            constexpr uint32_t id_qk = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(C::NS >> 3) << 17) | (8u << 24);
+            constexpr uint32_t id_pv = (1u << 4) | (type << 7) | (type << 10) | (1u << 15) | ((uint32_t)(C::NO >> 3) << 17) | (8u << 24);
+            auto mma = [&](uint32_t d, uint64_t ad, uint64_t bd, uint32_t id, bool acc) {
+                if (Q8) umma_f8(d, ad, bd, id, acc);
+                else tc5::umma_bf16(d, ad, bd, id, acc);
+            };
+            auto issue_qk = [&](int n) -> bool {
+                const int st = 2 * n % C::SLOTS, b = n & 1;
+                if (!mbar_wait(full(st), (uint32_t)((2 * n / C::SLOTS) & 1), abort_flag)) return false;
+                if (!mbar_wait(s_empty(b), (uint32_t)((n >> 1) & 1) ^ 1u, abort_flag)) return false;
+                tc5::tc_fence_after();
+#pragma unroll
+                for (int k = 0; k < 4 * C::ATOMS; ++k)                   // 32 bytes of the head dimension at a time
+                    mma(tmem + C::S_COL + b * C::NS, smem_desc(base + C::OFF_T + st * C::TILE + (k >> 2) * 16384 + (k & 3) * 32, 16, 1024),
+                        smem_desc(base + C::OFF_Q + (k >> 2) * (C::NS * 128) + (k & 3) * 32, 16, 1024), id_qk, k > 0);
+                tc5::umma_commit(empty(st));
+                tc5::umma_commit(s_full(b));
+                return true;
+            };
+            bool ok = mbar_wait(q_ready, 0, abort_flag);
+            tc5::tc_fence_after();
+            ok = ok && issue_qk(0);
+            for (int n = 0; n < count && ok; ++n) {
+                if (n + 1 < count) { ok = issue_qk(n + 1); if (!ok) break; }
+                const int st = (2 * n + 1) % C::SLOTS;
+                if (!mbar_wait(p_full, (uint32_t)(n & 1), abort_flag)) break;
+                if (!mbar_wait(full(st), (uint32_t)(((2 * n + 1) / C::SLOTS) & 1), abort_flag)) break;
+                tc5::tc_fence_after();
+                constexpr int KEYS = 32 / C::ELEM;                       // keys per MMA
+#pragma unroll
+                for (int h = 0; h < C::HALVES; ++h)
+#pragma unroll
+                    for (int k = 0; k < BKEY / KEYS; ++k)
+                        mma(tmem + C::O_COL + h * C::NO, smem_desc(base + C::OFF_T + st * C::TILE + h * C::ELEM * 16384 + k * KEYS * 128, 16384, 1024),
+                            smem_desc(base + C::OFF_P + (k >> 2) * (C::NO * 128) + (k & 3) * 32, 16, 1024), id_pv, n > 0 || k > 0);
+                tc5::umma_commit(empty(st));
+                tc5::umma_commit(o_done);
+            }
+        }
+    } else {
+        const int quad = warp & 3, key = quad * 32 + lane;                     // key of a block = TMEM lane
+        const uint32_t t_lane = (uint32_t)(quad * 32) << 16;
+        const int group = p.group, rows = s.n * group;                         // row = token * group + head
+        float* row_f = reinterpret_cast<float*>(gen + C::OFF_F);
+        float* row_slope = row_f + NR;
+        int* row_pos = reinterpret_cast<int*>(row_f + 2 * NR);
+        int* row_limit = row_pos + NR;
+        float* maxima = reinterpret_cast<float*>(gen + C::OFF_M);
+        float* in_use = reinterpret_cast<float*>(gen + C::OFF_W) + quad * 2 * NR;
+        float* rescale = in_use + NR;
+        const bool capped = a.cap > 0.f;
+        auto barrier = []() { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+        bool ok = true;
+
+        if (count > 0) {
+            // Q as the K-major operand, and what the rows have of their own
+            constexpr int PER = HDP / 32;                                      // elements of a lane: 4 or 8
+            for (int r = quad; r < C::NS / C::QT; r += 4) {
+                const int t = r / group, h = kv * group + r - t * group;
+                float q[PER];
+                uint32_t amax = 0;
+#pragma unroll
+                for (int i = 0; i < PER; i += 4) {
+                    uint2 u = make_uint2(0, 0);
+                    const int d = lane * PER + i;
+                    if (r < rows && d < a.dim) u = __ldg(reinterpret_cast<const uint2*>(static_cast<const bf16*>(a.q) + e * a.qs[0] + t * a.qs[1] + h * a.qs[2] + d));
+                    const float2 x = unpack_bf16x2(u.x), y = unpack_bf16x2(u.y);
+                    q[i] = x.x; q[i + 1] = x.y; q[i + 2] = y.x; q[i + 3] = y.y;
+                    amax = max(max(amax, max(u.x & 0x7fffu, (u.x >> 16) & 0x7fffu)), max(u.y & 0x7fffu, (u.y >> 16) & 0x7fffu));
+                }
+                float f = capped ? a.scale / a.cap : a.scale * kLog2e;
+                const int at = lane * PER * C::ELEM;                            // byte within the row
+                uint8_t* line = gen + C::OFF_Q + (at >> 7) * (C::NS * 128);
+                const int piece = (at & 127) >> 4, in = at & 15;
+                if (Q8) {
+                    amax = __reduce_max_sync(0xffffffffu, amax);
+                    const int ex = min(max((int)(amax >> 7) - 127, -119), 127);      // the largest element to 2^7..2^8
+                    const float up = __int_as_float((134 - ex) << 23);
+                    f *= __int_as_float((120 + ex) << 23);
+                    if (amax >= 0x7f80u) f = __int_as_float(0x7fffffff);        // an infinity or NaN: the row is NaN
+                    uint32_t one[PER / 4], two[PER / 4];
+#pragma unroll
+                    for (int i = 0; i < PER; i += 4) {
+                        const float x[4] = {q[i] * up, q[i + 1] * up, q[i + 2] * up, q[i + 3] * up};
+                        const uint32_t lo = q8::to_e4m3x2(x[0], x[1]), hi = q8::to_e4m3x2(x[2], x[3]);
+                        const float2 a0 = q8::from_e4m3x2(lo), a1 = q8::from_e4m3x2(hi);
+                        one[i / 4] = lo | hi << 16;
+                        two[i / 4] = q8::to_e4m3x2((x[0] - a0.x) * 32.f, (x[1] - a0.y) * 32.f) | q8::to_e4m3x2((x[2] - a1.x) * 32.f, (x[3] - a1.y) * 32.f) << 16;
+                    }
+#pragma unroll
+                    for (int i = 0; i < PER / 4; ++i) {
+                        *reinterpret_cast<uint32_t*>(line + r * 128 + ((piece ^ (r & 7)) << 4) + in + 4 * i) = one[i];
+                        *reinterpret_cast<uint32_t*>(line + (NR + r) * 128 + ((piece ^ ((NR + r) & 7)) << 4) + in + 4 * i) = two[i];
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < PER; i += 4)
+                        *reinterpret_cast<uint2*>(line + r * 128 + ((piece ^ (r & 7)) << 4) + in + 2 * i) = make_uint2(pack_bf16x2(q[i], q[i + 1]), pack_bf16x2(q[i + 2], q[i + 3]));
+                }
+                if (r < NR && lane == 0) {
+                    const int pos = s.start + t;
+                    row_f[r] = f;
+                    row_slope[r] = a.slopes && r < rows ? a.slopes[h] * kLog2e : 0.f;
+                    row_pos[r] = pos;
+                    row_limit[r] = a.causal ? max(pos, s.prefix - 1) : 0x7fffffff;
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            barrier();
+            if (lane == 0) tc5::mbar_arrive(q_ready);
+        }
+
+        float m_lane = -INFINITY;                                              // lane r: the maximum that row r's sums stand against
+        float l[NR];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) l[r] = 0.f;
+        const float cap2 = a.cap * kLog2e;
+        const float* ks = a.k_scale + (size_t)e * (Q8 ? a.keys / a.block : 0) * a.kv_heads + kv;
+        const float* vs = a.v_scale + (size_t)e * (Q8 ? a.keys / a.block : 0) * a.kv_heads + kv;
+        const int shift = Q8 ? 31 - __clz(a.block) : 0;                        // blocks are powers of two
+        for (int n = 0; n < count; ++n) {
+            const int b = n & 1, j = (first + n) * BKEY + key;
+            const bool inside = j < s.L;
+            float kf = 1.f, lv = 0.f, iv = 1.f;                                // K's scale; log2 of V's and its inverse
+            if (Q8) {
+                const size_t at = (size_t)(min(j, a.keys - 1) >> shift) * a.kv_heads;
+                kf = __ldg(ks + at);
+                const float x = __ldg(vs + at);
+                lv = (float)((int)(__float_as_uint(x) >> 23) - 127);
+                iv = q8::inverse_pow2(x);
+            }
+            const int kp = a.k_pos ? __ldg(a.k_pos + (size_t)e * a.keys + min(j, a.keys - 1)) : j;
+            ok = ok && mbar_wait(s_full(b), (uint32_t)((n >> 1) & 1), abort_flag);
+            __syncwarp();
+            tc5::tc_fence_after();
+            float c[C::NS];
+            tmem_ld(tmem + t_lane + C::S_COL + b * C::NS, c);
+            tc5::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) tc5::mbar_arrive(s_empty(b));
+            float v[NR];
+#pragma unroll
+            for (int r = 0; r < NR; ++r) v[r] = (Q8 ? fmaf(c[(NR + r) % C::NS], 1.f / 32.f, c[r]) : c[r]) * (row_f[r] * kf);
+            if (capped) {
+#pragma unroll
+                for (int r = 0; r < NR; ++r) v[r] = cap2 * tanh_f(v[r]);
+            }
+            if (a.slopes) {
+#pragma unroll
+                for (int r = 0; r < NR; ++r) v[r] = fmaf(-row_slope[r], fabsf((float)(row_pos[r] - kp)), v[r]);
+            }
+            if (a.causal) {
+#pragma unroll
+                for (int r = 0; r < NR; ++r) v[r] = inside && kp <= row_limit[r] ? v[r] : -INFINITY;
+            } else if (!inside) {
+#pragma unroll
+                for (int r = 0; r < NR; ++r) v[r] = -INFINITY;
+            }
+            if (Q8 && p.scores != nullptr) {
+#pragma unroll
+                for (int r = 0; r < NR; ++r)
+                    if (r < rows) {
+                        const int t = r / group;
+                        p.scores[(((size_t)e * a.heads + kv * group + r - t * group) * a.tokens + t) * p.pitch + j] = v[r];
+                    }
+            }
+            float mine = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                v[r] += lv;
+                const float x = redux_max(v[r]);
+                if (lane == r) mine = x;
+            }
+            float* board = maxima + b * 4 * NR;
+            if (lane < NR) board[quad * NR + lane] = mine;
+            barrier();
+            bool grow = false;
+            if (lane < NR) {
+                const float mx = fmaxf(fmaxf(board[lane], board[NR + lane]), fmaxf(board[2 * NR + lane], board[3 * NR + lane]));
+                grow = m_lane != -INFINITY && mx > m_lane + C::THRESHOLD;
+                rescale[lane] = grow ? fast_exp2(m_lane - mx) : 1.f;
+                if (grow || m_lane == -INFINITY) m_lane = mx;
+                in_use[lane] = (m_lane == -INFINITY ? 0.f : m_lane) - C::SHIFT;      // (nothing but NaN, or nothing at all, so far)
+            }
+            const bool any = __any_sync(0xffffffffu, grow);
+            __syncwarp();
+            // P of the block before, and its products, are done with; the same for every warp, since all of them see the same maxima
+            ok = ok && (n == 0 || mbar_wait(o_done, (uint32_t)((n - 1) & 1), abort_flag));
+            __syncwarp();
+            if (any) {
+                tc5::tc_fence_after();
+#pragma unroll
+                for (int h = 0; h < C::HALVES; ++h)
+#pragma unroll
+                    for (int c0 = 0; c0 < C::NO; c0 += 16) {
+                        float o[16];
+                        const uint32_t at = tmem + t_lane + C::O_COL + h * C::NO + c0;
+                        tc5::tmem_ld16(at, o);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] *= c0 + i < NR * C::PT ? rescale[(c0 + i) % NR] : 1.f;
+                        st16(at, o);
+                    }
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                tc5::tc_fence_before();
+#pragma unroll
+                for (int r = 0; r < NR; ++r) l[r] *= rescale[r];
+            }
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                v[r] = fast_exp2(v[r] - in_use[r]);
+                l[r] = fmaf(v[r], iv, l[r]);
+            }
+            // P^T: a row of 128 keys per row and term
+            if (Q8) {
+                auto at = [&](int row) { return gen + C::OFF_P + row * 128 + (((key >> 4) ^ (row & 7)) << 4) + (key & 15); };
+#pragma unroll
+                for (int r = 0; r < NR; r += 2) {
+                    float x = v[r], y = v[r + 1];
+                    float up = 1.f;
+#pragma unroll
+                    for (int term = 0; term < 3; ++term) {
+                        const uint32_t w = q8::to_e4m3x2(x * up, y * up);
+                        *at(term * NR + r) = (uint8_t)w;
+                        *at(term * NR + r + 1) = (uint8_t)(w >> 8);
+                        const float2 back = q8::from_e4m3x2(w);
+                        x = fmaf(-back.x, 1.f / up, x);
+                        y = fmaf(-back.y, 1.f / up, y);
+                        up *= 16.f;
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < NR; ++r)
+                    *reinterpret_cast<bf16*>(gen + C::OFF_P + (key >> 6) * (C::NO * 128) + r * 128 + ((((key & 63) >> 3) ^ (r & 7)) << 4) + (key & 7) * 2) = __float2bfloat16_rn(v[r]);
+            }
+            if ((first + n + 1) * BKEY > s.L) {
+                // values behind the last key may be anything, and 0 * NaN would reach every row: zeros in their place
+                const int vs_slot = (2 * n + 1) % C::SLOTS;
+                ok = ok && mbar_wait(full(vs_slot), (uint32_t)(((2 * n + 1) / C::SLOTS) & 1), abort_flag);
+                if (!inside)
+                    for (int i = 0; i < C::ATOMS * 8; ++i)
+                        *reinterpret_cast<uint4*>(gen + C::OFF_T + vs_slot * C::TILE + (i >> 3) * 16384 + key * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            tc5::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) tc5::mbar_arrive(p_full);
+        }
+        if (count > 0) ok = ok && mbar_wait(o_done, (uint32_t)((count - 1) & 1), abort_flag);
+        __syncwarp();
+        tc5::tc_fence_after();
+
+        // the rows' sums over the 128 threads, then O^T: thread = dim, so that a row's dims are stored side by side
+        float total = 0.f;
+        if (count > 0) {
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                const float x = warp_sum(l[r]);
+                if (lane == r) total = x;
+            }
+            barrier();                                                          // the last maxima have been read
+            if (lane < NR) maxima[quad * NR + lane] = total;
+            barrier();
+        }
+        const size_t all = (size_t)a.episodes * a.tokens * a.heads;
+        auto flat = [&](int r) {
+            const int t = r / group;
+            return (size_t)split * all + ((size_t)e * a.tokens + t) * a.heads + kv * group + r - t * group;
+        };
+        if (quad == 0 && lane < rows) {
+            const float sum = count > 0 ? maxima[lane] + maxima[NR + lane] + maxima[2 * NR + lane] + maxima[3 * NR + lane] : 0.f;
+            p.part_ml[flat(lane)] = make_float2(count > 0 ? in_use[lane] : -INFINITY, sum);
+        }
+        if (count > 0 && ok) {
+#pragma unroll
+            for (int h = 0; h < C::HALVES; ++h) {
+                float o[C::NO];
+                tmem_ld(tmem + t_lane + C::O_COL + h * C::NO, o);
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                    const float x = Q8 ? fmaf(fmaf(o[(2 * NR + r) % C::NO], 1.f / 16.f, o[(NR + r) % C::NO]), 1.f / 16.f, o[r]) : o[r];
+                    if (r < rows) p.part_o[flat(r) * HDP + h * 128 + key] = x;
+                }
+            }
+        }
+    }
+
+    tc5::tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc5::tc_fence_after();
+        tc5::tmem_dealloc(tmem, C::COLS);
+    }
+    if (tid == 0 && *abort_flag && p.status) atomicExch(p.status, 9);
+}
+
+// Rows that the kernel is built for.
+inline int few_rows(const Args& a) {
+    const int rows = a.tokens * (a.heads / a.kv_heads);
+    return rows <= 8 ? 8 : (rows <= 16 ? 16 : 32);
+}
+
+template <int HDP, bool Q8, int NR>
+inline int launch_few(const Tile& p, const CUtensorMap& tmK, const CUtensorMap& tmV, cudaStream_t st) {
+    using C = FewCfg<HDP, Q8, NR>;
+    auto kern = attention_few_rows_kernel<HDP, Q8, NR>;
+    static PerDeviceFlag configured;
+    if (!configured.get()) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return FVLA_ERR_LAUNCH; }
+        configured.set();
+    }
+    const cudaError_t e = launch_pdl(kern, dim3(p.splits, p.a.kv_heads, p.a.episodes), dim3(FEW_THREADS), C::SMEM, st, p, tmK, tmV);
+    if (e != cudaSuccess) { set_error("attention_few_rows_kernel: %s", cudaGetErrorString(e)); return FVLA_ERR_LAUNCH; }
+    return check_launch("attention_few_rows_kernel");
+}
+template <int HDP, bool Q8>
+inline int launch_few(const Tile& p, const CUtensorMap& tmK, const CUtensorMap& tmV, cudaStream_t st) {
+    const int nr = few_rows(p.a);
+    return nr == 8 ? launch_few<HDP, Q8, 8>(p, tmK, tmV, st) : (nr == 16 ? launch_few<HDP, Q8, 16>(p, tmK, tmV, st) : launch_few<HDP, Q8, 32>(p, tmK, tmV, st));
+}
+
+}  // namespace mattn
+}  // namespace fvla

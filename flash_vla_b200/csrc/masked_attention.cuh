@@ -652,48 +652,61 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
     if (tid == 0 && *abort_flag && p.status) atomicExch(p.status, 9);
 }
 
-// One warp per row: the splits' accumulators against the largest of their maxima.
+// The shares' sums against the largest of their maxima. `warps` of a CTA take a row together: each adds up every warps-th share, and the first adds
+// up the warps in their order.
+constexpr int JOIN_WARPS = 8;
 template <int HDP>
-__global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ Tile p) {
+__global__ void __launch_bounds__(32 * JOIN_WARPS) attention_join_kernel(const __grid_constant__ Tile p, int warps) {
+    __shared__ float sums[JOIN_WARPS][HDP + 1];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const Args& a = p.a;
-    const int lane = threadIdx.x & 31;
-    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5), rows = (long long)a.episodes * a.tokens * a.heads;
-    if (row >= rows) return;
-    const int h = (int)(row % a.heads), t = (int)(row / a.heads % a.tokens), e = (int)(row / a.heads / a.tokens);
-    if (t >= episode_of(a, e).n) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % warps;
+    const long long row = (long long)blockIdx.x * (JOIN_WARPS / warps) + warp / warps, rows = (long long)a.episodes * a.tokens * a.heads;
+    const int h = (int)(row % a.heads), t = (int)(row / a.heads % a.tokens), e = (int)min(row / a.heads / a.tokens, (long long)a.episodes - 1);
+    const bool mine = row < rows && t < episode_of(a, e).n;
     float m = -INFINITY;
-    for (int s = lane; s < p.splits; s += 32) {
-        const float2 ml = p.part_ml[s * rows + row];
-        if (ml.y != 0.f) m = fmaxf(m, ml.x);
-    }
+    if (mine)
+        for (int s = lane; s < p.splits; s += 32) {
+            const float2 ml = p.part_ml[s * rows + row];
+            if (ml.y != 0.f) m = fmaxf(m, ml.x);
+        }
     m = warp_max(m);
     const float top = m == -INFINITY ? 0.f : m;
-    constexpr int PER = HDP / 32 < 4 ? HDP / 32 : 4, ROUNDS = HDP / 32 / PER;      // consecutive columns of a lane
-    float acc[ROUNDS * PER], l = 0.f;
+    constexpr int PER = HDP / 32;                                                    // columns lane, lane + 32, ...
+    float acc[PER], l = 0.f;
 #pragma unroll
-    for (int c = 0; c < ROUNDS * PER; ++c) acc[c] = 0.f;
-    for (int s = 0; s < p.splits; ++s) {
-        const float2 ml = p.part_ml[s * rows + row];
-        if (ml.y == 0.f) continue;                                                   // this share held nothing that the row sees
-        const float w = ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - top);
-        l = fmaf(ml.y, w, l);
-        const float* o = p.part_o + (s * rows + row) * HDP;
+    for (int c = 0; c < PER; ++c) acc[c] = 0.f;
+    if (mine) {
+#pragma unroll 4
+        for (int s = part; s < p.splits; s += warps) {
+            const float2 ml = p.part_ml[s * rows + row];
+            if (ml.y == 0.f) continue;                                               // this share held nothing that the row sees
+            const float w = ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - top);
+            l = fmaf(ml.y, w, l);
+            const float* o = p.part_o + (s * rows + row) * HDP + lane;
 #pragma unroll
-        for (int r = 0; r < ROUNDS; ++r)
-#pragma unroll
-            for (int c = 0; c < PER; ++c) acc[r * PER + c] = fmaf(w, o[r * 32 * PER + lane * PER + c], acc[r * PER + c]);
+            for (int c = 0; c < PER; ++c) acc[c] = fmaf(w, o[32 * c], acc[c]);
+        }
     }
+    if (warps > 1) {
+#pragma unroll
+        for (int c = 0; c < PER; ++c) sums[warp][lane + 32 * c] = acc[c];
+        if (lane == 0) sums[warp][HDP] = l;
+        __syncthreads();
+        if (part != 0) return;
+        for (int w = 1; w < warps; ++w) {
+#pragma unroll
+            for (int c = 0; c < PER; ++c) acc[c] += sums[warp + w][lane + 32 * c];
+            l += sums[warp + w][HDP];
+        }
+    }
+    if (!mine) return;
     const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
     bf16* dst = a.out + e * a.os[0] + t * a.os[1] + h * a.os[2];
 #pragma unroll
-    for (int r = 0; r < ROUNDS; ++r)
-#pragma unroll
-        for (int c = 0; c < PER; c += 2) {
-            const int col = r * 32 * PER + lane * PER + c;
-            if (col < a.dim) *reinterpret_cast<uint32_t*>(dst + col) = pack_bf16x2(acc[r * PER + c] * inv, acc[r * PER + c + 1] * inv);
-        }
+    for (int c = 0; c < PER; ++c)
+        if (lane + 32 * c < a.dim) dst[lane + 32 * c] = __float2bfloat16_rn(acc[c] * inv);
     if (a.lse && lane == 0) a.lse[((size_t)e * a.heads + h) * a.tokens + t] = l > 0.f ? (top + log2f(l)) * 0.6931471805599453f : (l == 0.f ? -INFINITY : l);
 }
 
@@ -730,27 +743,43 @@ __global__ void __launch_bounds__(32 * WEIGHT_WARPS) key_weights_kernel(const __
 }
 
 // Tensor map of a strided operand, innermost axis contiguous; an axis of stride 0 is left at one element (its coordinate is 0).
-inline int make_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box) {
+inline int make_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box, int elem = 2) {
     tc5::EncodeTiledFn fn = tc5::encode_fn();
     if (fn == nullptr) { set_error("cuTensorMapEncodeTiled is not available from the driver"); return FVLA_ERR_LAUNCH; }
     cuuint64_t gdim[5], gstride[4];
     cuuint32_t b[5], step[5];
     for (int i = 0; i < rank; ++i) { gdim[i] = dims[i]; b[i] = box[i]; step[i] = 1; }
-    for (int i = 0; i + 1 < rank; ++i) gstride[i] = strides[i] * sizeof(bf16);
-    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), gdim, gstride, b, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    for (int i = 0; i + 1 < rank; ++i) gstride[i] = strides[i] * elem;
+    const CUresult r = fn(map, elem == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), gdim, gstride, b, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) { set_error("attention: cuTensorMapEncodeTiled failed with CUresult %d", (int)r); return FVLA_ERR_ARG; }
     return FVLA_OK;
 }
 
-// Head dimension that the kernel is built for.
-inline int padded_dim(int dim) { return dim <= 64 ? 64 : (dim <= 128 ? 128 : 256); }
+}  // namespace mattn
+}  // namespace fvla
 
-// Shares of the key blocks: as many as bring the CTAs up to the number of SMs, at most one per block.
+#include "few_rows_attention.cuh"
+
+namespace fvla {
+namespace mattn {
+
+// Up to 32 rows per episode and K/V head, and no documents: the kernel for few rows.
+inline bool takes_few(const Args& a) { return (long long)a.tokens * (a.heads / a.kv_heads) <= 32 && a.q_docs == nullptr; }
+// Head dimension that the kernel is built for.
+inline int padded_dim(const Args& a) { return a.dim <= 64 && !takes_few(a) ? 64 : (a.dim <= 128 ? 128 : 256); }
+
+// Shares of the key blocks: as many as bring the CTAs up to the number that are resident, at most one per block.
 inline int plan_splits(const Args& a) {
     const int group = a.heads / a.kv_heads, tile_tokens = BQ / group, blocks = (a.keys + BKEY - 1) / BKEY;
-    const long long tiles = (long long)((a.tokens + tile_tokens - 1) / tile_tokens) * a.kv_heads * a.episodes;
-    const long long room = tc5::num_sms() / tiles;
+    const bool few = takes_few(a);
+    const long long tiles = (few ? 1ll : (long long)((a.tokens + tile_tokens - 1) / tile_tokens)) * a.kv_heads * a.episodes;
+    int per_sm = 1;
+    if (few) {
+        const int tile_bytes = 128 * padded_dim(a) * (a.k_scale ? 1 : 2);
+        per_sm = few_rows(a) == 32 ? (tile_bytes == 16384 ? 2 : 1) : (tile_bytes == 16384 ? 3 : (tile_bytes == 32768 ? 2 : 1));
+    }
+    const long long room = (long long)tc5::num_sms() * per_sm * (few && tiles > tc5::num_sms() ? 2 : 1) / tiles;
     return (int)(room < 1 ? 1 : (room < blocks ? room : (blocks > 0 ? blocks : 1)));
 }
 inline size_t score_pitch(const Args& a) { return ((size_t)a.keys + BKEY - 1) / BKEY * BKEY; }
@@ -760,8 +789,17 @@ inline size_t workspace_bytes(const Args& a) {
     const size_t rows = (size_t)a.episodes * a.tokens * a.heads;
     size_t n = a.q_docs ? align256((size_t)a.episodes * ((a.keys + BKEY - 1) / BKEY) * sizeof(int2)) : 0;
     if (a.weights) n += rows * score_pitch(a) * sizeof(float);
-    if (splits > 1) n += align256(splits * rows * sizeof(float2)) + splits * rows * padded_dim(a.dim) * sizeof(float);
+    if (splits > 1 || takes_few(a)) n += align256(splits * rows * sizeof(float2)) + splits * rows * padded_dim(a) * sizeof(float);
     return n;
+}
+
+template <int HDP>
+inline int launch_join(const Tile& p, cudaStream_t st) {
+    const long long rows = (long long)p.a.episodes * p.a.tokens * p.a.heads;
+    const int warps = p.splits >= 16 ? 8 : (p.splits >= 8 ? 4 : (p.splits >= 4 ? 2 : 1)), each = JOIN_WARPS / warps;
+    const cudaError_t e = launch_pdl(attention_join_kernel<HDP>, dim3((unsigned)((rows + each - 1) / each)), dim3(32 * JOIN_WARPS), 0, st, p, warps);
+    if (e != cudaSuccess) { set_error("attention_join_kernel: %s", cudaGetErrorString(e)); return FVLA_ERR_LAUNCH; }
+    return check_launch("attention_join_kernel");
 }
 
 template <int HDP, bool Q8>
@@ -778,10 +816,7 @@ inline int launch_tile(const Tile& p, const CUtensorMap& tmQ, const CUtensorMap&
     cudaError_t e = launch_pdl(kern, dim3(p.tiles * p.splits, a.kv_heads, a.episodes), dim3(C::THREADS), C::SMEM, st, p, tmQ, tmK, tmV);
     if (e != cudaSuccess) { set_error("attention_tile_kernel: %s", cudaGetErrorString(e)); return FVLA_ERR_LAUNCH; }
     int rc = check_launch("attention_tile_kernel");
-    if (rc || p.splits == 1) return rc;
-    e = launch_pdl(attention_join_kernel<HDP>, dim3((unsigned)(((long long)a.episodes * a.tokens * a.heads + 3) / 4)), dim3(128), 0, st, p);
-    if (e != cudaSuccess) { set_error("attention_join_kernel: %s", cudaGetErrorString(e)); return FVLA_ERR_LAUNCH; }
-    return check_launch("attention_join_kernel");
+    return rc || p.splits == 1 ? rc : launch_join<HDP>(p, st);
 }
 
 inline int launch_attention(const Args& a, void* ws, int* status, cudaStream_t st) {
@@ -792,7 +827,7 @@ inline int launch_attention(const Args& a, void* ws, int* status, cudaStream_t s
     p.tiles = (a.tokens + p.tile_tokens - 1) / p.tile_tokens;
     p.splits = plan_splits(a);
     p.status = status;
-    const int blocks = (a.keys + BKEY - 1) / BKEY, hdp = padded_dim(a.dim);
+    const int blocks = (a.keys + BKEY - 1) / BKEY, hdp = padded_dim(a);
     const size_t rows = (size_t)a.episodes * a.tokens * a.heads;
     uint8_t* at = static_cast<uint8_t*>(ws);
     p.doc_range = nullptr;
@@ -817,6 +852,7 @@ inline int launch_attention(const Args& a, void* ws, int* status, cudaStream_t s
     p.part_ml = reinterpret_cast<float2*>(at);
     p.part_o = reinterpret_cast<float*>(at + align256(p.splits * rows * sizeof(float2)));
     CUtensorMap tmQ, tmK, tmV;
+    const bool few = takes_few(a), q8 = a.k_scale != nullptr;
     p.q_mul[0] = 1;
     p.q_mul[1] = a.qs[0] != 0;
     {
@@ -828,20 +864,27 @@ inline int launch_attention(const Args& a, void* ws, int* status, cudaStream_t s
     }
     tmK = tmV = tmQ;
     p.k_mul[0] = a.ks[2] != 0; p.k_mul[1] = a.ks[0] != 0; p.v_mul[0] = a.vs[2] != 0; p.v_mul[1] = a.vs[0] != 0;
-    if (a.k_scale == nullptr && a.keys > 0) {
+    if ((few || !q8) && a.keys > 0) {
         for (int i = 0; i < 2; ++i) {
             const long long* s = i == 0 ? a.ks : a.vs;
             const int* mul = i == 0 ? p.k_mul : p.v_mul;
             const uint64_t dims[4] = {(uint64_t)a.dim, (uint64_t)a.keys, mul[0] ? (uint64_t)a.kv_heads : 1, mul[1] ? (uint64_t)a.episodes : 1};
             const uint64_t strides[3] = {(uint64_t)s[1], mul[0] ? (uint64_t)s[2] : 256, mul[1] ? (uint64_t)s[0] : 256};
-            const uint32_t box[4] = {64, i == 0 ? 128u : 64u, 1, 1};
-            const int rc = make_map(i == 0 ? &tmK : &tmV, i == 0 ? a.k : a.v, 4, dims, strides, box);
+            const uint32_t box[4] = {q8 ? 128u : 64u, i == 0 || few ? 128u : 64u, 1, 1};
+            const int rc = make_map(i == 0 ? &tmK : &tmV, i == 0 ? a.k : a.v, 4, dims, strides, box, q8 ? 1 : 2);
             if (rc) return rc;
         }
     }
     int rc;
-    if (a.k_scale) rc = hdp == 64 ? launch_tile<64, true>(p, tmQ, tmK, tmV, st) : (hdp == 128 ? launch_tile<128, true>(p, tmQ, tmK, tmV, st) : launch_tile<256, true>(p, tmQ, tmK, tmV, st));
-    else rc = hdp == 64 ? launch_tile<64, false>(p, tmQ, tmK, tmV, st) : (hdp == 128 ? launch_tile<128, false>(p, tmQ, tmK, tmV, st) : launch_tile<256, false>(p, tmQ, tmK, tmV, st));
+    if (few) {
+        if (q8) rc = hdp == 128 ? launch_few<128, true>(p, tmK, tmV, st) : launch_few<256, true>(p, tmK, tmV, st);
+        else rc = hdp == 128 ? launch_few<128, false>(p, tmK, tmV, st) : launch_few<256, false>(p, tmK, tmV, st);
+        if (!rc) rc = hdp == 128 ? launch_join<128>(p, st) : launch_join<256>(p, st);
+    } else if (q8) {
+        rc = hdp == 64 ? launch_tile<64, true>(p, tmQ, tmK, tmV, st) : (hdp == 128 ? launch_tile<128, true>(p, tmQ, tmK, tmV, st) : launch_tile<256, true>(p, tmQ, tmK, tmV, st));
+    } else {
+        rc = hdp == 64 ? launch_tile<64, false>(p, tmQ, tmK, tmV, st) : (hdp == 128 ? launch_tile<128, false>(p, tmQ, tmK, tmV, st) : launch_tile<256, false>(p, tmQ, tmK, tmV, st));
+    }
     if (rc || a.weights == nullptr || a.keys == 0) return rc;
     const int rows_each = a.tokens * a.heads, warps = rows_each < 4 * WEIGHT_WARPS ? (rows_each + 3) / 4 : WEIGHT_WARPS;      // four rows or more for a warp
     const cudaError_t e = launch_pdl(key_weights_kernel, dim3((a.keys + 31) / 32, a.episodes), dim3(32 * warps), 0, st, p);

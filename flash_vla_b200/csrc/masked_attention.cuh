@@ -169,7 +169,7 @@ struct Walk {
     __device__ __forceinline__ bool sees(int i) const {
         if (range == nullptr) return true;
         const int2 r = __ldg(range + first + i);
-        return r.y >= max(q_low, 0) && r.x <= q_high;
+        return r.y >= q_low && r.x <= q_high;
     }
     __device__ __forceinline__ int next(int i) const {      // the first block from i on that is seen, or count
         while (i < count && !sees(i)) ++i;
@@ -242,8 +242,10 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
             const int blocks = (a.keys + BKEY - 1) / BKEY;
             for (int t = tid; t < tokens; t += C::THREADS) {
                 const int d = a.q_docs[(size_t)e * a.tokens + t0 + t];
-                atomicMin(shared_int, d);
-                atomicMax(shared_int + 1, d);
+                if (d >= 0) {                                  // padding sees nothing
+                    atomicMin(shared_int, d);
+                    atomicMax(shared_int + 1, d);
+                }
             }
             __syncthreads();
             walk.q_low = shared_int[0];
@@ -352,7 +354,7 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
         const int pos = s.start + t0 + t;
         const int limit = a.causal ? max(pos, s.prefix - 1) : 0x7fffffff;
         const int key_limit = a.k_pos || !a.causal ? s.L : min(s.L, limit < 0x7fffffff ? limit + 1 : limit);
-        const int doc = a.q_docs && mine ? a.q_docs[(size_t)e * a.tokens + t0 + t] : 0;
+        const int doc = a.q_docs && mine ? a.q_docs[(size_t)e * a.tokens + t0 + t] : -1;
         const float slope = a.slopes && mine ? a.slopes[h] * kLog2e : 0.f;
         const bool capped = a.cap > 0.f;
         float factor = capped ? a.scale / a.cap : a.scale * kLog2e;    // to the cap's argument, or straight to log2 units
@@ -453,15 +455,25 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                     see[0] = have >= 32 ? 0xffffffffu : (1u << have) - 1u;
                     see[1] = have >= 64 ? 0xffffffffu : (have > 32 ? (1u << (have - 32)) - 1u : 0u);
                 }
-                if (walk.range != nullptr || (a.k_pos && a.causal)) {
-                    const int* tag = (walk.range != nullptr ? a.k_docs : a.k_pos) + (size_t)e * a.keys;
-                    const bool docs = walk.range != nullptr;
+                if (walk.range != nullptr) {
+                    // a lane looks at two keys; one vote for each document among the warp's rows (one or two, as a rule)
+                    const int* tag = a.k_docs + (size_t)e * a.keys;
+                    const int low = __ldg(tag + min(key0 + lane, a.keys - 1)), high = __ldg(tag + min(key0 + 32 + lane, a.keys - 1));
+                    uint32_t left = __ballot_sync(0xffffffffu, doc >= 0);
+                    if (doc < 0) see[0] = see[1] = 0u;
+                    while (left) {
+                        const int d = __shfl_sync(0xffffffffu, doc, __ffs(left) - 1);
+                        const uint32_t b0 = __ballot_sync(0xffffffffu, low == d), b1 = __ballot_sync(0xffffffffu, high == d);
+                        if (doc == d) { see[0] &= b0; see[1] &= b1; }
+                        left &= ~__ballot_sync(0xffffffffu, doc == d);
+                    }
+                }
+                if (a.k_pos && a.causal) {
+                    const int* at = a.k_pos + (size_t)e * a.keys;
                     uint32_t seen[2] = {0u, 0u};
 #pragma unroll
-                    for (int c = 0; c < 64; ++c) {
-                        const int k = __ldg(tag + min(key0 + c, a.keys - 1));
-                        if (docs ? (k == doc && k >= 0) : k <= limit) seen[c >> 5] |= 1u << (c & 31);
-                    }
+                    for (int c = 0; c < 64; ++c)
+                        if (__ldg(at + min(key0 + c, a.keys - 1)) <= limit) seen[c >> 5] |= 1u << (c & 31);
                     see[0] &= seen[0];
                     see[1] &= seen[1];
                 }

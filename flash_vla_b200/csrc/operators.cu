@@ -101,7 +101,11 @@ int fvla_cache_append(const struct fvla_cache_append_args* a, void* stream) {
     p.starts = a->starts; p.counts = a->counts; p.status = device_status_ptr();
     p.tokens = a->tokens; p.rows = a->rows; p.blocks = a->rows / a->block; p.block = a->block; p.kv_heads = a->kv_heads; p.dim = a->head_dim;
     const int windows = (a->tokens + a->block - 2) / a->block + 1;           // blocks that a run of so many rows can touch
-    return launch("cache_append_kernel", q8::cache_append_kernel, dim3(windows * a->kv_heads, 2, a->episodes), dim3(q8::APPEND_THREADS), 0, S(stream), p);
+    const int chunks = a->block * a->head_dim / 16, threads = chunks < q8::APPEND_THREADS ? (chunks + 31) / 32 * 32 : q8::APPEND_THREADS;      // pieces of 16 values of a block
+    const dim3 grid(windows * a->kv_heads, 2, a->episodes);
+    const auto kern = chunks <= q8::APPEND_THREADS ? q8::cache_append_kernel<1> : (chunks <= 2 * q8::APPEND_THREADS ? q8::cache_append_kernel<2> :
+                      (chunks <= 4 * q8::APPEND_THREADS ? q8::cache_append_kernel<4> : q8::cache_append_kernel<8>));
+    return launch("cache_append_kernel", kern, grid, dim3(threads), 0, S(stream), p);
 }
 
 size_t fvla_cache_evict_workspace_bytes(int episodes, int keep) { return episodes > 0 && keep > 0 ? (size_t)episodes * keep * sizeof(int) : 0; }
@@ -136,7 +140,10 @@ int fvla_cache_evict(const struct fvla_cache_evict_args* a, void* stream) {
     p.kv_heads = a->kv_heads; p.dim = a->head_dim; p.keep = a->keep; p.sinks = a->sinks; p.recent = a->recent;
     int rc = launch("evict_select_kernel", q8::evict_select_kernel, dim3(a->episodes), dim3(q8::SELECT_THREADS), 0, S(stream), p);
     if (rc) return rc;
-    return launch("evict_move_kernel", q8::evict_move_kernel, dim3((a->keep + a->out_block - 1) / a->out_block * a->kv_heads, 2, a->episodes), dim3(q8::MOVE_THREADS), 0, S(stream), p);
+    const int chunks = a->out_block * a->head_dim / 16;
+    const auto move = chunks <= 2 * q8::MOVE_THREADS ? q8::evict_move_kernel<2> : (chunks <= 4 * q8::MOVE_THREADS ? q8::evict_move_kernel<4> :
+                      (chunks <= 8 * q8::MOVE_THREADS ? q8::evict_move_kernel<8> : q8::evict_move_kernel<16>));
+    return launch("evict_move_kernel", move, dim3((a->keep + a->out_block - 1) / a->out_block * a->kv_heads, 2, a->episodes), dim3(q8::MOVE_THREADS), 0, S(stream), p);
 }
 
 }  // extern "C"

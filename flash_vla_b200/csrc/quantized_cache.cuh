@@ -66,15 +66,17 @@ struct AppendArgs {
     int tokens, rows, blocks, block, kv_heads, dim;
 };
 
-constexpr int APPEND_THREADS = 128;
+constexpr int APPEND_THREADS = 256;
 
 // One CTA per (block that a run of new rows can touch and head, K or V, episode): its new rows' amax, the scale, then old rows moved to that scale
-// and new rows rounded. A thread takes 16 values at a time (32 bytes in, 16 out).
-__global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const AppendArgs p) {
+// and new rows rounded. A thread takes 16 values at a time (32 bytes in, 16 out) and keeps all of its PER pieces in registers between the two, so that
+// every byte is read once and all reads are in flight together; bound by the bytes.
+template <int PER>
+__global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const __grid_constant__ AppendArgs p) {
     __shared__ uint32_t warp_max[APPEND_THREADS / 32];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int e = blockIdx.z, kv = blockIdx.y, head = blockIdx.x % p.kv_heads, w = blockIdx.x / p.kv_heads;
+    const int e = blockIdx.z, kv = blockIdx.y, head = blockIdx.x % p.kv_heads, w = blockIdx.x / p.kv_heads, threads = blockDim.x;
     const long long start = p.starts[e];
     const int count = p.counts ? min(max(p.counts[e], 0), p.tokens) : p.tokens;
     if (count > 0 && (start < 0 || start + count > p.rows) && threadIdx.x == 0 && blockIdx.x == 0 && kv == 0 && p.status) atomicExch(p.status, 8);
@@ -88,41 +90,46 @@ __global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const Appe
     const bf16* x = p.x[kv] + e * p.xs[kv][0] + (row0 - start) * p.xs[kv][1] + head * p.xs[kv][2];
     uint8_t* held = p.held[kv] + e * p.hs[kv][0] + row0 * p.hs[kv][1] + head * p.hs[kv][2];
     float* scale = p.scale[kv] + ((size_t)e * p.blocks + b) * p.kv_heads + head;
+    const float was = old > 0 ? *scale : 0.f;
 
+    uint4 u[PER][2];
     uint32_t amax = 0;
-    for (int i = first * chunks + threadIdx.x; i < last * chunks; i += APPEND_THREADS) {
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int i = first * chunks + k * threads + threadIdx.x;
+        const bool mine = i < last * chunks;
         const uint4* src = reinterpret_cast<const uint4*>(x + (long long)(i / chunks) * p.xs[kv][1] + (i % chunks) * 16);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint4 u = __ldg(src + h);
-            amax = amax_pair(amax_pair(amax_pair(amax_pair(amax, u.x), u.y), u.z), u.w);
-        }
+        for (int h = 0; h < 2; ++h) u[k][h] = mine ? __ldg(src + h) : make_uint4(0, 0, 0, 0);
     }
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) amax = amax_pair(amax_pair(amax_pair(amax_pair(amax, u[k][h].x), u[k][h].y), u[k][h].z), u[k][h].w);
     amax = __reduce_max_sync(0xffffffffu, amax);
     if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = amax;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < APPEND_THREADS / 32; ++i) amax = max(amax, warp_max[i]);
-    const float needed = scale_of(amax), was = old > 0 ? *scale : 0.f, now = fmaxf(was, needed);
-    __syncthreads();                                             // every thread has read the old scale
+    __syncthreads();                                             // and every thread has read the old scale
+    for (int i = 0; i < threads / 32; ++i) amax = max(amax, warp_max[i]);
+    const float now = fmaxf(was, scale_of(amax));
     if (threadIdx.x == 0) *scale = now;
     if (now != was) {
         const float ratio = was * inverse_pow2(now);
-        for (int i = threadIdx.x; i < old * chunks; i += APPEND_THREADS) {
+        for (int i = threadIdx.x; i < old * chunks; i += threads) {
             uint4* at = reinterpret_cast<uint4*>(held + (long long)(i / chunks) * p.hs[kv][1] + (i % chunks) * 16);
-            uint4 u = *at;
-            *at = make_uint4(rescale4(u.x, ratio), rescale4(u.y, ratio), rescale4(u.z, ratio), rescale4(u.w, ratio));
+            const uint4 v = *at;
+            *at = make_uint4(rescale4(v.x, ratio), rescale4(v.y, ratio), rescale4(v.z, ratio), rescale4(v.w, ratio));
         }
     }
     const float inv = inverse_pow2(now);
-    for (int i = first * chunks + threadIdx.x; i < last * chunks; i += APPEND_THREADS) {
-        const uint4* src = reinterpret_cast<const uint4*>(x + (long long)(i / chunks) * p.xs[kv][1] + (i % chunks) * 16);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int i = first * chunks + k * threads + threadIdx.x;
+        if (i >= last * chunks) break;
         uint32_t o[4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint4 u = __ldg(src + h);
-            o[2 * h] = quantize_pair(u.x, inv) | (quantize_pair(u.y, inv) << 16);
-            o[2 * h + 1] = quantize_pair(u.z, inv) | (quantize_pair(u.w, inv) << 16);
+            o[2 * h] = quantize_pair(u[k][h].x, inv) | (quantize_pair(u[k][h].y, inv) << 16);
+            o[2 * h + 1] = quantize_pair(u[k][h].z, inv) | (quantize_pair(u[k][h].w, inv) << 16);
         }
         *reinterpret_cast<uint4*>(held + (long long)(i / chunks) * p.hs[kv][1] + (i % chunks) * 16) = make_uint4(o[0], o[1], o[2], o[3]);
     }
@@ -152,35 +159,56 @@ __device__ __forceinline__ uint32_t order_of(float w) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// One CTA per episode: the threshold by a radix select of 8 bits at a time, then one ordered pass that writes the rows which stay.
-__global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const EvictArgs p) {
+// One CTA per episode: the threshold by a radix select of 8 bits at a time, then the rows that stay, in order. For both each warp has a run of
+// rows of its own; lanes with equal digits add to the histogram together (weights are alike in their leading bits).
+__global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const __grid_constant__ EvictArgs p) {
+    constexpr int WARPS = SELECT_THREADS / 32;
     __shared__ uint32_t hist[256];
     __shared__ uint32_t s_prefix, s_left;
-    __shared__ int warp_sum[2][SELECT_THREADS / 32];
+    __shared__ int warp_ties[WARPS], warp_kept[WARPS];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int e = blockIdx.x, tid = threadIdx.x;
+    const int e = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int L = min(max(p.lengths[e], 0), p.rows);
     const int n = min(L, p.keep);
     const float* w = p.weights + (size_t)e * p.rows;
     const int low = min(p.sinks, L), high = max(low, L - p.recent);       // rows [low, high) compete
     const int wanted = n - low - (L - high);                              // and so many of them stay (sinks + recent <= keep)
-    uint32_t threshold = 0, ties = 0;
-    if (L > p.keep && wanted > 0) {
+    const int run = ((L + WARPS - 1) / WARPS + 31) / 32 * 32, begin = min(warp * run, L), end = min(begin + run, L);
+    const bool choose = L > p.keep;
+    uint32_t threshold = 0xffffffffu, ties = 0;                           // nothing lies above the largest order
+    if (choose && wanted > 0) {
         uint32_t prefix = 0, left = wanted;
         for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = tid; i < 256; i += SELECT_THREADS) hist[i] = 0;
+            if (tid < 256) hist[tid] = 0;
             __syncthreads();
-            for (int j = low + tid; j < high; j += SELECT_THREADS) {
-                const uint32_t u = order_of(w[j]);
-                if (shift == 24 || (u >> (shift + 8)) == prefix) atomicAdd(&hist[(u >> shift) & 255u], 1u);
+#pragma unroll 4
+            for (int j0 = begin; j0 < end; j0 += 32) {
+                const int j = j0 + lane;
+                const bool free = j < end && j >= low && j < high;
+                const uint32_t u = free ? order_of(w[j]) : 0;
+                const bool counts = free && (shift == 24 || (u >> (shift + 8)) == prefix);
+                const uint32_t digit = counts ? (u >> shift) & 255u : 256u;
+                const uint32_t same = __match_any_sync(0xffffffffu, digit);
+                if (counts && lane == __ffs(same) - 1) atomicAdd(&hist[digit], (uint32_t)__popc(same));
             }
             __syncthreads();
-            if (tid == 0) {
-                uint32_t d = 255, above = 0;
-                while (d > 0 && above + hist[d] < left) above += hist[d--];
-                s_prefix = (prefix << 8) | d;
-                s_left = left - above;
+            if (warp == 0) {
+                // lane i has the digits 255 - 8 i .. 248 - 8 i: the digit at which the rows from above reach `left`
+                uint32_t mine[8], sum = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) { mine[i] = hist[255 - 8 * lane - i]; sum += mine[i]; }
+                uint32_t upto = sum;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) { const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += x; }
+                uint32_t above = upto - sum;
+                if (above < left && upto >= left) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        if (above + mine[i] >= left) { s_prefix = (prefix << 8) | (uint32_t)(255 - 8 * lane - i); s_left = left - above; break; }
+                        above += mine[i];
+                    }
+                }
             }
             __syncthreads();
             prefix = s_prefix;
@@ -189,31 +217,48 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const Evic
         threshold = prefix;
         ties = left;                                                      // so many rows of exactly this weight stay, the first ones
     }
-    int kept = 0, equal = 0;                                              // before this round of rows
-    for (int j0 = 0; j0 < L; j0 += SELECT_THREADS) {
-        const int j = j0 + tid;
-        const bool inside = j < L, free = inside && j >= low && j < high && L > p.keep;
+    // what each warp's run has, then where its rows go
+    int tied = 0, kept = 0;
+#pragma unroll 4
+    for (int j0 = begin; j0 < end; j0 += 32) {
+        const int j = j0 + lane;
+        const bool inside = j < end, free = inside && choose && j >= low && j < high;
         const uint32_t u = free ? order_of(w[j]) : 0;
-        const bool tie = free && wanted > 0 && u == threshold;
+        tied += __popc(__ballot_sync(0xffffffffu, free && u == threshold));
+        kept += __popc(__ballot_sync(0xffffffffu, inside && (!free || u > threshold)));
+    }
+    if (lane == 0) { warp_ties[warp] = tied; warp_kept[warp] = kept; }
+    __syncthreads();
+    int ties_before = 0, kept_before = 0;
+    {
+        int x = warp_ties[lane], y = warp_kept[lane];                     // (32 warps)
+        const int own = x;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const int z = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += z; }
+        y += min(x, (int)ties) - min(x - own, (int)ties);                 // with the ties of the run that stay
+        const int all = y;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const int z = __shfl_up_sync(0xffffffffu, y, o); if (lane >= o) y += z; }
+        ties_before = __shfl_sync(0xffffffffu, x - own, warp);
+        kept_before = __shfl_sync(0xffffffffu, y - all, warp);
+    }
+    for (int j0 = begin; j0 < end; j0 += 32) {
+        const int j = j0 + lane;
+        const bool inside = j < end, free = inside && choose && j >= low && j < high;
+        const float x = inside ? w[j] : 0.f;
+        const uint32_t u = free ? order_of(x) : 0, below = (1u << lane) - 1u;
+        const bool tie = free && u == threshold;
         const uint32_t tie_mask = __ballot_sync(0xffffffffu, tie);
-        if ((tid & 31) == 0) warp_sum[0][tid >> 5] = __popc(tie_mask);
-        __syncthreads();
-        int tie_rank = equal + __popc(tie_mask & ((1u << (tid & 31)) - 1)), tie_all = 0;
-        for (int i = 0; i < SELECT_THREADS / 32; ++i) { if (i < (tid >> 5)) tie_rank += warp_sum[0][i]; tie_all += warp_sum[0][i]; }
-        const bool stays = inside && (!free || (wanted > 0 && (u > threshold || (tie && tie_rank < (int)ties))));
+        const bool stays = inside && (!free || u > threshold || (tie && ties_before + __popc(tie_mask & below) < (int)ties));
         const uint32_t mask = __ballot_sync(0xffffffffu, stays);
-        if ((tid & 31) == 0) warp_sum[1][tid >> 5] = __popc(mask);
-        __syncthreads();
-        int rank = kept + __popc(mask & ((1u << (tid & 31)) - 1)), all = 0;
-        for (int i = 0; i < SELECT_THREADS / 32; ++i) { if (i < (tid >> 5)) rank += warp_sum[1][i]; all += warp_sum[1][i]; }
         if (stays) {
+            const int rank = kept_before + __popc(mask & below);
             p.source[(size_t)e * p.keep + rank] = j;
-            if (p.out_weights) p.out_weights[(size_t)e * p.out_rows + rank] = w[j];
+            if (p.out_weights) p.out_weights[(size_t)e * p.out_rows + rank] = x;
             if (p.out_positions) p.out_positions[(size_t)e * p.out_rows + rank] = p.positions ? p.positions[(size_t)e * p.rows + j] : j;
         }
-        kept += all;
-        equal += tie_all;
-        __syncthreads();
+        ties_before += __popc(tie_mask);
+        kept_before += __popc(mask);
     }
     if (tid == 0) p.out_lengths[e] = n;
 }
@@ -221,35 +266,45 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const Evic
 constexpr int MOVE_THREADS = 128;
 
 // One CTA per (block of the result and head, K or V, episode): its scale is the largest of its rows' source scales; rows of another scale
-// are moved to it by a power of two.
-__global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const EvictArgs p) {
+// are moved to it by a power of two. Rows are fetched, PER pieces of 16 bytes a thread in flight, while the scales are looked up.
+template <int PER>
+__global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const __grid_constant__ EvictArgs p) {
     __shared__ int row_of[128];
     __shared__ float scale_of_row[128];
+    __shared__ float warp_top[MOVE_THREADS / 32];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int e = blockIdx.z, kv = blockIdx.y, head = blockIdx.x % p.kv_heads, b = blockIdx.x / p.kv_heads, tid = threadIdx.x;
     const int n = min(min(max(p.lengths[e], 0), p.rows), p.keep);
     const int row0 = b * p.out_block, have = min(p.out_block, n - row0);
     if (have <= 0) return;
-    for (int i = tid; i < have; i += MOVE_THREADS) {
-        const int j = p.source[(size_t)e * p.keep + row0 + i];
-        row_of[i] = j;
-        scale_of_row[i] = p.scale[kv][((size_t)e * p.blocks + j / p.block) * p.kv_heads + head];
-    }
+    const int j = tid < have ? p.source[(size_t)e * p.keep + row0 + tid] : 0;
+    row_of[tid] = j;
     __syncthreads();
-    float now = 0.f;
-    for (int i = 0; i < have; ++i) now = fmaxf(now, scale_of_row[i]);
-    if (tid == 0) p.out_scale[kv][((size_t)e * p.out_blocks + b) * p.kv_heads + head] = now;
-    const float inv = inverse_pow2(now);
     const int chunks = p.dim / 16;
     const uint8_t* held = p.held[kv] + e * p.hs[kv][0] + head * p.hs[kv][2];
     uint8_t* out = p.out[kv] + e * p.os[kv][0] + (long long)row0 * p.os[kv][1] + head * p.os[kv][2];
-    for (int i = tid; i < have * chunks; i += MOVE_THREADS) {
-        const int r = i / chunks, c = i % chunks;
-        uint4 u = __ldg(reinterpret_cast<const uint4*>(held + row_of[r] * p.hs[kv][1] + c * 16));
+    float top = tid < have ? p.scale[kv][((size_t)e * p.blocks + j / p.block) * p.kv_heads + head] : 0.f;
+    uint4 u[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int i = k * MOVE_THREADS + tid;
+        u[k] = i < have * chunks ? __ldg(reinterpret_cast<const uint4*>(held + row_of[i / chunks] * p.hs[kv][1] + i % chunks * 16)) : make_uint4(0, 0, 0, 0);
+    }
+    scale_of_row[tid] = top;
+    top = warp_max(top);
+    if ((tid & 31) == 0) warp_top[tid >> 5] = top;
+    __syncthreads();
+    const float now = fmaxf(fmaxf(warp_top[0], warp_top[1]), fmaxf(warp_top[2], warp_top[3]));
+    if (tid == 0) p.out_scale[kv][((size_t)e * p.out_blocks + b) * p.kv_heads + head] = now;
+    const float inv = inverse_pow2(now);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int i = k * MOVE_THREADS + tid, r = i / chunks;
+        if (i >= have * chunks) break;
         const float ratio = scale_of_row[r] * inv;
-        if (ratio != 1.f) u = make_uint4(rescale4(u.x, ratio), rescale4(u.y, ratio), rescale4(u.z, ratio), rescale4(u.w, ratio));
-        *reinterpret_cast<uint4*>(out + r * p.os[kv][1] + c * 16) = u;
+        if (ratio != 1.f) u[k] = make_uint4(rescale4(u[k].x, ratio), rescale4(u[k].y, ratio), rescale4(u[k].z, ratio), rescale4(u[k].w, ratio));
+        *reinterpret_cast<uint4*>(out + r * p.os[kv][1] + i % chunks * 16) = u[k];
     }
 }
 

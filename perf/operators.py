@@ -345,10 +345,10 @@ def _plain(s):
 
 # ------------------------------------------------------------------------------------------------ the framework's calls
 def _own(s):
-    from flash_vla_b200 import op_table
-    from flash_vla_b200.hardware.nvidia.b200.pi0.buffers import QuantizedCache
     ops = s.get("ops")
-    if ops is None:                      # a program builds its table once
+    if ops is None:                      # a program imports the package and builds its table once
+        from flash_vla_b200 import op_table
+        from flash_vla_b200.hardware.nvidia.b200.pi0.buffers import QuantizedCache
         ops = s["ops"] = op_table()
         for name in ("cache", "out_cache"):
             if name in s:

@@ -664,53 +664,54 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
     if (tid == 0 && *abort_flag && p.status) atomicExch(p.status, 9);
 }
 
-// The shares' sums against the largest of their maxima. `warps` of a CTA take a row together: each adds up every warps-th share, and the first adds
-// up the warps in their order.
+// The shares' sums against the largest of their maxima. `warps` of a CTA take 32 * PER columns of a row together (grid.y: which): each adds up every
+// warps-th share, and the first adds up the warps in their order.
 constexpr int JOIN_WARPS = 8;
-template <int HDP>
-__global__ void __launch_bounds__(32 * JOIN_WARPS) attention_join_kernel(const __grid_constant__ Tile p, int warps) {
-    __shared__ float sums[JOIN_WARPS][HDP + 1];
+template <int PER>
+__global__ void __launch_bounds__(32 * JOIN_WARPS) attention_join_kernel(const __grid_constant__ Tile p, int hdp, int warps) {
+    __shared__ float sums[JOIN_WARPS][32 * PER + 1];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const Args& a = p.a;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % warps;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % warps, col0 = blockIdx.y * 32 * PER + lane;
     const long long row = (long long)blockIdx.x * (JOIN_WARPS / warps) + warp / warps, rows = (long long)a.episodes * a.tokens * a.heads;
     const int h = (int)(row % a.heads), t = (int)(row / a.heads % a.tokens), e = (int)min(row / a.heads / a.tokens, (long long)a.episodes - 1);
     const bool mine = row < rows && t < episode_of(a, e).n;
     float m = -INFINITY;
-    if (mine)
+    if (mine) {
+#pragma unroll 4
         for (int s = lane; s < p.splits; s += 32) {
             const float2 ml = p.part_ml[s * rows + row];
             if (ml.y != 0.f) m = fmaxf(m, ml.x);
         }
+    }
     m = warp_max(m);
     const float top = m == -INFINITY ? 0.f : m;
-    constexpr int PER = HDP / 32;                                                    // columns lane, lane + 32, ...
-    float acc[PER], l = 0.f;
+    float acc[PER], l = 0.f;                                                         // columns lane, lane + 32, ...
 #pragma unroll
     for (int c = 0; c < PER; ++c) acc[c] = 0.f;
     if (mine) {
-#pragma unroll 4
+#pragma unroll (PER == 1 ? 8 : 4)
         for (int s = part; s < p.splits; s += warps) {
             const float2 ml = p.part_ml[s * rows + row];
-            if (ml.y == 0.f) continue;                                               // this share held nothing that the row sees
+            const bool used = ml.y != 0.f;                                           // else this share held nothing that the row sees
             const float w = ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - top);
-            l = fmaf(ml.y, w, l);
-            const float* o = p.part_o + (s * rows + row) * HDP + lane;
+            const float* o = p.part_o + (s * rows + row) * hdp + col0;
+            l = used ? fmaf(ml.y, w, l) : l;
 #pragma unroll
-            for (int c = 0; c < PER; ++c) acc[c] = fmaf(w, o[32 * c], acc[c]);
+            for (int c = 0; c < PER; ++c) { const float x = used ? o[32 * c] : 0.f; acc[c] = fmaf(used ? w : 0.f, x, acc[c]); }
         }
     }
     if (warps > 1) {
 #pragma unroll
         for (int c = 0; c < PER; ++c) sums[warp][lane + 32 * c] = acc[c];
-        if (lane == 0) sums[warp][HDP] = l;
+        if (lane == 0) sums[warp][32 * PER] = l;
         __syncthreads();
         if (part != 0) return;
         for (int w = 1; w < warps; ++w) {
 #pragma unroll
             for (int c = 0; c < PER; ++c) acc[c] += sums[warp + w][lane + 32 * c];
-            l += sums[warp + w][HDP];
+            l += sums[warp + w][32 * PER];
         }
     }
     if (!mine) return;
@@ -718,8 +719,8 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) attention_join_kernel(const _
     bf16* dst = a.out + e * a.os[0] + t * a.os[1] + h * a.os[2];
 #pragma unroll
     for (int c = 0; c < PER; ++c)
-        if (lane + 32 * c < a.dim) dst[lane + 32 * c] = __float2bfloat16_rn(acc[c] * inv);
-    if (a.lse && lane == 0) a.lse[((size_t)e * a.heads + h) * a.tokens + t] = l > 0.f ? (top + log2f(l)) * 0.6931471805599453f : (l == 0.f ? -INFINITY : l);
+        if (col0 + 32 * c < a.dim) dst[col0 + 32 * c] = __float2bfloat16_rn(acc[c] * inv);
+    if (a.lse && lane == 0 && blockIdx.y == 0) a.lse[((size_t)e * a.heads + h) * a.tokens + t] = l > 0.f ? (top + log2f(l)) * 0.6931471805599453f : (l == 0.f ? -INFINITY : l);
 }
 
 // weights[e][j] = decay * weights[e][j] + the probabilities that key j got, from the scores that the attention left and the rows' log-sum-exps. A CTA
@@ -805,11 +806,12 @@ inline size_t workspace_bytes(const Args& a) {
     return n;
 }
 
-template <int HDP>
-inline int launch_join(const Tile& p, cudaStream_t st) {
+inline int launch_join(const Tile& p, int hdp, cudaStream_t st) {
     const long long rows = (long long)p.a.episodes * p.a.tokens * p.a.heads;
-    const int warps = p.splits >= 16 ? 8 : (p.splits >= 8 ? 4 : (p.splits >= 4 ? 2 : 1)), each = JOIN_WARPS / warps;
-    const cudaError_t e = launch_pdl(attention_join_kernel<HDP>, dim3((unsigned)((rows + each - 1) / each)), dim3(32 * JOIN_WARPS), 0, st, p, warps);
+    // many shares: eight warps for 32 columns of a row; few: a warp or some for the whole row
+    const int warps = p.splits >= 16 ? 8 : (p.splits >= 8 ? 4 : (p.splits >= 4 ? 2 : 1)), each = JOIN_WARPS / warps, per = p.splits >= 16 ? 1 : hdp / 32;
+    const auto kern = per == 1 ? attention_join_kernel<1> : (per == 2 ? attention_join_kernel<2> : (per == 4 ? attention_join_kernel<4> : attention_join_kernel<8>));
+    const cudaError_t e = launch_pdl(kern, dim3((unsigned)((rows + each - 1) / each), hdp / (32 * per)), dim3(32 * JOIN_WARPS), 0, st, p, hdp, warps);
     if (e != cudaSuccess) { set_error("attention_join_kernel: %s", cudaGetErrorString(e)); return FVLA_ERR_LAUNCH; }
     return check_launch("attention_join_kernel");
 }
@@ -828,7 +830,7 @@ inline int launch_tile(const Tile& p, const CUtensorMap& tmQ, const CUtensorMap&
     cudaError_t e = launch_pdl(kern, dim3(p.tiles * p.splits, a.kv_heads, a.episodes), dim3(C::THREADS), C::SMEM, st, p, tmQ, tmK, tmV);
     if (e != cudaSuccess) { set_error("attention_tile_kernel: %s", cudaGetErrorString(e)); return FVLA_ERR_LAUNCH; }
     int rc = check_launch("attention_tile_kernel");
-    return rc || p.splits == 1 ? rc : launch_join<HDP>(p, st);
+    return rc || p.splits == 1 ? rc : launch_join(p, HDP, st);
 }
 
 inline int launch_attention(const Args& a, void* ws, int* status, cudaStream_t st) {
@@ -863,18 +865,17 @@ inline int launch_attention(const Args& a, void* ws, int* status, cudaStream_t s
     }
     p.part_ml = reinterpret_cast<float2*>(at);
     p.part_o = reinterpret_cast<float*>(at + align256(p.splits * rows * sizeof(float2)));
-    CUtensorMap tmQ, tmK, tmV;
+    CUtensorMap tmQ = {}, tmK = {}, tmV = {};
     const bool few = takes_few(a), q8 = a.k_scale != nullptr;
     p.q_mul[0] = 1;
     p.q_mul[1] = a.qs[0] != 0;
-    {
+    if (!few) {
         const uint64_t dims[5] = {(uint64_t)a.dim, (uint64_t)p.group, (uint64_t)a.tokens, (uint64_t)a.kv_heads, p.q_mul[1] ? (uint64_t)a.episodes : 1};
         const uint64_t strides[4] = {(uint64_t)a.qs[2], (uint64_t)a.qs[1], (uint64_t)a.qs[2] * p.group, p.q_mul[1] ? (uint64_t)a.qs[0] : 256};
         const uint32_t box[5] = {64, (uint32_t)p.group, (uint32_t)p.tile_tokens, 1, 1};
         const int rc = make_map(&tmQ, a.q, 5, dims, strides, box);
         if (rc) return rc;
     }
-    tmK = tmV = tmQ;
     p.k_mul[0] = a.ks[2] != 0; p.k_mul[1] = a.ks[0] != 0; p.v_mul[0] = a.vs[2] != 0; p.v_mul[1] = a.vs[0] != 0;
     if ((few || !q8) && a.keys > 0) {
         for (int i = 0; i < 2; ++i) {
@@ -891,7 +892,7 @@ inline int launch_attention(const Args& a, void* ws, int* status, cudaStream_t s
     if (few) {
         if (q8) rc = hdp == 128 ? launch_few<128, true>(p, tmK, tmV, st) : launch_few<256, true>(p, tmK, tmV, st);
         else rc = hdp == 128 ? launch_few<128, false>(p, tmK, tmV, st) : launch_few<256, false>(p, tmK, tmV, st);
-        if (!rc) rc = hdp == 128 ? launch_join<128>(p, st) : launch_join<256>(p, st);
+        if (!rc) rc = launch_join(p, hdp, st);
     } else if (q8) {
         rc = hdp == 64 ? launch_tile<64, true>(p, tmQ, tmK, tmV, st) : (hdp == 128 ? launch_tile<128, true>(p, tmQ, tmK, tmV, st) : launch_tile<256, true>(p, tmQ, tmK, tmV, st));
     } else {

@@ -103,9 +103,9 @@ SIGNATURES: dict[str, list] = {
     "fvla_encoder_layers_run": [ctypes.POINTER(EncoderLayers), _P],
     "fvla_embed_rows": [_P, _P, _P, _I, _I, ctypes.c_longlong, _P],
     "fvla_convert_copy": [_P, _I, _P, _I, _P, _Z, _P],
-    "fvla_attention_run": [ctypes.POINTER(Attention), _P],
-    "fvla_cache_append": [ctypes.POINTER(CacheAppend), _P],
-    "fvla_cache_evict": [ctypes.POINTER(CacheEvict), _P],
+    "fvla_attention_run": [_P, _P],      # the three below: Attention, CacheAppend and CacheEvict, by reference or as their bytes
+    "fvla_cache_append": [_P, _P],
+    "fvla_cache_evict": [_P, _P],
     "fvla_selftest_wait_timeout": [_P, _P, _P, _I, _I, _I, ctypes.c_uint, _P],
     "fvla_gemm_plan_set": [_I, _I, _I, _I, _I, _I, _I],
     "fvla_gemm_plan_clear": [],

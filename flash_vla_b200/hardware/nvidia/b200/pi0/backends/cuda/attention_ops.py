@@ -17,6 +17,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import struct
 
 import torch
 
@@ -76,9 +77,22 @@ def _cache_layout(c):
     return tuple(t.shape for t in c), tuple(t.stride() for t in c), tuple(t.dtype for t in c)
 
 
+# The argument blocks of the C entries (`_lib.Attention` and so on) are put together as bytes, addresses first, then what a layout determines and a plan
+# remembers: setting some forty ctypes fields costs more than the launch.
+_ATTENTION_HEAD, _FLOATS, _CAUSAL = struct.Struct("17PQ"), struct.Struct("3f"), struct.Struct("ii")
+_APPEND_HEAD, _EVICT_HEAD = struct.Struct("8P"), struct.Struct("15PQ")
+
+
+def _between(block, first, last):
+    """The bytes of a ctypes structure from field `first` up to field `last` (the end, where there is none)."""
+    end = getattr(type(block), last).offset if last else ctypes.sizeof(block)
+    return bytes(block)[getattr(type(block), first).offset:end]
+
+
 @functools.lru_cache(maxsize=1024)
 def _attention_plan(q, k, v, out, cache):
-    """(argument block without addresses, scratch bytes without and with documents or weights) of an attention with operands of these layouts; `cache`: layout of a QuantizedCache, or None."""
+    """What operands of these layouts determine of an attention's argument block: (strides, dimensions, scratch bytes without and with documents or
+    weights, episodes, tokens, keys, heads). `cache`: layout of a QuantizedCache, or None."""
     a = _lib.Attention()
     if cache is None:
         multiple, want, dim_multiple = 8, torch.bfloat16, 8
@@ -102,27 +116,25 @@ def _attention_plan(q, k, v, out, cache):
     a.episodes, a.tokens, a.keys, a.heads, a.kv_heads, a.head_dim = E, T, S, H, HK, D
     nbytes = [0, 0]
     for i, extra in enumerate(((), ("q_docs", "k_docs") if cache is None else ("weights", "lse"))):
-        b = _copy(a)
+        b = type(a).from_buffer_copy(a)
         for name in ("q", "out", "k", "v", *(("k_scale", "v_scale") if cache is not None else ()), *extra):
             setattr(b, name, 16)                # an address that only says that there is a tensor
         if E and T:
             nbytes[i] = _lib.load().fvla_attention_workspace_bytes(ctypes.byref(b))
-    return a, nbytes
+    return _between(a, "q_stride", "scale"), _between(a, "episodes", "causal"), nbytes, E, T, S, H
 
 
 def _vector(name, t, shape, dtype, device):
-    """Address of an optional small operand. (Without a GPU the large operands, which come last, are the ones refused for their device.)"""
-    if t is None:
-        return None
+    """Address of a small operand. (Without a GPU the large operands, which come last, are the ones refused for their device.)"""
+    if t.dtype is dtype and t.shape == shape and t.is_contiguous() and (t.get_device() == device or device < 0):
+        return t.data_ptr()
     if t.dtype != dtype:
         raise ValueError(f"{name}: expected {dtype}, got {t.dtype}")
     if t.shape != shape:
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     if not t.is_contiguous():
         raise ValueError(f"{name}: expected a contiguous tensor, got strides {t.stride()}")
-    if t.get_device() != device and device >= 0:
-        raise ValueError(f"{name}: expected a tensor on the current CUDA device, got {t.device}")
-    return t.data_ptr()
+    raise ValueError(f"{name}: expected a tensor on the current CUDA device, got {t.device}")
 
 
 def _address(name, t, device):
@@ -136,24 +148,26 @@ def _address(name, t, device):
 
 
 def _device():
-    return torch._C._cuda_getDevice() if torch.cuda.is_available() else -2      # -1 is the CPU's number
+    try:
+        return torch._C._cuda_getDevice()
+    except Exception:
+        return -2                               # no GPU (-1 is the number of the CPU)
 
 
-def _scratch(role, nbytes, like):
-    if not nbytes:
-        return None
+def _scratch(role, nbytes, device):
     if _w.default_pool():
-        return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
-    return _w.scratch(role, (nbytes,), torch.uint8, like.device)
-
-
-def _copy(struct):
-    return type(struct).from_buffer_copy(struct)
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return _w.scratch(role, (nbytes,), torch.uint8, device)
 
 
 def _attend(Q, K, V, cache, scale, out, causal, prefix, q_lens, k_lens, q_start, q_docs, k_docs, k_pos, cap, slopes, lse, weights, decay):
-    plan, nbytes = _attention_plan(_layout(Q), None if cache else _layout(K), None if cache else _layout(V), _layout(out), _cache_layout(cache) if cache else None)
-    E, T, S, H = plan.episodes, plan.tokens, plan.keys, plan.heads
+    if cache is None:
+        K_scale = V_scale = None
+        plan = _attention_plan(_layout(Q), _layout(K), _layout(V), _layout(out), None)
+    else:
+        K, V, K_scale, V_scale = cache
+        plan = _attention_plan(_layout(Q), None, None, _layout(out), _cache_layout(cache))
+    strides, dims, nbytes, E, T, S, H = plan
     scale, cap, decay = float(scale), float(cap or 0.0), float(decay)
     if not math.isfinite(scale) or not (0.0 <= cap < math.inf) or not math.isfinite(decay):
         raise ValueError(f"attention: scale {scale}, cap {cap}, decay {decay}: finite numbers, the cap not negative")
@@ -161,31 +175,32 @@ def _attend(Q, K, V, cache, scale, out, causal, prefix, q_lens, k_lens, q_start,
         raise ValueError("attention: a prefix without the causal mask")
     if (q_docs is None) != (k_docs is None):
         raise ValueError("attention: documents of queries and keys, or of neither")
-    device, a = _device(), _copy(plan)
-    a.prefix, a.q_lens = _vector("prefix", prefix, (E,), _INT32, device), _vector("q_lens", q_lens, (E,), _INT32, device)
-    a.k_lens, a.q_start = _vector("k_lens", k_lens, (E,), _INT32, device), _vector("q_start", q_start, (E,), _INT32, device)
-    a.q_docs, a.k_docs = _vector("q_docs", q_docs, (E, T), _INT32, device), _vector("k_docs", k_docs, (E, S), _INT32, device)
-    a.k_pos, a.slopes = _vector("k_pos", k_pos, (E, S), _INT32, device), _vector("slopes", slopes, (H,), _F32, device)
-    a.lse, a.weights = _vector("lse", lse, (E, H, T), _F32, device), _vector("weights", weights, (E, S), _F32, device)
-    a.scale, a.cap, a.decay, a.causal = scale, cap, decay, int(bool(causal))
-    a.q, a.out = _address("Q", Q, device), _address("out", out, device)
-    if cache:
-        a.k, a.v = _address("cache.K", cache[0], device), _address("cache.V", cache[1], device)
-        a.k_scale, a.v_scale = _vector("cache.K_scale", cache[2], cache[2].shape, _F32, device), _vector("cache.V_scale", cache[3], cache[3].shape, _F32, device)
-    else:
-        a.k, a.v = _address("K", K, device), _address("V", V, device)
+    device = _device()
+    prefix = 0 if prefix is None else _vector("prefix", prefix, (E,), _INT32, device)
+    q_lens = 0 if q_lens is None else _vector("q_lens", q_lens, (E,), _INT32, device)
+    k_lens = 0 if k_lens is None else _vector("k_lens", k_lens, (E,), _INT32, device)
+    q_start = 0 if q_start is None else _vector("q_start", q_start, (E,), _INT32, device)
+    q_docs = 0 if q_docs is None else _vector("q_docs", q_docs, (E, T), _INT32, device)
+    k_docs = 0 if k_docs is None else _vector("k_docs", k_docs, (E, S), _INT32, device)
+    k_pos = 0 if k_pos is None else _vector("k_pos", k_pos, (E, S), _INT32, device)
+    slopes = 0 if slopes is None else _vector("slopes", slopes, (H,), _F32, device)
+    lse = 0 if lse is None else _vector("lse", lse, (E, H, T), _F32, device)
+    weights = 0 if weights is None else _vector("weights", weights, (E, S), _F32, device)
+    if cache is not None:
+        K_scale, V_scale = _vector("cache.K_scale", K_scale, K_scale.shape, _F32, device), _vector("cache.V_scale", V_scale, V_scale.shape, _F32, device)
+    q, k, v, o = _address("Q", Q, device), _address("K", K, device), _address("V", V, device), _address("out", out, device)
     if E == 0 or T == 0:
         return out
-    if weights is not None:
-        if a.out == a.q:
-            raise ValueError("attention: the weights are taken from Q, which out would overwrite")
-        if lse is None:
-            held = _scratch("attention_lse", 4 * E * H * T, Q)
-            a.lse = held.data_ptr()
-    ws = _scratch("attention_ws", nbytes[q_docs is not None or weights is not None], Q)
-    if ws is not None:
-        a.ws, a.ws_bytes = ws.data_ptr(), ws.numel()
-    _lib.call("fvla_attention_run", ctypes.byref(a), _w._stream())
+    if weights and o == q:
+        raise ValueError("attention: the weights are taken from Q, which out would overwrite")
+    if weights and not lse:
+        held = _scratch("attention_lse", 4 * E * H * T, Q.device)
+        lse = held.data_ptr()
+    need = nbytes[1 if q_docs or weights else 0]
+    ws = _scratch("attention_ws", need, Q.device) if need else None
+    block = _ATTENTION_HEAD.pack(q, k, v, K_scale or 0, V_scale or 0, o, lse, weights, ws.data_ptr() if need else 0, prefix, q_lens, k_lens, q_start, q_docs, k_docs,
+                                 k_pos, slopes, need) + strides + _FLOATS.pack(scale, cap, decay) + dims + _CAUSAL.pack(1 if causal else 0, 0)
+    _lib.call("fvla_attention_run", block, torch._C._cuda_getCurrentRawStream(device))
     return out
 
 
@@ -212,7 +227,6 @@ def cache_attention(Q, cache, lengths, scale, out, causal=False, prefix=None, q_
     number; a cache that `cache_evict` has thinned out needs both for `causal`, `prefix` (then positions below `prefix`) and `slopes`.
     weights (E, rows) fp32: weights = decay * weights + the probability mass that each row received from all queries and heads; rows
     behind `lengths` stay as they were. decay = 0 overwrites. `out` may be Q, unless weights are asked for."""
-    cache = tuple(cache)
     return _attend(Q, None, None, cache, scale, out, causal, prefix, q_lens, lengths, q_start, None, None, k_pos, cap, slopes, lse, weights, decay)
 
 
@@ -233,7 +247,7 @@ def _append_plan(k, v, cache):
     if E >= 1 << 16 or rows >= 1 << 31 or HK == 0:
         raise ValueError(f"cache_append: a cache of {tuple(cache[0][0])}")
     a.episodes, a.tokens, a.rows, a.kv_heads, a.head_dim = E, T, rows, HK, D
-    return a
+    return _between(a, "k_stride", None), E, T
 
 
 def cache_append(K, V, cache, starts, counts=None):
@@ -242,15 +256,16 @@ def cache_append(K, V, cache, starts, counts=None):
     The scale of a block is the smallest power of two that brings its new values into e4m3's range, or the block's own where that is larger and the
     block holds rows before starts[e]; where it has grown, those rows are moved to it. Rows behind the new ones are taken to be unused. Values
     that are not finite become NaN and leave the scale alone. Rows that would lie outside the cache are left out (device status 8)."""
-    cache = tuple(cache)
-    plan = _append_plan(_layout(K), _layout(V), _cache_layout(cache))
-    device, a = _device(), _copy(plan)
-    a.starts, a.counts = _vector("starts", starts, (plan.episodes,), _INT32, device), _vector("counts", counts, (plan.episodes,), _INT32, device)
-    a.k, a.v = _address("K", K, device), _address("V", V, device)
-    a.k_held, a.v_held = _address("cache.K", cache[0], device), _address("cache.V", cache[1], device)
-    a.k_scale, a.v_scale = _vector("cache.K_scale", cache[2], cache[2].shape, _F32, device), _vector("cache.V_scale", cache[3], cache[3].shape, _F32, device)
-    if plan.episodes and plan.tokens:
-        _lib.call("fvla_cache_append", ctypes.byref(a), _w._stream())
+    held_k, held_v, k_scale, v_scale = cache
+    rest, E, T = _append_plan(_layout(K), _layout(V), _cache_layout(cache))
+    device = _device()
+    starts = _vector("starts", starts, (E,), _INT32, device)
+    counts = 0 if counts is None else _vector("counts", counts, (E,), _INT32, device)
+    k_scale, v_scale = _vector("cache.K_scale", k_scale, k_scale.shape, _F32, device), _vector("cache.V_scale", v_scale, v_scale.shape, _F32, device)
+    block = _APPEND_HEAD.pack(_address("K", K, device), _address("V", V, device), _address("cache.K", held_k, device), _address("cache.V", held_v, device),
+                              k_scale, v_scale, starts, counts) + rest
+    if E and T:
+        _lib.call("fvla_cache_append", block, torch._C._cuda_getCurrentRawStream(device))
 
 
 @functools.lru_cache(maxsize=1024)
@@ -271,12 +286,9 @@ def _evict_plan(cache, out, keep, sinks, recent):
     if E >= 1 << 16 or rows >= 1 << 31 or HK == 0:
         raise ValueError(f"cache_evict: a cache of {tuple(cache[0][0])}")
     a.episodes, a.rows, a.out_rows, a.kv_heads, a.head_dim, a.keep, a.sinks, a.recent = E, rows, out_rows, HK, D, keep, sinks, recent
-    return a, _lib.load().fvla_cache_evict_workspace_bytes(E, keep)
-
-
-def _span(t):
-    """First and last byte of a tensor's memory."""
-    return t.data_ptr(), t.data_ptr() + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) * t.element_size()
+    extent = lambda layout, i: 1 + sum((n - 1) * st for n, st in zip(layout[0][i], layout[1][i]))      # noqa: E731  bytes of an 8-bit operand
+    return (_between(a, "k_stride", None), _lib.load().fvla_cache_evict_workspace_bytes(E, keep), E, rows, out_rows,
+            (extent(cache, 0), extent(cache, 1), extent(out, 0), extent(out, 1)))
 
 
 def cache_evict(cache, lengths, weights, keep, out_cache, out_lengths, out_weights=None, positions=None, out_positions=None, sinks=0, recent=0):
@@ -286,30 +298,40 @@ def cache_evict(cache, lengths, weights, keep, out_cache, out_lengths, out_weigh
     `cache_attention` adds them up; equal weights: the first rows; NaN: as -inf). out_lengths (E,) receives their number; out_weights
     (E, out rows) fp32 and out_positions (E, out rows) int32 what weight and position each had (positions (E, rows), or the row numbers). A block's
     scale is the largest among its rows', and values are rounded again where theirs was smaller. What lies behind the last row stays as it was."""
-    cache, out_cache = tuple(cache), tuple(out_cache)
-    plan, nbytes = _evict_plan(_cache_layout(cache), _cache_layout(out_cache), int(keep), int(sinks), int(recent))
-    E, rows, out_rows = plan.episodes, plan.rows, plan.out_rows
-    device, a = _device(), _copy(plan)
-    a.lengths, a.out_lengths = _vector("lengths", lengths, (E,), _INT32, device), _vector("out_lengths", out_lengths, (E,), _INT32, device)
-    a.weights, a.out_weights = _vector("weights", weights, (E, rows), _F32, device), _vector("out_weights", out_weights, (E, out_rows), _F32, device)
-    a.positions, a.out_positions = _vector("positions", positions, (E, rows), _INT32, device), _vector("out_positions", out_positions, (E, out_rows), _INT32, device)
-    a.k, a.v = _address("cache.K", cache[0], device), _address("cache.V", cache[1], device)
-    a.out_k, a.out_v = _address("out_cache.K", out_cache[0], device), _address("out_cache.V", out_cache[1], device)
-    a.k_scale, a.v_scale = _vector("cache.K_scale", cache[2], cache[2].shape, _F32, device), _vector("cache.V_scale", cache[3], cache[3].shape, _F32, device)
-    a.out_k_scale = _vector("out_cache.K_scale", out_cache[2], out_cache[2].shape, _F32, device)
-    a.out_v_scale = _vector("out_cache.V_scale", out_cache[3], out_cache[3].shape, _F32, device)
+    held_k, held_v, k_scale, v_scale = cache
+    to_k, to_v, to_k_scale, to_v_scale = out_cache
+    rest, nbytes, E, rows, out_rows, extents = _evict_plan(_cache_layout(cache), _cache_layout(out_cache), int(keep), int(sinks), int(recent))
+    device = _device()
+    n, out_n = _vector("lengths", lengths, (E,), _INT32, device), _vector("out_lengths", out_lengths, (E,), _INT32, device)
+    w = _vector("weights", weights, (E, rows), _F32, device)
+    out_w = 0 if out_weights is None else _vector("out_weights", out_weights, (E, out_rows), _F32, device)
+    pos = 0 if positions is None else _vector("positions", positions, (E, rows), _INT32, device)
+    out_pos = 0 if out_positions is None else _vector("out_positions", out_positions, (E, out_rows), _INT32, device)
+    ks, vs = _vector("cache.K_scale", k_scale, k_scale.shape, _F32, device), _vector("cache.V_scale", v_scale, v_scale.shape, _F32, device)
+    to_ks = _vector("out_cache.K_scale", to_k_scale, to_k_scale.shape, _F32, device)
+    to_vs = _vector("out_cache.V_scale", to_v_scale, to_v_scale.shape, _F32, device)
+    k, v = _address("cache.K", held_k, device), _address("cache.V", held_v, device)
+    to_k, to_v = _address("out_cache.K", to_k, device), _address("out_cache.V", to_v, device)
     if E == 0:
         return
-    reads = [cache[0], cache[1], cache[2], cache[3], weights, lengths] + ([positions] if positions is not None else [])
-    writes = [*out_cache, out_lengths] + [t for t in (out_weights, out_positions) if t is not None]
-    spans = [_span(t) for t in reads]
-    for t in writes:
-        low, high = _span(t)
-        if any(low <= b and a_ <= high for a_, b in spans):
-            raise ValueError("cache_evict: a destination lies over what it is made of")
-    ws = _scratch("evict_ws", nbytes, weights)
-    a.ws, a.ws_bytes = ws.data_ptr(), nbytes
-    _lib.call("fvla_cache_evict", ctypes.byref(a), _w._stream())
+    # (first byte, byte behind the last, a destination)
+    small, large = 4 * k_scale.numel(), 4 * to_k_scale.numel()
+    spans = [(n, n + 4 * E, 0), (w, w + 4 * E * rows, 0), (pos, pos + 4 * E * rows if pos else 0, 0), (ks, ks + small, 0), (vs, vs + small, 0), (k, k + extents[0], 0),
+             (v, v + extents[1], 0), (out_n, out_n + 4 * E, 1), (out_w, out_w + 4 * E * out_rows if out_w else 0, 1),
+             (out_pos, out_pos + 4 * E * out_rows if out_pos else 0, 1), (to_ks, to_ks + large, 1), (to_vs, to_vs + large, 1), (to_k, to_k + extents[2], 1),
+             (to_v, to_v + extents[3], 1)]
+    spans.sort()
+    read = written = 0                          # how far the operands so far reach
+    for first, last, out in spans:
+        if first < written or (out and first < read):
+            raise ValueError("cache_evict: a destination lies over another operand")
+        if out:
+            written = last if last > written else written
+        else:
+            read = last if last > read else read
+    ws = _scratch("evict_ws", nbytes, weights.device)
+    block = _EVICT_HEAD.pack(k, v, ks, vs, w, to_k, to_v, to_ks, to_vs, out_w, ws.data_ptr(), n, pos, out_n, out_pos, nbytes) + rest
+    _lib.call("fvla_cache_evict", block, torch._C._cuda_getCurrentRawStream(device))
 
 
 OPERATORS = {f.__name__: f for f in (masked_attention, cache_append, cache_attention, cache_evict)}

@@ -119,8 +119,8 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
     const Episode s = episode_of(a, e);
     int most = s.n > 0 ? s.L : 0;
     if (a.causal && a.k_pos == nullptr) most = max(0, min(most, max(s.start + s.n, s.prefix)));
-    const int blocks = (most + BKEY - 1) / BKEY, share = (blocks + p.splits - 1) / p.splits;
-    const int first = split * share, count = max(0, min(share, blocks - first));
+    const int blocks = (most + BKEY - 1) / BKEY;
+    const int first = (int)((long long)blocks * split / p.splits), count = (int)((long long)blocks * (split + 1) / p.splits) - first;
 
     if (warp == 0) {
         if (lane == 0) {

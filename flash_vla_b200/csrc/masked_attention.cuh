@@ -677,29 +677,35 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) attention_join_kernel(const _
     const long long row = (long long)blockIdx.x * (JOIN_WARPS / warps) + warp / warps, rows = (long long)a.episodes * a.tokens * a.heads;
     const int h = (int)(row % a.heads), t = (int)(row / a.heads % a.tokens), e = (int)min(row / a.heads / a.tokens, (long long)a.episodes - 1);
     const bool mine = row < rows && t < episode_of(a, e).n;
+    // no load waits for another, but for the maxima: shares that held nothing are read as well, and dropped
     float m = -INFINITY;
-    if (mine) {
 #pragma unroll 4
-        for (int s = lane; s < p.splits; s += 32) {
-            const float2 ml = p.part_ml[s * rows + row];
-            if (ml.y != 0.f) m = fmaxf(m, ml.x);
-        }
+    for (int s = lane; s < p.splits; s += 32) {
+        const float2 ml = mine ? p.part_ml[s * rows + row] : make_float2(0.f, 0.f);
+        if (ml.y != 0.f) m = fmaxf(m, ml.x);
     }
     m = warp_max(m);
     const float top = m == -INFINITY ? 0.f : m;
     float acc[PER], l = 0.f;                                                         // columns lane, lane + 32, ...
 #pragma unroll
     for (int c = 0; c < PER; ++c) acc[c] = 0.f;
-    if (mine) {
-#pragma unroll (PER == 1 ? 8 : 4)
-        for (int s = part; s < p.splits; s += warps) {
-            const float2 ml = p.part_ml[s * rows + row];
-            const bool used = ml.y != 0.f;                                           // else this share held nothing that the row sees
-            const float w = ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - top);
-            const float* o = p.part_o + (s * rows + row) * hdp + col0;
-            l = used ? fmaf(ml.y, w, l) : l;
+    const float* o = p.part_o + (mine ? row : 0) * hdp + col0;
+    const size_t pitch = (size_t)rows * hdp;
+    for (int s0 = part; s0 < p.splits; s0 += 32 * warps) {
+        // lane i: the factor of share s0 + i * warps
+        const int s = s0 + lane * warps;
+        const float2 ml = mine && s < p.splits ? p.part_ml[s * rows + row] : make_float2(0.f, 0.f);
+        const float w = ml.y == 0.f ? 0.f : (ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - top));
+        l += warp_sum(ml.y == 0.f ? 0.f : ml.y * w);
+        const int have = min(32, (p.splits - s0 + warps - 1) / warps);
+#pragma unroll (PER == 1 ? 16 : 4)
+        for (int i = 0; i < have; ++i) {
+            const float f = __shfl_sync(0xffffffffu, w, i), used = __shfl_sync(0xffffffffu, ml.y, i);
 #pragma unroll
-            for (int c = 0; c < PER; ++c) { const float x = used ? o[32 * c] : 0.f; acc[c] = fmaf(used ? w : 0.f, x, acc[c]); }
+            for (int c = 0; c < PER; ++c) {
+                const float x = o[(size_t)(s0 + i * warps) * pitch + 32 * c];
+                acc[c] = fmaf(f, used != 0.f ? x : 0.f, acc[c]);
+            }
         }
     }
     if (warps > 1) {
@@ -739,13 +745,12 @@ __global__ void __launch_bounds__(32 * WEIGHT_WARPS) key_weights_kernel(const __
     // tokens before this one do not see key j (by its number), and their scores were not left
     const int from = by_number && j >= s.prefix ? max(0, j - s.start) : 0;
     float sum = 0.f;
-#pragma unroll 4
+#pragma unroll 8
     for (int r = warp; r < rows; r += warps) {
         const int h = r / s.n, t = r - h * s.n;
-        if (!inside || t < from) continue;
         const size_t row = row0 + (size_t)h * a.tokens + t;
-        const float z = a.lse[row], x = p.scores[row * p.pitch + j];
-        if (z != -INFINITY) sum += fast_exp2(fmaf(z, -kLog2e, x));
+        const float z = a.lse[row], x = p.scores[row * p.pitch + j];      // what was not left is read as well (j < pitch), and dropped
+        if (inside && t >= from && z != -INFINITY) sum += fast_exp2(fmaf(z, -kLog2e, x));
     }
     part[warp][threadIdx.x & 31] = sum;
     __syncthreads();

@@ -138,7 +138,20 @@ int fvla_cache_evict(const struct fvla_cache_evict_args* a, void* stream) {
     p.source = static_cast<int*>(a->ws);
     p.rows = a->rows; p.blocks = a->rows / a->block; p.out_rows = a->out_rows; p.out_blocks = a->out_rows / a->out_block; p.block = a->block; p.out_block = a->out_block;
     p.kv_heads = a->kv_heads; p.dim = a->head_dim; p.keep = a->keep; p.sinks = a->sinks; p.recent = a->recent;
-    int rc = launch("evict_select_kernel", q8::evict_select_kernel, dim3(a->episodes), dim3(q8::SELECT_THREADS), 0, S(stream), p);
+    // up to 2 048 rows one CTA (two rows a thread), beyond them eight
+    const int ctas = a->rows <= 2 * q8::SELECT_THREADS ? 1 : 8;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a->episodes * ctas); cfg.blockDim = dim3(q8::SELECT_THREADS); cfg.stream = S(stream);
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    const cudaError_t launched = cudaLaunchKernelEx(&cfg, q8::evict_select_kernel, p, ctas);
+    if (launched != cudaSuccess) { set_error("evict_select_kernel: %s", cudaGetErrorString(launched)); return FVLA_ERR_LAUNCH; }
+    const int rc = check_launch("evict_select_kernel");
     if (rc) return rc;
     const int chunks = a->out_block * a->head_dim / 16;
     const auto move = chunks <= 2 * q8::MOVE_THREADS ? q8::evict_move_kernel<2> : (chunks <= 4 * q8::MOVE_THREADS ? q8::evict_move_kernel<4> :

@@ -159,28 +159,44 @@ __device__ __forceinline__ uint32_t order_of(float w) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// One CTA per episode: the threshold by a radix select of 8 bits at a time, then the rows that stay, in order. For both each warp has a run of
-// rows of its own; lanes with equal digits add to the histogram together (weights are alike in their leading bits).
-__global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const __grid_constant__ EvictArgs p) {
+// A cluster of `ctas` CTAs per episode: the threshold by a radix select of 8 bits at a time, then the rows that stay, in order. For both each warp has
+// a run of rows of its own; lanes with equal digits add to the histogram together (weights are alike in their leading bits). The CTAs read
+// one another's histograms (two in turn, so that one barrier per digit is enough) and, at last, counts. Bound by latencies: a digit takes a load,
+// the votes, the barrier and a scan of 256 sums.
+__device__ __forceinline__ uint32_t remote(const void* shared, int rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(shared)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ uint32_t load_remote(uint32_t at) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+__global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const __grid_constant__ EvictArgs p, int ctas) {
     constexpr int WARPS = SELECT_THREADS / 32;
+    __shared__ uint32_t hists[2][256];
     __shared__ uint32_t hist[256];
+    __shared__ int cta_ties, cta_kept;
     __shared__ uint32_t s_prefix, s_left;
     __shared__ int warp_ties[WARPS], warp_kept[WARPS];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int e = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int e = blockIdx.x / ctas, rank = blockIdx.x % ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;      // (clusters are consecutive CTAs)
+    auto cluster_barrier = []() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); };
     const int L = min(max(p.lengths[e], 0), p.rows);
     const int n = min(L, p.keep);
     const float* w = p.weights + (size_t)e * p.rows;
     const int low = min(p.sinks, L), high = max(low, L - p.recent);       // rows [low, high) compete
     const int wanted = n - low - (L - high);                              // and so many of them stay (sinks + recent <= keep)
-    const int run = ((L + WARPS - 1) / WARPS + 31) / 32 * 32, begin = min(warp * run, L), end = min(begin + run, L);
+    const int run = ((L + ctas * WARPS - 1) / (ctas * WARPS) + 31) / 32 * 32, begin = (int)min((long long)(rank * WARPS + warp) * run, (long long)L), end = min(begin + run, L);
     const bool choose = L > p.keep;
     uint32_t threshold = 0xffffffffu, ties = 0;                           // nothing lies above the largest order
     if (choose && wanted > 0) {
         uint32_t prefix = 0, left = wanted;
         for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) hist[tid] = 0;
+            uint32_t* part = hists[shift >> 3 & 1];
+            if (tid < 256) part[tid] = 0;
             __syncthreads();
 #pragma unroll 4
             for (int j0 = begin; j0 < end; j0 += 32) {
@@ -190,7 +206,13 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const __gr
                 const bool counts = free && (shift == 24 || (u >> (shift + 8)) == prefix);
                 const uint32_t digit = counts ? (u >> shift) & 255u : 256u;
                 const uint32_t same = __match_any_sync(0xffffffffu, digit);
-                if (counts && lane == __ffs(same) - 1) atomicAdd(&hist[digit], (uint32_t)__popc(same));
+                if (counts && lane == __ffs(same) - 1) atomicAdd(&part[digit], (uint32_t)__popc(same));
+            }
+            cluster_barrier();
+            if (tid < 256) {
+                uint32_t sum = 0;
+                for (int c = 0; c < ctas; ++c) sum += load_remote(remote(part + tid, c));
+                hist[tid] = sum;
             }
             __syncthreads();
             if (warp == 0) {
@@ -229,14 +251,23 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const __gr
     }
     if (lane == 0) { warp_ties[warp] = tied; warp_kept[warp] = kept; }
     __syncthreads();
+    if (warp == 0) {
+        const int x = __reduce_add_sync(0xffffffffu, warp_ties[lane]), y = __reduce_add_sync(0xffffffffu, warp_kept[lane]);      // (32 warps)
+        if (lane == 0) { cta_ties = x; cta_kept = y; }
+    }
+    cluster_barrier();
     int ties_before = 0, kept_before = 0;
     {
-        int x = warp_ties[lane], y = warp_kept[lane];                     // (32 warps)
+        int ties_cta = 0, kept_cta = 0;                                   // of the CTAs before this one
+        for (int c = 0; c < rank; ++c) { ties_cta += (int)load_remote(remote(&cta_ties, c)); kept_cta += (int)load_remote(remote(&cta_kept, c)); }
+        int x = warp_ties[lane], y = warp_kept[lane];
         const int own = x;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) { const int z = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += z; }
+        x += ties_cta;
         y += min(x, (int)ties) - min(x - own, (int)ties);                 // with the ties of the run that stay
-        const int all = y;
+        if (lane == 0) y += kept_cta + min(ties_cta, (int)ties);
+        const int all = y - (lane == 0 ? kept_cta + min(ties_cta, (int)ties) : 0);
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) { const int z = __shfl_up_sync(0xffffffffu, y, o); if (lane >= o) y += z; }
         ties_before = __shfl_sync(0xffffffffu, x - own, warp);
@@ -260,7 +291,8 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const __gr
         ties_before += __popc(tie_mask);
         kept_before += __popc(mask);
     }
-    if (tid == 0) p.out_lengths[e] = n;
+    if (tid == 0 && rank == 0) p.out_lengths[e] = n;
+    cluster_barrier();                                                    // nobody leaves while its counts may be read
 }
 
 constexpr int MOVE_THREADS = 128;

@@ -9,7 +9,8 @@
 //   warp 0      TMA: K and V tiles of 128 keys in turn through a ring of SLOTS
 //   warp 1      one lane issues the MMAs, S^T a block ahead
 //   warps 2-5   softmax: thread = key. The rows' maxima by redux and through shared memory, sums kept per thread until the end.
-// Each CTA has a share of an episode's blocks of one K/V head and leaves unnormalised sums; attention_join_kernel adds them up.
+// Each CTA has a share of an episode's blocks of one K/V head. Up to eight shares are a cluster: its CTAs leave their unnormalised sums in shared
+// memory and each puts together a part of the result. More than eight leave them in scratch, and attention_join_kernel adds them up.
 #pragma once
 
 namespace fvla {
@@ -409,11 +410,14 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
             const int t = r / group;
             return (size_t)split * all + ((size_t)e * a.tokens + t) * a.heads + kv * group + r - t * group;
         };
-        if (quad == 0 && lane < rows) {
+        if (quad == 0 && lane < NR) {
             const float sum = count > 0 ? maxima[lane] + maxima[NR + lane] + maxima[2 * NR + lane] + maxima[3 * NR + lane] : 0.f;
-            p.part_ml[flat(lane)] = make_float2(count > 0 ? in_use[lane] : -INFINITY, sum);
+            const float2 ml = make_float2(count > 0 ? in_use[lane] : -INFINITY, sum);
+            if (p.cluster) reinterpret_cast<float2*>(gen + C::OFF_F)[lane] = ml;      // (the rows' factors are no longer needed)
+            else if (lane < rows) p.part_ml[flat(lane)] = ml;
         }
-        if (count > 0 && ok) {
+        if (count > 0) {
+            float* sums = reinterpret_cast<float*>(gen + C::OFF_T);                     // (all tiles have been read)
 #pragma unroll
             for (int h = 0; h < C::HALVES; ++h) {
                 float o[C::NO];
@@ -421,10 +425,52 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
 #pragma unroll
                 for (int r = 0; r < NR; ++r) {
                     const float x = Q8 ? fmaf(fmaf(o[(2 * NR + r) % C::NO], 1.f / 16.f, o[(NR + r) % C::NO]), 1.f / 16.f, o[r]) : o[r];
-                    if (r < rows) p.part_o[flat(r) * HDP + h * 128 + key] = x;
+                    if (p.cluster) sums[r * HDP + h * 128 + key] = x;
+                    else if (r < rows && ok) p.part_o[flat(r) * HDP + h * 128 + key] = x;
                 }
             }
         }
+    }
+    if (p.cluster) {
+        auto cluster_barrier = []() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); };
+        __syncwarp();
+        cluster_barrier();
+        if (warp >= 2 && s.n > 0) {
+            // row r of this CTA's part: its shares against the largest of their maxima
+            const int group = p.group, rows = s.n * group, me = tid - 64;
+            for (int i = split * 128 + me; i < rows * HDP; i += p.splits * 128) {
+                const int r = i / HDP, d = i % HDP;
+                float2 ml[8];
+                float top = -INFINITY, sum = 0.f, x = 0.f;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    ml[c] = make_float2(-INFINITY, 0.f);
+                    if (c < p.splits) {
+                        uint32_t at;
+                        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(base + C::OFF_F + r * 8), "r"(c));
+                        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(ml[c].x), "=f"(ml[c].y) : "r"(at) : "memory");
+                    }
+                    if (ml[c].y != 0.f) top = fmaxf(top, ml[c].x);
+                }
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    if (ml[c].y == 0.f) continue;                                       // this share held nothing that the row sees
+                    uint32_t at;
+                    float y;
+                    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(base + C::OFF_T + i * 4), "r"(c));
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(y) : "r"(at) : "memory");
+                    const float w = fast_exp2(ml[c].x - top);
+                    sum = fmaf(ml[c].y, w, sum);
+                    x = fmaf(y, w, x);
+                }
+                const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);
+                const int t = r / group, h = kv * group + r - t * group;
+                if (d < a.dim) a.out[e * a.os[0] + t * a.os[1] + h * a.os[2] + d] = __float2bfloat16_rn(x * inv);
+                if (a.lse && d == 0) a.lse[((size_t)e * a.heads + h) * a.tokens + t] = sum > 0.f ? (top + log2f(sum)) * 0.6931471805599453f : (sum == 0.f ? -INFINITY : sum);
+            }
+        }
+        __syncwarp();
+        cluster_barrier();                                                              // nobody leaves while its sums may be read
     }
 
     tc5::tc_fence_before();
@@ -452,7 +498,16 @@ inline int launch_few(const Tile& p, const CUtensorMap& tmK, const CUtensorMap& 
         if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return FVLA_ERR_LAUNCH; }
         configured.set();
     }
-    const cudaError_t e = launch_pdl(kern, dim3(p.splits, p.a.kv_heads, p.a.episodes), dim3(FEW_THREADS), C::SMEM, st, p, tmK, tmV);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.splits, p.a.kv_heads, p.a.episodes); cfg.blockDim = dim3(FEW_THREADS); cfg.dynamicSmemBytes = C::SMEM; cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = p.cluster ? p.splits : 1; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p, tmK, tmV);
     if (e != cudaSuccess) { set_error("attention_few_rows_kernel: %s", cudaGetErrorString(e)); return FVLA_ERR_LAUNCH; }
     return check_launch("attention_few_rows_kernel");
 }

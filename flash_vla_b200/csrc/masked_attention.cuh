@@ -73,6 +73,7 @@ struct Cfg {
 
 struct Tile {
     Args a;
+    int cluster;                                // few rows: the shares of a row are one cluster
     int group, tile_tokens, tiles, splits;      // query heads per K/V head, tokens per tile
     int q_mul[2], k_mul[2], v_mul[2];           // 0 where an axis (K/V head, episode) is broadcast: its coordinate stays 0
     float* part_o;                              // [split][row][HDP] fp32, row = ((e * tokens + t) * heads + h)
@@ -787,6 +788,7 @@ inline bool takes_few(const Args& a) { return (long long)a.tokens * (a.heads / a
 // Head dimension that the kernel is built for.
 inline int padded_dim(const Args& a) { return a.dim <= 64 && !takes_few(a) ? 64 : (a.dim <= 128 ? 128 : 256); }
 
+constexpr int CLUSTER = 8;      // shares that a cluster puts together
 // Shares of the key blocks: as many as bring the CTAs up to the number that are resident, at most one per block.
 inline int plan_splits(const Args& a) {
     const int group = a.heads / a.kv_heads, tile_tokens = BQ / group, blocks = (a.keys + BKEY - 1) / BKEY;
@@ -798,6 +800,7 @@ inline int plan_splits(const Args& a) {
         per_sm = few_rows(a) == 32 ? (tile_bytes == 16384 ? 2 : 1) : (tile_bytes == 16384 ? 3 : (tile_bytes == 32768 ? 2 : 1));
     }
     const long long room = (long long)tc5::num_sms() * per_sm * (few && tiles > tc5::num_sms() ? 2 : 1) / tiles;
+    if (few && room > CLUSTER && blocks <= 2 * CLUSTER) return blocks < CLUSTER ? (blocks > 0 ? blocks : 1) : CLUSTER;      // no second launch for two blocks each
     return (int)(room < 1 ? 1 : (room < blocks ? room : (blocks > 0 ? blocks : 1)));
 }
 inline size_t score_pitch(const Args& a) { return ((size_t)a.keys + BKEY - 1) / BKEY * BKEY; }
@@ -807,7 +810,7 @@ inline size_t workspace_bytes(const Args& a) {
     const size_t rows = (size_t)a.episodes * a.tokens * a.heads;
     size_t n = a.q_docs ? align256((size_t)a.episodes * ((a.keys + BKEY - 1) / BKEY) * sizeof(int2)) : 0;
     if (a.weights) n += rows * score_pitch(a) * sizeof(float);
-    if (splits > 1 || takes_few(a)) n += align256(splits * rows * sizeof(float2)) + splits * rows * padded_dim(a) * sizeof(float);
+    if (splits > (takes_few(a) ? CLUSTER : 1)) n += align256(splits * rows * sizeof(float2)) + splits * rows * padded_dim(a) * sizeof(float);
     return n;
 }
 
@@ -845,6 +848,7 @@ inline int launch_attention(const Args& a, void* ws, int* status, cudaStream_t s
     p.tile_tokens = BQ / p.group;
     p.tiles = (a.tokens + p.tile_tokens - 1) / p.tile_tokens;
     p.splits = plan_splits(a);
+    p.cluster = takes_few(a) && p.splits <= CLUSTER;
     p.status = status;
     const int blocks = (a.keys + BKEY - 1) / BKEY, hdp = padded_dim(a);
     const size_t rows = (size_t)a.episodes * a.tokens * a.heads;
@@ -897,7 +901,7 @@ inline int launch_attention(const Args& a, void* ws, int* status, cudaStream_t s
     if (few) {
         if (q8) rc = hdp == 128 ? launch_few<128, true>(p, tmK, tmV, st) : launch_few<256, true>(p, tmK, tmV, st);
         else rc = hdp == 128 ? launch_few<128, false>(p, tmK, tmV, st) : launch_few<256, false>(p, tmK, tmV, st);
-        if (!rc) rc = launch_join(p, hdp, st);
+        if (!rc && !p.cluster) rc = launch_join(p, hdp, st);
     } else if (q8) {
         rc = hdp == 64 ? launch_tile<64, true>(p, tmQ, tmK, tmV, st) : (hdp == 128 ? launch_tile<128, true>(p, tmQ, tmK, tmV, st) : launch_tile<256, true>(p, tmQ, tmK, tmV, st));
     } else {

@@ -183,7 +183,10 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const __gr
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int e = blockIdx.x / ctas, rank = blockIdx.x % ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;      // (clusters are consecutive CTAs)
-    auto cluster_barrier = []() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); };
+    auto cluster_barrier = [ctas]() {
+        if (ctas == 1) { __syncthreads(); return; }
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    };
     const int L = min(max(p.lengths[e], 0), p.rows);
     const int n = min(L, p.keep);
     const float* w = p.weights + (size_t)e * p.rows;
@@ -211,7 +214,9 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const __gr
             cluster_barrier();
             if (tid < 256) {
                 uint32_t sum = 0;
-                for (int c = 0; c < ctas; ++c) sum += load_remote(remote(part + tid, c));
+                if (ctas == 1) sum = part[tid];
+                else
+                    for (int c = 0; c < ctas; ++c) sum += load_remote(remote(part + tid, c));
                 hist[tid] = sum;
             }
             __syncthreads();

@@ -74,7 +74,9 @@ def _layout(t):
 
 
 def _cache_layout(c):
-    return tuple(t.shape for t in c), tuple(t.stride() for t in c), tuple(t.dtype for t in c)
+    K, V, K_scale, V_scale = c
+    return ((K.shape, V.shape, K_scale.shape, V_scale.shape), (K.stride(), V.stride(), K_scale.stride(), V_scale.stride()),
+            (K.dtype, V.dtype, K_scale.dtype, V_scale.dtype))
 
 
 # The argument blocks of the C entries (`_lib.Attention` and so on) are put together as bytes, addresses first, then what a layout determines and a plan

@@ -36,6 +36,11 @@ __device__ __forceinline__ float2 from_e4m3x2(uint32_t pair) {
     asm("{.reg .f16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;}" : "=f"(f.x), "=f"(f.y) : "r"(h));
     return f;
 }
+__device__ __forceinline__ uint32_t to_e5m2x2(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
 // Two bf16 values over a power of two -> e4m3 pair; what is not finite becomes NaN (0x7f).
 __device__ __forceinline__ uint32_t quantize_pair(uint32_t bf, float inv) {
     const float2 f = unpack_bf16x2(bf);

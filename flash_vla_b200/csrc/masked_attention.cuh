@@ -44,7 +44,7 @@ __device__ __forceinline__ Episode episode_of(const Args& p, int e) {
     return s;
 }
 
-constexpr int BQ = 128, BKEY = 128, SOFTMAX_WARPS = 16, SOFTMAX0 = 4;
+constexpr int BQ = 128, BKEY = 128, SOFTMAX_WARPS = 8, SOFTMAX0 = 4;
 constexpr float RESCALE_THRESHOLD = 8.0f;      // log2 units
 
 struct Tile {

@@ -3,11 +3,10 @@
 //   warp 0      TMA: the Q tile, then K and V in granules of 16 KB through one ring, in the order in which they are multiplied (K: 128 bytes of the
 //               head dimension of 128 keys; V: some keys, whole): what is in flight is then limited by shared memory alone, not by tile sizes
 //   warp 1      one lane issues S = Q K^T into one of BUFFERS TMEM score buffers, BUFFERS - 1 blocks ahead of O += P V (TMEM)
-//   warps 4-19  softmax: two groups of 256 threads, two threads per row with 64 keys each, which take the blocks in turn. P goes back to TMEM over
-//               the scores, as the A operand of P V, so that nothing crosses shared memory. All that one block needs from the one before is
-//               the running maximum: the other group hands it on (for 32 rows at a time) before it begins its exponentials, and those of one block
-//               run beside the other's loads and maxima. The accumulator is rescaled only where the maximum has grown by more than a threshold.
-// Bound by the softmax's latencies, which is why it has sixteen warps (eight, a row per thread: 325 us at head dim 128, 4 096 keys, 32 heads).
+//   warps 4-11  softmax: two groups of 128 threads, thread = row, which take the blocks in turn. P goes back to TMEM over the scores, as the A operand
+//               of P V, so that nothing crosses shared memory. All that one block needs from the one before is the running maximum: the other group
+//               hands it on (per warp, 32 rows) before it begins its exponentials, and those of one block run beside the other's
+//               loads and maxima. The accumulator is rescaled only where the maximum has grown by more than a threshold.
 // The 8-bit cache runs in 8 bits (kind::f8f6f4), its values straight from TMA: a bf16 row of Q, brought to 2^7..2^8 by its own power of two, is the sum
 // of an e4m3 term and an e5m2 term (what rounding to 4 bits leaves of 8 has at most 3; below 2^-16, 2^-23 of the largest, is lost), a probability the sum
 // of two e4m3 terms and an e5m2 term (11 bits; the last holds what is below e4m3's range). Probabilities stand against the running maximum at 2^6
@@ -52,20 +51,32 @@ __device__ __forceinline__ void st32_nowait(uint32_t taddr, const uint32_t* v) {
           "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
         : "memory");
 }
-__device__ __forceinline__ void st16_nowait(uint32_t taddr, const uint32_t* v) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
-        ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
-          "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+// Two fp32 operations at a time: (a0, a1) * b + c;  (a0, a1) + (x0, x1) * b;  (a0, a1) + (b0, b1);  (a0, a1) * b
+__device__ __forceinline__ unsigned long long pair(float x, float y) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
 }
-// (a0, a1) * b + c, two at a time
+__device__ __forceinline__ void unpair(unsigned long long v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
 __device__ __forceinline__ void fma2(float& a0, float& a1, float b, float c) {
-    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %2};\n\tmov.b64 c, {%3, %3};\n\tfma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
-        : "+f"(a0), "+f"(a1) : "f"(b), "f"(c));
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair(a0, a1)), "l"(pair(b, b)), "l"(pair(c, c)));
+    unpair(r, a0, a1);
+}
+__device__ __forceinline__ void axpy2(float& a0, float& a1, float x0, float x1, float b) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair(x0, x1)), "l"(pair(b, b)), "l"(pair(a0, a1)));
+    unpair(r, a0, a1);
 }
 __device__ __forceinline__ void add2(float& a0, float& a1, float b0, float b1) {
-    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
-        : "+f"(a0), "+f"(a1) : "f"(b0), "f"(b1));
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair(a0, a1)), "l"(pair(b0, b1)));
+    unpair(r, a0, a1);
+}
+__device__ __forceinline__ void mul2(float& a0, float& a1, float b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair(a0, a1)), "l"(pair(b, b)));
+    unpair(r, a0, a1);
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
@@ -81,8 +92,8 @@ struct TileCfg {
     static constexpr int Q_ATOMS = HDP / 64, Q_BYTES = Q_ATOMS * 16384;            // as bf16, and as two terms of e4m3
     static constexpr int BUFFERS = HDP == 256 ? 2 : 3;                             // 128 columns each, beside HDP columns of the accumulator
     static constexpr int SLOTS = HDP == 256 ? 9 : (HDP == 128 ? 11 : 12);
-    static constexpr int OFF_Q = 0, OFF_R = OFF_Q + Q_BYTES, OFF_X = OFF_R + SLOTS * GRANULE;      // ring; a maximum per row, two floats per row, group and half
-    static constexpr int OFF_BAR = OFF_X + 9 * BQ * 4;
+    static constexpr int OFF_Q = 0, OFF_R = OFF_Q + Q_BYTES, OFF_X = OFF_R + SLOTS * GRANULE;      // ring; a maximum per row, a float per row and group
+    static constexpr int OFF_BAR = OFF_X + 3 * BQ * 4;
     static constexpr int SMEM = 1024 + OFF_BAR + 352;
     static constexpr int THREADS = 32 * (SOFTMAX0 + SOFTMAX_WARPS);
     static constexpr uint32_t O_COL = BUFFERS * BKEY;
@@ -175,7 +186,7 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
     walk.count = first + (int)((long long)(last - first) * (split + 1) / p.splits) - walk.first;
     const bool any = walk.next(0) < walk.count;
 
-    // 640 threads start with 96 registers each: 56 + 4 x 104 = 472 of 5 x 96
+    // 384 threads start with 168 registers each: 56 + 2 x 224 = 504 = 3 x 168
     if (warp < SOFTMAX0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 0) {
@@ -225,7 +236,7 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                 }
             }
         } else if (warp == 1) {
-            if (tc5::elect_one() && any) {
+            if (any && tc5::elect_one()) {
                 constexpr uint32_t type = Q8 ? 0u : 1u, E5M2 = 1u << 7;      // e4m3 or bf16 operands; A in e5m2
                 constexpr uint32_t id_qk = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(BKEY >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
                 constexpr uint32_t id_pv = (1u << 4) | (type << 7) | (type << 10) | (1u << 16) | ((uint32_t)(HDP >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
@@ -285,13 +296,13 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         // Every thread runs every iteration and every named barrier even after a wait has given up (`ok` false), so nobody is left behind.
-        const int quad = warp & 3, half = (warp >> 2) - 1 & 1, g = (warp - SOFTMAX0) >> 3;      // TMEM lanes that this warp may access; which 64 keys of a block; which blocks
+        const int quad = warp & 3, g = (warp - SOFTMAX0) >> 2;         // TMEM lanes that this warp may access; which blocks it takes
         const int row = quad * 32 + lane;
         const uint32_t t_lane = (uint32_t)(quad * 32) << 16;
         float* m_shared = reinterpret_cast<float*>(gen + C::OFF_X);    // the maximum that each row's accumulator stands against
-        float* xch = m_shared + BQ;                                    // [group][half][row], of two blocks in turn: a warp may be a block ahead
+        float* xch = m_shared + BQ;                                    // [group][row]
         const bool busy = quad * 32 < tokens * p.group;                // a warp without rows only signals
         const int t = row / p.group, h = kv * p.group + row - t * p.group;
         const bool mine = t < tokens;
@@ -306,25 +317,23 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
         bool ok = true;
 
         if (Q8 && any) {
-            // Q from bf16 to its two terms, in place: a thread has a quarter of a row, and a row stays on its own lines
+            // Q from bf16 to its two terms, in place: a thread has half of a row, and a row stays on its own lines
             ok = mbar_wait(q_full, 0, abort_flag);
             __syncwarp();
-            constexpr int PIECES = HDP / 32;                           // of 16 bytes, 8 values, of a quarter of a row
-            const int part = g * 2 + half;
+            constexpr int PIECES = HDP / 16;                           // of 16 bytes, 8 values, of half a row
             uint4 u[PIECES];
             uint32_t amax = 0;
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) {
-                const int at = part * PIECES + i;
+                const int at = g * PIECES + i;
                 u[i] = *reinterpret_cast<const uint4*>(gen + C::OFF_Q + (at >> 3) * 16384 + row * 128 + (((at & 7) ^ (row & 7)) << 4));
                 const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
 #pragma unroll
                 for (int k = 0; k < 4; ++k) amax = max(amax, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
             }
-            xch[part * BQ + row] = __uint_as_float(amax);
-            asm volatile("bar.sync 9, 512;" ::: "memory");
-#pragma unroll
-            for (int i = 0; i < 4; ++i) amax = max(amax, __float_as_uint(xch[i * BQ + row]));
+            xch[g * BQ + row] = __uint_as_float(amax);
+            asm volatile("bar.sync 9, 256;" ::: "memory");
+            amax = max(amax, __float_as_uint(xch[(g ^ 1) * BQ + row]));
             const int ex = min(max((int)(amax >> 7) - 127, -119), 127);      // the largest element to 2^7..2^8
             const float up = __int_as_float((134 - ex) << 23);
             factor *= __int_as_float((120 + ex) << 23);
@@ -342,13 +351,13 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                     one[k] = lo | hi << 16;
                     two[k] = q8::to_e5m2x2(f[0] - a0.x, f[1] - a0.y) | q8::to_e5m2x2(f[2] - a1.x, f[3] - a1.y) << 16;
                 }
-                const int at = (part * PIECES + i) / 2;                             // piece of 16 values in the row
+                const int at = (g * PIECES + i) / 2;                             // piece of 16 values in the row
                 uint8_t* line = gen + C::OFF_Q + (at >> 3) * 16384 + row * 128 + (((at & 7) ^ (row & 7)) << 4);
                 *reinterpret_cast<uint4*>(line) = make_uint4(one[0], one[1], one[2], one[3]);
                 *reinterpret_cast<uint4*>(line + C::GRANULES * 16384) = make_uint4(two[0], two[1], two[2], two[3]);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            asm volatile("bar.sync 9, 512;" ::: "memory");                       // xch is free again
+            asm volatile("bar.sync 9, 256;" ::: "memory");                       // xch is free again
             if (lane == 0) tc5::mbar_arrive(q_ready);
         }
 
@@ -356,112 +365,128 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
         const int shift = Q8 ? 31 - __clz(a.block) : 0;                // blocks are powers of two
         const bool plain = !capped && a.slopes == nullptr && (factor > 1e-30f || !mine);
         const bool fast = !Q8 && __all_sync(0xffffffffu, plain);       // the factor goes into the exponential's argument
-        int n = 0;
-        for (int i = walk.next(0), after_i; i < walk.count; i = after_i, ++n) {
-            after_i = walk.next(i + 1);
-            if ((n & 1) != g) continue;
-            const int buffer = n % C::BUFFERS, block0 = (walk.first + i) * BKEY, key0 = block0 + half * 64;
-            float kf[4], lv[4];                                        // (8-bit cache) per 16 keys: factor of the scores, log2 of V's scale
+        const bool tagged = walk.range != nullptr || (a.k_pos != nullptr && a.causal);
+        const int clear = tagged ? 0 : __reduce_min_sync(0xffffffffu, mine ? key_limit : s.L);      // below, every row of the warp sees every key
+        const int nearest = __reduce_min_sync(0xffffffffu, mine ? pos : 0x7fffffff);                // and no row's position lies before a key
+        int n = 0, buffer = g, parity = 0, i = walk.next(0);
+        if (g == 1 && i < walk.count) { i = walk.next(i + 1); n = 1; }
+        while (i < walk.count) {
+            const int after_i = walk.next(i + 1), key0 = (walk.first + i) * BKEY;
+            float kf[8], lv[8];                                        // (8-bit cache) per 16 keys: factor of the scores, log2 of V's scale
             if (Q8 && busy) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                for (int c = 0; c < 8; ++c) {
                     const size_t at = ((size_t)e * (a.keys >> shift) + (min(key0 + c * 16, a.keys - 1) >> shift)) * a.kv_heads + kv;
                     kf[c] = factor * __ldg(a.k_scale + at);
                     lv[c] = (float)((int)(__float_as_uint(__ldg(a.v_scale + at)) >> 23) - 127);
                 }
             }
             const uint32_t t_s = tmem + t_lane + buffer * BKEY;
-            ok = ok && mbar_wait(s_full(buffer), (uint32_t)(n / C::BUFFERS & 1), abort_flag);
+            ok = ok && mbar_wait(s_full(buffer), (uint32_t)parity, abort_flag);
             __syncwarp();                                              // the TMEM accesses below are warp-collective
             tc5::tc_fence_after();
             if (busy) {
-                constexpr int KEYS = 64;
-                uint32_t r[KEYS];
+                uint32_t r[BKEY];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) ld32_nowait(t_s + half * KEYS + 32 * c, r + 32 * c);
+                for (int c = 0; c < 4; ++c) ld32_nowait(t_s + 32 * c, r + 32 * c);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                float (&v)[KEYS] = reinterpret_cast<float (&)[KEYS]>(r);
+                float (&v)[BKEY] = reinterpret_cast<float (&)[BKEY]>(r);
                 if (!fast) {
+                    if (Q8 || capped || a.k_pos) {
 #pragma unroll
-                    for (int c = 0; c < KEYS; ++c) v[c] *= Q8 ? kf[c >> 4] : factor;
-                    if (capped) {
+                        for (int c = 0; c < BKEY; c += 2) mul2(v[c], v[c + 1], Q8 ? kf[c >> 4] : factor);
+                        if (capped) {
 #pragma unroll
-                        for (int c = 0; c < KEYS; ++c) v[c] = cap2 * tanh_f(v[c]);
-                    }
-                    if (a.slopes) {
-                        if (a.k_pos) {
+                            for (int c = 0; c < BKEY; ++c) v[c] = cap2 * tanh_f(v[c]);
+                        }
+                        if (a.slopes) {
+                            if (a.k_pos) {
+                                const int* at = a.k_pos + (size_t)e * a.keys;
 #pragma unroll
-                            for (int c = 0; c < KEYS; ++c) v[c] = fmaf(-slope, fabsf((float)(pos - __ldg(a.k_pos + (size_t)e * a.keys + min(key0 + c, a.keys - 1)))), v[c]);
+                                for (int c = 0; c < BKEY; ++c) v[c] = fmaf(-slope, fabsf((float)(pos - __ldg(at + min(key0 + c, a.keys - 1)))), v[c]);
+                            } else {
+                                const float d0 = (float)(pos - key0);
+#pragma unroll
+                                for (int c = 0; c < BKEY; ++c) v[c] = fmaf(-slope, fabsf(d0 - (float)c), v[c]);
+                            }
+                        }
+                    } else {
+                        const float d0 = (float)(pos - key0);
+                        if (key0 + BKEY - 1 <= nearest) {
+                            // keys before every row of the warp: score + slope c - slope d0
+                            const float off = -slope * d0;
+                            float c0 = 0.f, c1 = 1.f;
+#pragma unroll
+                            for (int c = 0; c < BKEY; c += 2) {
+                                fma2(v[c], v[c + 1], factor, off);
+                                axpy2(v[c], v[c + 1], c0, c1, slope);
+                                add2(c0, c1, 2.f, 2.f);
+                            }
                         } else {
-                            const float d0 = (float)(pos - key0);
 #pragma unroll
-                            for (int c = 0; c < KEYS; ++c) v[c] = fmaf(-slope, fabsf(d0 - (float)c), v[c]);
+                            for (int c = 0; c < BKEY; ++c) v[c] = fmaf(-slope, fabsf(d0 - (float)c), v[c] * factor);
                         }
                     }
                 }
-                // visible keys, as bits; what is hidden becomes -infinity, and 2^-infinity is 0
-                uint32_t see[2] = {0xffffffffu, 0xffffffffu};
-                if (key0 + KEYS > key_limit) {
+                if (key0 + BKEY > clear) {
+                    // visible keys, as bits; what is hidden becomes -infinity, and 2^-infinity is 0
+                    uint32_t see[4];
 #pragma unroll
-                    for (int w = 0; w < 2; ++w) {
+                    for (int w = 0; w < 4; ++w) {
                         const int have = key_limit - key0 - 32 * w;
                         see[w] = have >= 32 ? 0xffffffffu : (have > 0 ? (1u << have) - 1u : 0u);
                     }
-                }
-                if (walk.range != nullptr) {
-                    // a lane looks at two keys; one vote for each document among the warp's rows (one or two, as a rule)
-                    const int* tag = a.k_docs + (size_t)e * a.keys;
-                    int ids[2];
+                    if (walk.range != nullptr) {
+                        // a lane looks at four keys; one vote for each document among the warp's rows (one or two, as a rule)
+                        const int* tag = a.k_docs + (size_t)e * a.keys;
+                        int ids[4];
 #pragma unroll
-                    for (int w = 0; w < 2; ++w) ids[w] = __ldg(tag + min(key0 + 32 * w + lane, a.keys - 1));
-                    uint32_t left = __ballot_sync(0xffffffffu, doc >= 0);
-                    if (doc < 0) see[0] = see[1] = 0u;
-                    while (left) {
-                        const int d = __shfl_sync(0xffffffffu, doc, __ffs(left) - 1);
+                        for (int w = 0; w < 4; ++w) ids[w] = __ldg(tag + min(key0 + 32 * w + lane, a.keys - 1));
+                        uint32_t left = __ballot_sync(0xffffffffu, doc >= 0);
+                        if (doc < 0) see[0] = see[1] = see[2] = see[3] = 0u;
+                        while (left) {
+                            const int d = __shfl_sync(0xffffffffu, doc, __ffs(left) - 1);
 #pragma unroll
-                        for (int w = 0; w < 2; ++w) {
-                            const uint32_t votes = __ballot_sync(0xffffffffu, ids[w] == d);
-                            if (doc == d) see[w] &= votes;
+                            for (int w = 0; w < 4; ++w) {
+                                const uint32_t votes = __ballot_sync(0xffffffffu, ids[w] == d);
+                                if (doc == d) see[w] &= votes;
+                            }
+                            left &= ~__ballot_sync(0xffffffffu, doc == d);
                         }
-                        left &= ~__ballot_sync(0xffffffffu, doc == d);
                     }
-                }
-                if (a.k_pos && a.causal) {
-                    const int* at = a.k_pos + (size_t)e * a.keys;
+                    if (a.k_pos && a.causal) {
+                        const int* at = a.k_pos + (size_t)e * a.keys;
 #pragma unroll
-                    for (int w = 0; w < 2; ++w) {
-                        uint32_t seen = 0u;
+                        for (int w = 0; w < 4; ++w) {
+                            uint32_t seen = 0u;
 #pragma unroll
-                        for (int c = 0; c < 32; ++c)
-                            if (__ldg(at + min(key0 + 32 * w + c, a.keys - 1)) <= limit) seen |= 1u << c;
-                        see[w] &= seen;
+                            for (int c = 0; c < 32; ++c)
+                                if (__ldg(at + min(key0 + 32 * w + c, a.keys - 1)) <= limit) seen |= 1u << c;
+                            see[w] &= seen;
+                        }
                     }
-                }
-                if (!__all_sync(0xffffffffu, (see[0] & see[1]) == 0xffffffffu)) {
+                    if (!__all_sync(0xffffffffu, (see[0] & see[1] & see[2] & see[3]) == 0xffffffffu)) {
 #pragma unroll
-                    for (int c = 0; c < KEYS; ++c) v[c] = see[c >> 5] & (1u << (c & 31)) ? v[c] : -INFINITY;
+                        for (int c = 0; c < BKEY; ++c) v[c] = see[c >> 5] & (1u << (c & 31)) ? v[c] : -INFINITY;
+                    }
                 }
                 if (Q8 && p.scores != nullptr && mine) {
                     float4* dst = reinterpret_cast<float4*>(p.scores + (((size_t)e * a.heads + h) * a.tokens + t0 + t) * p.pitch + key0);
 #pragma unroll
-                    for (int c = 0; c < KEYS; c += 4) dst[c / 4] = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+                    for (int c = 0; c < BKEY; c += 4) dst[c / 4] = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
                 }
-                float top[4];
+                float top[8];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
+                for (int q = 0; q < 8; ++q) {
                     float x = fmaxf(v[16 * q], v[16 * q + 1]);
 #pragma unroll
                     for (int c = 2; c < 16; c += 2) x = max3(x, v[16 * q + c], v[16 * q + c + 1]);
                     top[q] = Q8 ? x + lv[q] : x;
                 }
-                float mx = max3(fmaxf(top[0], top[1]), top[2], top[3]);
+                float mx = max3(max3(top[0], top[1], top[2]), max3(top[3], top[4], top[5]), fmaxf(top[6], top[7]));
                 if (fast) mx *= factor;
-                // the row's other thread, and the maximum that the blocks before have left: both halves wait for each other and for the other group's
-                // two to hand it on
-                float* board = xch + (n >> 1 & 1) * 4 * BQ + g * 2 * BQ + row;
-                board[half * BQ] = mx;
-                asm volatile("bar.sync %0, %1;" ::"r"(1 + g * 4 + quad), "r"(n > 0 ? 128 : 64) : "memory");
-                mx = fmaxf(mx, board[(half ^ 1) * BQ]);
+                // the maximum that the blocks before have left, and what becomes of it
+                if (n > 0) asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + quad) : "memory");
                 const float m_old = n > 0 ? m_shared[row] : -INFINITY;
                 const bool grow = m_old != -INFINITY && mx > m_old + C::THRESHOLD;
                 const float m_new = grow || m_old == -INFINITY ? mx : m_old;
@@ -472,7 +497,7 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                     tc5::tc_fence_after();
                     const float alpha = grow ? fast_exp2(m_old - m_new) : 1.0f;
 #pragma unroll 1
-                    for (int c = half * (HDP / 64); c < (half + 1) * (HDP / 64); ++c) {
+                    for (int c = 0; c < HDP / 32; ++c) {
                         uint32_t o[32];
                         ld32_nowait(tmem + t_lane + C::O_COL + c * 32, o);
                         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -483,8 +508,8 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     tc5::tc_fence_before();
                 }
-                if (half == 0) m_shared[row] = m_new;
-                if (after_i < walk.count) asm volatile("bar.arrive %0, 128;" ::"r"(1 + (g ^ 1) * 4 + quad) : "memory");
+                m_shared[row] = m_new;
+                if (after_i < walk.count) asm volatile("bar.arrive %0, 64;" ::"r"(1 + (g ^ 1) * 4 + quad) : "memory");
                 if (m_new != m_used) {
                     l *= m_used == -INFINITY ? 1.f : fast_exp2(m_used - m_new);
                     m_used = m_new;
@@ -492,22 +517,26 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                 const float m = (m_new == -INFINITY ? 0.f : m_new) - C::SHIFT;      // (nothing but NaN, or nothing at all, so far)
                 if (!Q8) {
                     const float f = fast ? factor : 1.f;
-                    float s0 = 0.f, s1 = 0.f;
+                    float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll
-                    for (int c = 0; c < KEYS; c += 2) {
+                    for (int c = 0; c < BKEY; c += 4) {
                         fma2(v[c], v[c + 1], f, -m);
-                        v[c] = fast_exp2(v[c]);
-                        v[c + 1] = fast_exp2(v[c + 1]);
-                        add2(s0, s1, v[c], v[c + 1]);
-                        r[c / 2] = pack_bf16x2(v[c], v[c + 1]);
-                    }
-                    l += s0 + s1;
-                    st32_nowait(t_s + half * 32, r);
-                } else {
-                    // three terms of four values to a word, 16 columns each
-                    uint32_t w[3][16];
+                        fma2(v[c + 2], v[c + 3], f, -m);
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
+                        for (int k = 0; k < 4; ++k) v[c + k] = fast_exp2(v[c + k]);
+                        add2(s0, s1, v[c], v[c + 1]);
+                        add2(s2, s3, v[c + 2], v[c + 3]);
+                        r[c / 2] = pack_bf16x2(v[c], v[c + 1]);
+                        r[c / 2 + 1] = pack_bf16x2(v[c + 2], v[c + 3]);
+                        if (c == 60) st32_nowait(t_s, r);
+                    }
+                    l += (s0 + s1) + (s2 + s3);
+                    st32_nowait(t_s + 32, r + 32);
+                } else {
+                    // three terms of four values to a word, 32 columns each
+                    uint32_t w[3][32];
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {
                         float sum = 0.f;
                         const float off = lv[q] - m;
 #pragma unroll
@@ -529,25 +558,25 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                         l = fmaf(sum, fast_exp2(-lv[q]), l);
                     }
 #pragma unroll
-                    for (int term = 0; term < 3; ++term) st16_nowait(t_s + 32 * term + half * 16, w[term]);
+                    for (int term = 0; term < 3; ++term) st32_nowait(t_s + 32 * term, w[term]);
                 }
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             }
             // keys whose values may be anything, behind the last one or under a negative document: zeros, for 0 * NaN would reach every row
-            bool tail = block0 + BKEY > s.L;
+            bool tail = key0 + BKEY > s.L;
             if (walk.range != nullptr) tail = tail || __ldg(walk.range + walk.first + i).x < 0;
             if (tail) {
                 // in the ring, V of block n has n blocks of V before it, and K up to BUFFERS - 1 blocks further on
                 int blocks = 2 * n + 1;
                 for (int b = 1, j = after_i; b < C::BUFFERS && j < walk.count; ++b, j = walk.next(j + 1)) ++blocks;
-                const int key = row, at = block0 + key, before = blocks * C::GRANULES;
+                const int key = row, at = key0 + key, before = blocks * C::GRANULES;
                 const bool bad = at >= s.L || (walk.range != nullptr && __ldg(a.k_docs + (size_t)e * a.keys + at) < 0);
 #pragma unroll 1
                 for (int c = 0; c < C::GRANULES; ++c) {
                     const int at_slot = (before + c) % C::SLOTS;
                     ok = ok && mbar_wait(full(at_slot), (uint32_t)(((before + c) / C::SLOTS) & 1), abort_flag);
                     if (bad && key / C::V_KEYS == c)
-                        for (int k = half * 4; k < C::GRANULES * 8; k = (k & 3) == 3 ? k + 5 : k + 1)
+                        for (int k = 0; k < C::GRANULES * 8; ++k)
                             *reinterpret_cast<uint4*>(gen + C::OFF_R + at_slot * C::GRANULE + (k >> 3) * (C::V_KEYS * 128) + key % C::V_KEYS * 128 + (k & 7) * 16) = make_uint4(0, 0, 0, 0);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -555,52 +584,56 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
             tc5::tc_fence_before();
             __syncwarp();
             if (lane == 0) tc5::mbar_arrive(p_full(buffer));
+            // this group's next block is the one after the other group's
+            buffer += 2;
+            if (buffer >= C::BUFFERS) { buffer -= C::BUFFERS; parity ^= 1; }
+            n += 2;
+            i = after_i < walk.count ? walk.next(after_i + 1) : walk.count;
         }
-        if (n > 0) ok = ok && mbar_wait(finished, 0, abort_flag);
+        if (any) ok = ok && mbar_wait(finished, 0, abort_flag);
         __syncwarp();
-        asm volatile("bar.sync 9, 512;" ::: "memory");                               // and every row's last maximum is there
+        asm volatile("bar.sync 9, 256;" ::: "memory");                               // and every row's last maximum is there
         tc5::tc_fence_after();
-        // the row's sum from its four threads; then two of them store half of the columns each
-        const float m_all = n > 0 && busy ? m_shared[row] : -INFINITY;
+        // the row's sum from its two threads, then half of the columns each
+        const float m_all = any && busy ? m_shared[row] : -INFINITY;
         if (m_used != -INFINITY) l *= fast_exp2(m_used - m_all);
-        xch[(g * 2 + half) * BQ + row] = l;
-        asm volatile("bar.sync 9, 512;" ::: "memory");
-        l = xch[row] + xch[BQ + row] + xch[2 * BQ + row] + xch[3 * BQ + row];
+        xch[g * BQ + row] = l;
+        asm volatile("bar.sync 9, 256;" ::: "memory");
+        l = xch[row] + xch[BQ + row];
         const float m_end = (m_all == -INFINITY ? 0.f : m_all) - C::SHIFT;
         if (busy) {
-            const int part = g * 2 + half;
-            constexpr int SPAN = HDP / 4;                              // columns of a thread: 16, 32 or 64
+            constexpr int SPAN = HDP / 2;                              // columns of a thread
             const size_t flat = ((size_t)e * a.tokens + t0 + (mine ? t : 0)) * a.heads + h;
             const bool store = ok && mine;
             if (p.splits > 1) {
                 const size_t at = (size_t)split * a.episodes * a.tokens * a.heads + flat;
-                if (store && part == 0) p.part_ml[at] = make_float2(l == 0.f ? -INFINITY : m_end, l);
+                if (store && g == 0) p.part_ml[at] = make_float2(l == 0.f ? -INFINITY : m_end, l);
 #pragma unroll 1
-                for (int c = 0; c < (n > 0 ? SPAN : 0); c += 16) {
-                    float o[16];
-                    tc5::tmem_ld16(tmem + t_lane + C::O_COL + part * SPAN + c, o);
+                for (int c = 0; c < (any ? SPAN : 0); c += 32) {
+                    float o[32];
+                    tc5::tmem_ld32(tmem + t_lane + C::O_COL + g * SPAN + c, o);
                     if (store) {
-                        float4* dst = reinterpret_cast<float4*>(p.part_o + at * HDP + part * SPAN + c);
+                        float4* dst = reinterpret_cast<float4*>(p.part_o + at * HDP + g * SPAN + c);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) dst[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                        for (int k = 0; k < 8; ++k) dst[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
                     }
                     __syncwarp();
                 }
             } else {
                 const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);         // NaN stays
-                if (store && part == 0 && a.lse)
+                if (store && g == 0 && a.lse)
                     a.lse[((size_t)e * a.heads + h) * a.tokens + t0 + t] = l > 0.f ? (m_end + log2f(l)) * 0.6931471805599453f : (l == 0.f ? -INFINITY : l);
                 bf16* dst = a.out + e * a.os[0] + (t0 + (mine ? t : 0)) * a.os[1] + h * a.os[2];
 #pragma unroll 1
-                for (int c = 0; c < SPAN; c += 16) {
-                    float o[16];
-                    const int col = part * SPAN + c;
-                    if (n > 0) tc5::tmem_ld16(tmem + t_lane + C::O_COL + col, o);
+                for (int c = 0; c < SPAN; c += 32) {
+                    float o[32];
+                    const int col = g * SPAN + c;
+                    if (any) tc5::tmem_ld32(tmem + t_lane + C::O_COL + col, o);
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) o[k] = n > 0 ? o[k] * inv : 0.f;
+                    for (int k = 0; k < 32; ++k) o[k] = any ? o[k] * inv : 0.f;
                     if (store) {
 #pragma unroll
-                        for (int k = 0; k < 2; ++k)
+                        for (int k = 0; k < 4; ++k)
                             if (col + k * 8 < a.dim)
                                 *reinterpret_cast<uint4*>(dst + col + k * 8) = make_uint4(pack_bf16x2(o[8 * k], o[8 * k + 1]), pack_bf16x2(o[8 * k + 2], o[8 * k + 3]),
                                                                                         pack_bf16x2(o[8 * k + 4], o[8 * k + 5]), pack_bf16x2(o[8 * k + 6], o[8 * k + 7]));

@@ -1,8 +1,9 @@
 // Attention of many rows. One CTA has 128 rows (tokens x the query heads of one K/V head) of an episode and walks the key blocks that any of them
 // sees, or one of `splits` equal shares of them:
-//   warp 0      TMA: the Q tile, then K and V in granules of 16 KB through one ring, in the order in which they are multiplied (K: 128 bytes of the
-//               head dimension of 128 keys; V: some keys, whole): what is in flight is then limited by shared memory alone, not by tile sizes
-//   warp 1      one lane issues S = Q K^T into one of BUFFERS TMEM score buffers, BUFFERS - 1 blocks ahead of O += P V (TMEM)
+//   warps 0, 3  TMA: the Q tile and K, and V, each in granules of 16 KB through a ring (K: 128 bytes of the head dimension of 128 keys; V: some
+//               keys, whole): what is in flight is then limited by shared memory alone, not by tile sizes
+//   warps 1, 2  one lane of each issues S = Q K^T into one of BUFFERS TMEM score buffers, and O += P V (TMEM). (An issue takes 50 to 100 clocks with
+//               its waits; one lane for both was the bottleneck, 2 070 clocks a block at head dim 128.)
 //   warps 4-11  softmax: two groups of 128 threads, thread = row, which take the blocks in turn. P goes back to TMEM over the scores, as the A operand
 //               of P V, so that nothing crosses shared memory. All that one block needs from the one before is the running maximum: the other group
 //               hands it on (per warp, 32 rows) before it begins its exponentials, and those of one block run beside the other's
@@ -91,10 +92,10 @@ struct TileCfg {
     static constexpr int V_KEYS = BKEY / GRANULES;                                 // keys of a V granule
     static constexpr int Q_ATOMS = HDP / 64, Q_BYTES = Q_ATOMS * 16384;            // as bf16, and as two terms of e4m3
     static constexpr int BUFFERS = HDP == 256 ? 2 : 3;                             // 128 columns each, beside HDP columns of the accumulator
-    static constexpr int SLOTS = HDP == 256 ? 9 : (HDP == 128 ? 11 : 12);
-    static constexpr int OFF_Q = 0, OFF_R = OFF_Q + Q_BYTES, OFF_X = OFF_R + SLOTS * GRANULE;      // ring; a maximum per row, a float per row and group
+    static constexpr int SLOTS = HDP == 256 ? 5 : 6;                               // of each ring
+    static constexpr int OFF_Q = 0, OFF_R = OFF_Q + Q_BYTES, OFF_X = OFF_R + 2 * SLOTS * GRANULE;      // rings; a maximum per row, a float per row and group
     static constexpr int OFF_BAR = OFF_X + 3 * BQ * 4;
-    static constexpr int SMEM = 1024 + OFF_BAR + 352;
+    static constexpr int SMEM = 1024 + OFF_BAR + 344;
     static constexpr int THREADS = 32 * (SOFTMAX0 + SOFTMAX_WARPS);
     static constexpr uint32_t O_COL = BUFFERS * BKEY;
     static constexpr float SHIFT = Q8 ? 6.f : 0.f, THRESHOLD = Q8 ? 2.f : RESCALE_THRESHOLD;
@@ -114,10 +115,12 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
     auto p_full = [&](int b) { return bars + 40 + b * 8; };
     auto o_done = [&](int b) { return bars + 64 + b * 8; };                // of even and odd blocks
     const uint32_t finished = bars + 80;                                   // all products (a wait for a block's own phase could come too late for its parity)
-    auto full = [&](int s) { return bars + 88 + s * 8; };
-    auto empty = [&](int s) { return bars + 88 + C::SLOTS * 8 + s * 8; };
-    const uint32_t tmem_slot = bars + 88 + C::SLOTS * 16;
-    uint8_t* after = gen + C::OFF_BAR + 88 + C::SLOTS * 16;
+    auto p_read = [&](int b) { return bars + 96 + b * 8; };                // the product has read P: the buffer may take scores
+    // rings: K slots, then V slots
+    auto full = [&](int s) { return bars + 120 + s * 8; };
+    auto empty = [&](int s) { return bars + 120 + C::SLOTS * 16 + s * 8; };
+    const uint32_t tmem_slot = bars + 120 + C::SLOTS * 32;
+    uint8_t* after = gen + C::OFF_BAR + 120 + C::SLOTS * 32;
     volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(after);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(after + 4);
     int* shared_int = reinterpret_cast<int*>(after + 8);      // smallest and largest document of the queries, first and last block seen
@@ -131,10 +134,10 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
 
     if (tid == 0) {
         mbar_init(q_full, 1); mbar_init(q_ready, SOFTMAX_WARPS);
-        for (int b = 0; b < C::BUFFERS; ++b) { mbar_init(s_full(b), 1); mbar_init(p_full(b), SOFTMAX_WARPS / 2); }
+        for (int b = 0; b < C::BUFFERS; ++b) { mbar_init(s_full(b), 1); mbar_init(p_full(b), SOFTMAX_WARPS / 2); mbar_init(p_read(b), 1); }
         for (int b = 0; b < 2; ++b) mbar_init(o_done(b), 1);
         mbar_init(finished, 1);
-        for (int s = 0; s < C::SLOTS; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+        for (int s = 0; s < 2 * C::SLOTS; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
         *abort_flag = 0;
         shared_int[0] = shared_int[2] = 0x7fffffff;
         shared_int[1] = shared_int[3] = -0x7fffffff - 1;
@@ -189,108 +192,106 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
     // 384 threads start with 168 registers each: 56 + 2 x 224 = 504 = 3 x 168
     if (warp < SOFTMAX0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        constexpr uint32_t type = Q8 ? 0u : 1u, E5M2 = 1u << 7;      // e4m3 or bf16 operands; A in e5m2
+        int at = 0;                                                  // slot of this warp's ring, and the parity of its round
+        uint32_t phase = 0;
+        auto advance = [&]() { if (++at == C::SLOTS) { at = 0; phase ^= 1u; } };
         if (warp == 0) {
             if (lane == 0 && any) {
                 tc5::prefetch_tensormap(&tmQ);
                 tc5::prefetch_tensormap(&tmK);
-                tc5::prefetch_tensormap(&tmV);
                 mbar_expect_tx(q_full, C::Q_ATOMS * 128 * p.group * p.tile_tokens);
 #pragma unroll
                 for (int c = 0; c < C::Q_ATOMS; ++c) tma_load_5d(sQ + c * 16384, &tmQ, q_full, c * 64, 0, t0, kv * p.q_mul[0], e * p.q_mul[1]);
-                int at = 0;
-                uint32_t phase = 1;
-                auto slot = [&]() -> bool {
-                    if (!mbar_wait(empty(at), phase, abort_flag)) return false;
-                    mbar_expect_tx(full(at), C::GRANULE);
-                    return true;
-                };
-                auto advance = [&]() { if (++at == C::SLOTS) { at = 0; phase ^= 1u; } };
-                auto load_k = [&](int i) -> bool {
+                bool ok = true;
+                for (int i = walk.next(0); i < walk.count && ok; i = walk.next(i + 1)) {
 #pragma unroll 1
                     for (int c = 0; c < C::GRANULES; ++c) {
-                        if (!slot()) return false;
+                        ok = mbar_wait(empty(at), phase ^ 1u, abort_flag);
+                        if (!ok) break;
+                        mbar_expect_tx(full(at), C::GRANULE);
                         tma_load_4d(ring + at * C::GRANULE, &tmK, full(at), c * (128 / C::ELEM), (walk.first + i) * BKEY, kv * p.k_mul[0], e * p.k_mul[1]);
                         advance();
                     }
-                    return true;
-                };
-                auto load_v = [&](int i) -> bool {
+                }
+            }
+        } else if (warp == 3) {
+            if (lane == 0 && any) {
+                tc5::prefetch_tensormap(&tmV);
+                bool ok = true;
+                for (int i = walk.next(0); i < walk.count && ok; i = walk.next(i + 1)) {
 #pragma unroll 1
                     for (int c = 0; c < C::GRANULES; ++c) {
-                        if (!slot()) return false;
+                        const int slot = C::SLOTS + at;
+                        ok = mbar_wait(empty(slot), phase ^ 1u, abort_flag);
+                        if (!ok) break;
+                        mbar_expect_tx(full(slot), C::GRANULE);
 #pragma unroll
                         for (int d = 0; d < C::GRANULES; ++d)
-                            tma_load_4d(ring + at * C::GRANULE + d * C::V_KEYS * 128, &tmV, full(at), d * (128 / C::ELEM), (walk.first + i) * BKEY + c * C::V_KEYS,
+                            tma_load_4d(ring + slot * C::GRANULE + d * C::V_KEYS * 128, &tmV, full(slot), d * (128 / C::ELEM), (walk.first + i) * BKEY + c * C::V_KEYS,
                                         kv * p.v_mul[0], e * p.v_mul[1]);
                         advance();
                     }
-                    return true;
-                };
-                // K runs BUFFERS - 1 blocks ahead of V, as the products do
-                int i = walk.next(0), j = i;
-                bool ok = true;
-                for (int b = 0; b < C::BUFFERS - 1 && j < walk.count && ok; ++b, j = walk.next(j + 1)) ok = load_k(j);
-                for (; i < walk.count && ok; i = walk.next(i + 1)) {
-                    if (j < walk.count) { ok = load_k(j); j = walk.next(j + 1); }
-                    ok = ok && load_v(i);
                 }
             }
         } else if (warp == 1) {
             if (any && tc5::elect_one()) {
-                constexpr uint32_t type = Q8 ? 0u : 1u, E5M2 = 1u << 7;      // e4m3 or bf16 operands; A in e5m2
                 constexpr uint32_t id_qk = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(BKEY >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
-                constexpr uint32_t id_pv = (1u << 4) | (type << 7) | (type << 10) | (1u << 16) | ((uint32_t)(HDP >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
-                int at = 0;
-                uint32_t phase = 0;
-                auto advance = [&]() { if (++at == C::SLOTS) { at = 0; phase ^= 1u; } };
-                auto issue_qk = [&](int n) -> bool {
-#pragma unroll 1
-                    for (int c = 0; c < C::GRANULES; ++c) {
-                        if (!mbar_wait(full(at), phase, abort_flag)) return false;
-                        tc5::tc_fence_after();
-#pragma unroll
-                        for (int term = 0; term < C::QT; ++term)
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const uint64_t ad = smem_desc(sQ + (term * C::GRANULES + c) * 16384 + k * 32, 16, 1024);
-                                const uint64_t bd = smem_desc(ring + at * C::GRANULE + k * 32, 16, 1024);
-                                if (Q8) umma_f8(tmem + n % C::BUFFERS * BKEY, ad, bd, id_qk | (term == 1 ? E5M2 : 0u), c > 0 || term > 0 || k > 0);
-                                else tc5::umma_bf16(tmem + n % C::BUFFERS * BKEY, ad, bd, id_qk, c > 0 || k > 0);
-                            }
-                        tc5::umma_commit(empty(at));
-                        advance();
-                    }
-                    tc5::umma_commit(s_full(n % C::BUFFERS));
-                    return true;
-                };
                 bool ok = mbar_wait(Q8 ? q_ready : q_full, 0, abort_flag);
-                tc5::tc_fence_after();
-                int i = walk.next(0), j = i, n = 0, ahead = 0;
-                for (; ahead < C::BUFFERS - 1 && j < walk.count && ok; ++ahead, j = walk.next(j + 1)) ok = issue_qk(ahead);
-                for (; i < walk.count && ok; ++n, i = walk.next(i + 1)) {
-                    // S of this block lies where P of block n - 1 was, whose product has been issued before
-                    if (j < walk.count) { ok = issue_qk(ahead++); j = walk.next(j + 1); if (!ok) break; }
-                    ok = mbar_wait(p_full(n % C::BUFFERS), (uint32_t)(n / C::BUFFERS & 1), abort_flag);
-                    if (!ok) break;
+                int buffer = 0, round = 0;
+                for (int i = walk.next(0); i < walk.count && ok; i = walk.next(i + 1)) {
+                    if (round > 0) { ok = mbar_wait(p_read(buffer), (uint32_t)(round - 1) & 1u, abort_flag); if (!ok) break; }
 #pragma unroll 1
                     for (int c = 0; c < C::GRANULES; ++c) {
                         ok = mbar_wait(full(at), phase, abort_flag);
                         if (!ok) break;
                         tc5::tc_fence_after();
-                        constexpr int KEYS = 32 / C::ELEM;                       // keys per MMA, 8 columns of P
+                        const uint64_t ad = smem_desc(sQ + c * 16384, 16, 1024), bd = smem_desc(ring + at * C::GRANULE, 16, 1024);
 #pragma unroll
-                        for (int k = 0; k < C::V_KEYS / KEYS; ++k) {
-                            const uint64_t bd = smem_desc(ring + at * C::GRANULE + k * KEYS * 128, C::V_KEYS * 128, 1024);
+                        for (int term = 0; term < C::QT; ++term)
 #pragma unroll
-                            for (int term = 0; term < C::PT; ++term)
-                                umma_ts<Q8>(tmem + C::O_COL, tmem + n % C::BUFFERS * BKEY + term * 32 + (c * (C::V_KEYS / KEYS) + k) * 8, bd, id_pv | (term == 2 ? E5M2 : 0u),
-                                            n > 0 || c > 0 || k > 0 || term > 0);
-                        }
+                            for (int k = 0; k < 4; ++k) {             // 32 bytes further on: 2 in a descriptor
+                                if (Q8) umma_f8(tmem + buffer * BKEY, ad + term * C::GRANULES * 1024 + 2 * k, bd + 2 * k, id_qk | (term == 1 ? E5M2 : 0u), c > 0 || term > 0 || k > 0);
+                                else tc5::umma_bf16(tmem + buffer * BKEY, ad + 2 * k, bd + 2 * k, id_qk, c > 0 || k > 0);
+                            }
                         tc5::umma_commit(empty(at));
                         advance();
                     }
                     if (!ok) break;
+                    tc5::umma_commit(s_full(buffer));
+                    if (++buffer == C::BUFFERS) { buffer = 0; ++round; }
+                }
+            }
+        } else if (warp == 2) {
+            if (any && tc5::elect_one()) {
+                constexpr uint32_t id_pv = (1u << 4) | (type << 7) | (type << 10) | (1u << 16) | ((uint32_t)(HDP >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
+                constexpr int KEYS = 32 / C::ELEM;                     // keys per MMA, 8 columns of P
+                bool ok = true;
+                int buffer = 0, n = 0;
+                uint32_t round = 0;
+                for (int i = walk.next(0); i < walk.count && ok; i = walk.next(i + 1), ++n) {
+                    ok = mbar_wait(p_full(buffer), round, abort_flag);
+                    if (!ok) break;
+#pragma unroll 1
+                    for (int c = 0; c < C::GRANULES; ++c) {
+                        const int slot = C::SLOTS + at;
+                        ok = mbar_wait(full(slot), phase, abort_flag);
+                        if (!ok) break;
+                        tc5::tc_fence_after();
+                        const uint64_t bd = smem_desc(ring + slot * C::GRANULE, C::V_KEYS * 128, 1024);
+                        const uint32_t pa = tmem + buffer * BKEY + c * (C::V_KEYS / KEYS) * 8;
+#pragma unroll
+                        for (int k = 0; k < C::V_KEYS / KEYS; ++k)
+#pragma unroll
+                            for (int term = 0; term < C::PT; ++term)
+                                umma_ts<Q8>(tmem + C::O_COL, pa + term * 32 + k * 8, bd + k * KEYS * 8, id_pv | (term == 2 ? E5M2 : 0u), n > 0 || c > 0 || k > 0 || term > 0);
+                        tc5::umma_commit(empty(slot));
+                        advance();
+                    }
+                    if (!ok) break;
+                    tc5::umma_commit(p_read(buffer));
                     tc5::umma_commit(o_done(n & 1));
+                    if (++buffer == C::BUFFERS) { buffer = 0; round ^= 1u; }
                 }
                 if (ok) tc5::umma_commit(finished);
             }
@@ -566,18 +567,15 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
             bool tail = key0 + BKEY > s.L;
             if (walk.range != nullptr) tail = tail || __ldg(walk.range + walk.first + i).x < 0;
             if (tail) {
-                // in the ring, V of block n has n blocks of V before it, and K up to BUFFERS - 1 blocks further on
-                int blocks = 2 * n + 1;
-                for (int b = 1, j = after_i; b < C::BUFFERS && j < walk.count; ++b, j = walk.next(j + 1)) ++blocks;
-                const int key = row, at = key0 + key, before = blocks * C::GRANULES;
+                const int key = row, at = key0 + key;
                 const bool bad = at >= s.L || (walk.range != nullptr && __ldg(a.k_docs + (size_t)e * a.keys + at) < 0);
 #pragma unroll 1
                 for (int c = 0; c < C::GRANULES; ++c) {
-                    const int at_slot = (before + c) % C::SLOTS;
-                    ok = ok && mbar_wait(full(at_slot), (uint32_t)(((before + c) / C::SLOTS) & 1), abort_flag);
+                    const int granule = n * C::GRANULES + c, slot = C::SLOTS + granule % C::SLOTS;
+                    ok = ok && mbar_wait(full(slot), (uint32_t)(granule / C::SLOTS & 1), abort_flag);
                     if (bad && key / C::V_KEYS == c)
                         for (int k = 0; k < C::GRANULES * 8; ++k)
-                            *reinterpret_cast<uint4*>(gen + C::OFF_R + at_slot * C::GRANULE + (k >> 3) * (C::V_KEYS * 128) + key % C::V_KEYS * 128 + (k & 7) * 16) = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4*>(gen + C::OFF_R + slot * C::GRANULE + (k >> 3) * (C::V_KEYS * 128) + key % C::V_KEYS * 128 + (k & 7) * 16) = make_uint4(0, 0, 0, 0);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             }

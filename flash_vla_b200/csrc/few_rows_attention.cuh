@@ -279,7 +279,7 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
             for (int r = 0; r < NR; ++r) v[r] = (Q8 ? fmaf(c[(NR + r) % C::NS], 1.f / 32.f, c[r]) : c[r]) * (row_f[r] * kf);
             if (capped) {
 #pragma unroll
-                for (int r = 0; r < NR; ++r) v[r] = cap2 * tanh_f(v[r]);
+                for (int r = 0; r < NR; ++r) v[r] = cap2 * tanh_far(v[r]);
             }
             if (a.slopes) {
 #pragma unroll

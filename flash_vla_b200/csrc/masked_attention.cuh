@@ -89,11 +89,18 @@ __device__ __forceinline__ float fast_rcp(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// tanh(y) = 1 - 2 / (1 + e^2y), good to 2^-22 of 1; its series up to y^7 where that would cancel (the next term is below 2^-22 of y).
-__device__ __forceinline__ float tanh_f(float y) {
+// tanh of scores over their cap. Its Taylor series to y^13 where every |y| of a thread's scores is at most 1/2 (the next term is below 2^-22 of y), which
+// is all but always so and costs multiply-adds alone; else 1 - 2 / (1 + e^2y), good to 2^-22 of 1, with two special-function instructions and the series
+// to y^7 where that would cancel (|y| < 1/5).
+constexpr float kTanh3 = -1.f / 3.f, kTanh5 = 2.f / 15.f, kTanh7 = -17.f / 315.f, kTanh9 = 62.f / 2835.f, kTanh11 = -1382.f / 155925.f, kTanh13 = 21844.f / 6081075.f;
+__device__ __forceinline__ float tanh_far(float y) {
     const float far = fmaf(-2.f, fast_rcp(1.f + fast_exp2(2.f * kLog2e * y)), 1.f), y2 = y * y;
-    const float near = fmaf(y * y2, fmaf(y2, fmaf(y2, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), y);
+    const float near = fmaf(y * y2, fmaf(y2, fmaf(y2, kTanh7, kTanh5), kTanh3), y);
     return y2 < 0.04f ? near : far;
+}
+__device__ __forceinline__ float tanh_near(float y) {
+    const float y2 = y * y;
+    return y * fmaf(y2, fmaf(y2, fmaf(y2, fmaf(y2, fmaf(y2, fmaf(y2, kTanh13, kTanh11), kTanh9), kTanh7), kTanh5), kTanh3), 1.f);
 }
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int w) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
@@ -115,14 +122,16 @@ __device__ __forceinline__ void ld32_nowait(uint32_t taddr, uint32_t* r) {
           "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr) : "memory");
 }
-// What a CTA's rows may see, block by block. Every role evaluates it from the same memory.
+// What a CTA's rows may see, block by block. Every role evaluates it from the same memory. The last block comes first: where scores fall with distance
+// the maximum is found at once, and nothing is rescaled (every block otherwise: 241 us against 180 at head dim 128, 4 096 causal keys, 32 heads).
 struct Walk {
     int first, count;                 // key blocks of this CTA (of its split), some of which may hold nothing that is seen
     int q_low, q_high;                // documents of the tile's queries
     const int2* range;                // of the episode's key blocks, or null
+    __device__ __forceinline__ int block(int i) const { return first + count - 1 - i; }
     __device__ __forceinline__ bool sees(int i) const {
         if (range == nullptr) return true;
-        const int2 r = __ldg(range + first + i);
+        const int2 r = __ldg(range + block(i));
         return r.y >= q_low && r.x <= q_high;
     }
     __device__ __forceinline__ int next(int i) const {      // the first block from i on that is seen, or count

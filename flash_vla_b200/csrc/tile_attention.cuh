@@ -79,6 +79,20 @@ __device__ __forceinline__ void mul2(float& a0, float& a1, float b) {
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair(a0, a1)), "l"(pair(b, b)));
     unpair(r, a0, a1);
 }
+// scale tanh of two values of at most 1/2, by the series
+__device__ __forceinline__ void tanh2(float& a0, float& a1, float scale) {
+    unsigned long long y = pair(a0, a1), q, t;
+    asm("mul.rn.f32x2 %0, %1, %1;" : "=l"(q) : "l"(y));
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(t) : "l"(q), "l"(pair(kTanh13, kTanh13)), "l"(pair(kTanh11, kTanh11)));
+    asm("fma.rn.f32x2 %0, %1, %0, %2;" : "+l"(t) : "l"(q), "l"(pair(kTanh9, kTanh9)));
+    asm("fma.rn.f32x2 %0, %1, %0, %2;" : "+l"(t) : "l"(q), "l"(pair(kTanh7, kTanh7)));
+    asm("fma.rn.f32x2 %0, %1, %0, %2;" : "+l"(t) : "l"(q), "l"(pair(kTanh5, kTanh5)));
+    asm("fma.rn.f32x2 %0, %1, %0, %2;" : "+l"(t) : "l"(q), "l"(pair(kTanh3, kTanh3)));
+    asm("fma.rn.f32x2 %0, %1, %0, %2;" : "+l"(t) : "l"(q), "l"(pair(1.f, 1.f)));
+    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(y) : "l"(pair(scale, scale)));
+    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(y) : "l"(t));
+    unpair(y, a0, a1);
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -92,8 +106,10 @@ struct TileCfg {
     static constexpr int V_KEYS = BKEY / GRANULES;                                 // keys of a V granule
     static constexpr int Q_ATOMS = HDP / 64, Q_BYTES = Q_ATOMS * 16384;            // as bf16, and as two terms of e4m3
     static constexpr int BUFFERS = HDP == 256 ? 2 : 3;                             // 128 columns each, beside HDP columns of the accumulator
-    static constexpr int SLOTS = HDP == 256 ? 5 : 6;                               // of each ring
-    static constexpr int OFF_Q = 0, OFF_R = OFF_Q + Q_BYTES, OFF_X = OFF_R + 2 * SLOTS * GRANULE;      // rings; a maximum per row, a float per row and group
+    // P as an operand in shared memory: where tensor memory has only two score buffers, these are then free again as soon as the scores have been read
+    static constexpr bool P_SHARED = HDP == 256 && !Q8;
+    static constexpr int SLOTS = P_SHARED ? 4 : (HDP == 256 ? 5 : 6);              // of each ring
+    static constexpr int OFF_Q = 0, OFF_P = OFF_Q + Q_BYTES, OFF_R = OFF_P + (P_SHARED ? BQ * BKEY * 2 : 0), OFF_X = OFF_R + 2 * SLOTS * GRANULE;      // rings; a maximum per row, a float per row and group
     static constexpr int OFF_BAR = OFF_X + 3 * BQ * 4;
     static constexpr int SMEM = 1024 + OFF_BAR + 344;
     static constexpr int THREADS = 32 * (SOFTMAX0 + SOFTMAX_WARPS);
@@ -115,7 +131,7 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
     auto p_full = [&](int b) { return bars + 40 + b * 8; };
     auto o_done = [&](int b) { return bars + 64 + b * 8; };                // of even and odd blocks
     const uint32_t finished = bars + 80;                                   // all products (a wait for a block's own phase could come too late for its parity)
-    auto p_read = [&](int b) { return bars + 96 + b * 8; };                // the product has read P: the buffer may take scores
+    auto p_read = [&](int b) { return bars + 96 + b * 8; };                // the buffer may take scores: the product has read P, or (P_SHARED) the softmax its scores
     // rings: K slots, then V slots
     auto full = [&](int s) { return bars + 120 + s * 8; };
     auto empty = [&](int s) { return bars + 120 + C::SLOTS * 16 + s * 8; };
@@ -134,7 +150,7 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
 
     if (tid == 0) {
         mbar_init(q_full, 1); mbar_init(q_ready, SOFTMAX_WARPS);
-        for (int b = 0; b < C::BUFFERS; ++b) { mbar_init(s_full(b), 1); mbar_init(p_full(b), SOFTMAX_WARPS / 2); mbar_init(p_read(b), 1); }
+        for (int b = 0; b < C::BUFFERS; ++b) { mbar_init(s_full(b), 1); mbar_init(p_full(b), SOFTMAX_WARPS / 2); mbar_init(p_read(b), C::P_SHARED ? 4 : 1); }
         for (int b = 0; b < 2; ++b) mbar_init(o_done(b), 1);
         mbar_init(finished, 1);
         for (int s = 0; s < 2 * C::SLOTS; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
@@ -178,8 +194,9 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
             walk.q_high = shared_int[1];
             walk.range = p.doc_range + (size_t)e * blocks;
             walk.first = 0;
+            walk.count = last;
             for (int j = tid; j < last; j += C::THREADS)
-                if (walk.sees(j)) { atomicMin(shared_int + 2, j); atomicMax(shared_int + 3, j); }
+                if (walk.sees(j)) { atomicMin(shared_int + 2, walk.block(j)); atomicMax(shared_int + 3, walk.block(j)); }
             __syncthreads();
             first = min(shared_int[2], last);
             last = max(first, min(last, shared_int[3] + 1));
@@ -210,7 +227,7 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                         ok = mbar_wait(empty(at), phase ^ 1u, abort_flag);
                         if (!ok) break;
                         mbar_expect_tx(full(at), C::GRANULE);
-                        tma_load_4d(ring + at * C::GRANULE, &tmK, full(at), c * (128 / C::ELEM), (walk.first + i) * BKEY, kv * p.k_mul[0], e * p.k_mul[1]);
+                        tma_load_4d(ring + at * C::GRANULE, &tmK, full(at), c * (128 / C::ELEM), walk.block(i) * BKEY, kv * p.k_mul[0], e * p.k_mul[1]);
                         advance();
                     }
                 }
@@ -228,7 +245,7 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                         mbar_expect_tx(full(slot), C::GRANULE);
 #pragma unroll
                         for (int d = 0; d < C::GRANULES; ++d)
-                            tma_load_4d(ring + slot * C::GRANULE + d * C::V_KEYS * 128, &tmV, full(slot), d * (128 / C::ELEM), (walk.first + i) * BKEY + c * C::V_KEYS,
+                            tma_load_4d(ring + slot * C::GRANULE + d * C::V_KEYS * 128, &tmV, full(slot), d * (128 / C::ELEM), walk.block(i) * BKEY + c * C::V_KEYS,
                                         kv * p.v_mul[0], e * p.v_mul[1]);
                         advance();
                     }
@@ -284,12 +301,13 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                         for (int k = 0; k < C::V_KEYS / KEYS; ++k)
 #pragma unroll
                             for (int term = 0; term < C::PT; ++term)
-                                umma_ts<Q8>(tmem + C::O_COL, pa + term * 32 + k * 8, bd + k * KEYS * 8, id_pv | (term == 2 ? E5M2 : 0u), n > 0 || c > 0 || k > 0 || term > 0);
+                                if (C::P_SHARED) tc5::umma_bf16(tmem + C::O_COL, smem_desc(base + C::OFF_P + (c >> 1) * 16384 + ((c & 1) * 2 + k) * 32, 16, 1024), bd + k * KEYS * 8, id_pv, n > 0 || c > 0 || k > 0);
+                                else umma_ts<Q8>(tmem + C::O_COL, pa + term * 32 + k * 8, bd + k * KEYS * 8, id_pv | (term == 2 ? E5M2 : 0u), n > 0 || c > 0 || k > 0 || term > 0);
                         tc5::umma_commit(empty(slot));
                         advance();
                     }
                     if (!ok) break;
-                    tc5::umma_commit(p_read(buffer));
+                    if (!C::P_SHARED) tc5::umma_commit(p_read(buffer));
                     tc5::umma_commit(o_done(n & 1));
                     if (++buffer == C::BUFFERS) { buffer = 0; round ^= 1u; }
                 }
@@ -372,7 +390,7 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
         int n = 0, buffer = g, parity = 0, i = walk.next(0);
         if (g == 1 && i < walk.count) { i = walk.next(i + 1); n = 1; }
         while (i < walk.count) {
-            const int after_i = walk.next(i + 1), key0 = (walk.first + i) * BKEY;
+            const int after_i = walk.next(i + 1), key0 = walk.block(i) * BKEY;
             float kf[8], lv[8];                                        // (8-bit cache) per 16 keys: factor of the scores, log2 of V's scale
             if (Q8 && busy) {
 #pragma unroll
@@ -391,14 +409,27 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
 #pragma unroll
                 for (int c = 0; c < 4; ++c) ld32_nowait(t_s + 32 * c, r + 32 * c);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                if (C::P_SHARED) {
+                    tc5::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc5::mbar_arrive(p_read(buffer));
+                }
                 float (&v)[BKEY] = reinterpret_cast<float (&)[BKEY]>(r);
                 if (!fast) {
                     if (Q8 || capped || a.k_pos) {
 #pragma unroll
                         for (int c = 0; c < BKEY; c += 2) mul2(v[c], v[c + 1], Q8 ? kf[c >> 4] : factor);
                         if (capped) {
+                            float size = 0.f;
 #pragma unroll
-                            for (int c = 0; c < BKEY; ++c) v[c] = cap2 * tanh_f(v[c]);
+                            for (int c = 0; c < BKEY; c += 2) size = max3(size, fabsf(v[c]), fabsf(v[c + 1]));
+                            if (__all_sync(0xffffffffu, size <= 0.5f)) {
+#pragma unroll
+                                for (int c = 0; c < BKEY; c += 2) tanh2(v[c], v[c + 1], cap2);
+                            } else {
+#pragma unroll
+                                for (int c = 0; c < BKEY; ++c) v[c] = cap2 * tanh_far(v[c]);
+                            }
                         }
                         if (a.slopes) {
                             if (a.k_pos) {
@@ -529,10 +560,21 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                         add2(s2, s3, v[c + 2], v[c + 3]);
                         r[c / 2] = pack_bf16x2(v[c], v[c + 1]);
                         r[c / 2 + 1] = pack_bf16x2(v[c + 2], v[c + 3]);
-                        if (c == 60) st32_nowait(t_s, r);
+                        if (!C::P_SHARED && c == 60) st32_nowait(t_s, r);
                     }
                     l += (s0 + s1) + (s2 + s3);
-                    st32_nowait(t_s + 32, r + 32);
+                    if (C::P_SHARED) {
+                        // the products of the block before have read P (128-byte swizzle: 8 keys are a piece of a row's 128 bytes in an atom of 64)
+                        ok = ok && (n == 0 || mbar_wait(o_done(g ^ 1), (uint32_t)(((n - 1) >> 1) & 1), abort_flag));
+                        __syncwarp();
+#pragma unroll
+                        for (int k = 0; k < 16; ++k)
+                            *reinterpret_cast<uint4*>(gen + C::OFF_P + (k >> 3) * 16384 + row * 128 + (((k & 7) ^ (row & 7)) << 4)) =
+                                make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    } else {
+                        st32_nowait(t_s + 32, r + 32);
+                    }
                 } else {
                     // three terms of four values to a word, 32 columns each
                     uint32_t w[3][32];
@@ -561,11 +603,16 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
 #pragma unroll
                     for (int term = 0; term < 3; ++term) st32_nowait(t_s + 32 * term, w[term]);
                 }
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                if (!C::P_SHARED) asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            } else if (C::P_SHARED) {
+                // (waits like the others: two blocks on, it would otherwise signal the same barrier before they have signalled it for this one)
+                if (lane == 0) tc5::mbar_arrive(p_read(buffer));
+                ok = ok && (n == 0 || mbar_wait(o_done(g ^ 1), (uint32_t)(((n - 1) >> 1) & 1), abort_flag));
+                __syncwarp();
             }
             // keys whose values may be anything, behind the last one or under a negative document: zeros, for 0 * NaN would reach every row
             bool tail = key0 + BKEY > s.L;
-            if (walk.range != nullptr) tail = tail || __ldg(walk.range + walk.first + i).x < 0;
+            if (walk.range != nullptr) tail = tail || __ldg(walk.range + walk.block(i)).x < 0;
             if (tail) {
                 const int key = row, at = key0 + key;
                 const bool bad = at >= s.L || (walk.range != nullptr && __ldg(a.k_docs + (size_t)e * a.keys + at) < 0);

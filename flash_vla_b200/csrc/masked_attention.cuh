@@ -54,8 +54,9 @@ struct Tile {
     int q_mul[2], k_mul[2], v_mul[2];           // 0 where an axis (K/V head, episode) is broadcast: its coordinate stays 0
     float* part_o;                              // [split][row][HDP] fp32, row = ((e * tokens + t) * heads + h)
     float2* part_ml;                            // [split][row] maximum (log2) and sum
-    float* scores;                              // [row][pitch] log2 units, or null: what the keys' weights are made of
-    long long pitch;
+    float* scores;                              // log2 units, or null: what the keys' weights are made of
+    long long pitch;                            // few rows: [row][pitch]
+    int key_blocks;                             // many: [episode, K/V head, tile][key block][4 keys][128 rows][4]
     const int2* doc_range;                      // [episode][key block] smallest and largest document
     int* status;
 };
@@ -174,13 +175,18 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) attention_join_kernel(const _
         const float w = ml.y == 0.f ? 0.f : (ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - top));
         l += warp_sum(ml.y == 0.f ? 0.f : ml.y * w);
         const int have = min(32, (p.splits - s0 + warps - 1) / warps);
-#pragma unroll (PER == 1 ? 16 : 4)
-        for (int i = 0; i < have; ++i) {
-            const float f = __shfl_sync(0xffffffffu, w, i), used = __shfl_sync(0xffffffffu, ml.y, i);
+        constexpr int BATCH = PER == 1 ? 16 : 4;                                     // loads in flight before the first is used
+        for (int i = 0; i < have; i += BATCH) {
+            float x[BATCH][PER];
 #pragma unroll
-            for (int c = 0; c < PER; ++c) {
-                const float x = o[(size_t)(s0 + i * warps) * pitch + 32 * c];
-                acc[c] = fmaf(f, used != 0.f ? x : 0.f, acc[c]);
+            for (int k = 0; k < BATCH; ++k)
+#pragma unroll
+                for (int c = 0; c < PER; ++c) x[k][c] = o[(size_t)(s0 + min(i + k, have - 1) * warps) * pitch + 32 * c];
+#pragma unroll
+            for (int k = 0; k < BATCH; ++k) {
+                const float f = __shfl_sync(0xffffffffu, w, i + k & 31), used = __shfl_sync(0xffffffffu, ml.y, i + k & 31);
+#pragma unroll
+                for (int c = 0; c < PER; ++c) acc[c] = fmaf(i + k < have ? f : 0.f, i + k < have && used != 0.f ? x[k][c] : 0.f, acc[c]);
             }
         }
     }
@@ -221,12 +227,20 @@ __global__ void __launch_bounds__(32 * WEIGHT_WARPS) key_weights_kernel(const __
     // tokens before this one do not see key j (by its number), and their scores were not left
     const int from = by_number && j >= s.prefix ? max(0, j - s.start) : 0;
     float sum = 0.f;
-#pragma unroll 8
-    for (int r = warp; r < rows; r += warps) {
-        const int h = r / s.n, t = r - h * s.n;
-        const size_t row = row0 + (size_t)h * a.tokens + t;
-        const float z = a.lse[row], x = p.scores[row * p.pitch + j];      // what was not left is read as well (j < pitch), and dropped
-        if (inside && t >= from && z != -INFINITY) sum += fast_exp2(fmaf(z, -kLog2e, x));
+    constexpr int BATCH = 8;                                                         // loads in flight before the first is used
+    for (int r0 = warp; r0 < rows; r0 += BATCH * warps) {
+        float z[BATCH], x[BATCH];
+        bool seen[BATCH];
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            const int r = min(r0 + k * warps, rows - 1), h = r / s.n, t = r - h * s.n;
+            const size_t row = row0 + (size_t)h * a.tokens + t;
+            z[k] = a.lse[row];
+            x[k] = p.scores[row * p.pitch + j];                                      // what was not left is read as well (j < pitch), and dropped
+            seen[k] = r0 + k * warps < rows && inside && t >= from;
+        }
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) sum += seen[k] && z[k] != -INFINITY ? fast_exp2(fmaf(z[k], -kLog2e, x[k])) : 0.f;
     }
     part[warp][threadIdx.x & 31] = sum;
     __syncthreads();
@@ -234,6 +248,46 @@ __global__ void __launch_bounds__(32 * WEIGHT_WARPS) key_weights_kernel(const __
     for (int w = 1; w < warps; ++w) sum += part[w][threadIdx.x];
     float* at = a.weights + (size_t)e * a.keys + j;
     *at = (a.decay != 0.f ? a.decay * *at : 0.f) + sum;
+}
+
+// The same from the scores of tiles: a CTA has a block of 128 keys of an episode, a warp four keys at a time, a lane every 32nd row.
+__global__ void __launch_bounds__(32 * WEIGHT_WARPS) tile_weights_kernel(const __grid_constant__ Tile p) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const Args& a = p.a;
+    const int e = blockIdx.y, block = blockIdx.x / 2, lane = threadIdx.x & 31, quad = blockIdx.x % 2 * WEIGHT_WARPS + (threadIdx.x >> 5);
+    const Episode s = episode_of(a, e);
+    const int j = block * BKEY + quad * 4;
+    if (j >= s.L) return;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int kt = 0; kt < a.kv_heads * p.tiles; ++kt) {
+        const int kv = kt / p.tiles, tile = kt - kv * p.tiles, t0 = tile * p.tile_tokens, tokens = min(p.tile_tokens, s.n - t0);
+        // what the tile has walked (as the attention kernel has it)
+        if (tokens <= 0 || (a.causal && a.k_pos == nullptr && block * BKEY >= max(s.start + t0 + tokens, s.prefix))) continue;
+        const float4* from = reinterpret_cast<const float4*>(p.scores) + ((((size_t)e * a.kv_heads + kv) * p.tiles + tile) * p.key_blocks + block) * (BQ * BKEY / 4) + quad * BQ;
+        float4 x[BQ / 32];
+        float z[BQ / 32];
+#pragma unroll
+        for (int k = 0; k < BQ / 32; ++k) {
+            const int r = k * 32 + lane, t = r / p.group, h = kv * p.group + r - t * p.group;
+            const bool mine = t < tokens;
+            x[k] = mine ? from[r] : make_float4(0.f, 0.f, 0.f, 0.f);
+            z[k] = mine ? a.lse[((size_t)e * a.heads + h) * a.tokens + t0 + t] : -INFINITY;
+        }
+#pragma unroll
+        for (int k = 0; k < BQ / 32; ++k) {
+            const float v[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) sum[c] += z[k] != -INFINITY ? fast_exp2(fmaf(z[k], -kLog2e, v[c])) : 0.f;
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) sum[c] = warp_sum(sum[c]);
+    if (lane < 4 && j + lane < s.L) {
+        float* at = a.weights + (size_t)e * a.keys + j + lane;
+        const float mine = lane == 0 ? sum[0] : (lane == 1 ? sum[1] : (lane == 2 ? sum[2] : sum[3]));
+        *at = (a.decay != 0.f ? a.decay * *at : 0.f) + mine;
+    }
 }
 
 // Tensor map of a strided operand, innermost axis contiguous; an axis of stride 0 is left at one element (its coordinate is 0).
@@ -280,12 +334,18 @@ inline int plan_splits(const Args& a) {
     return (int)(room < 1 ? 1 : (room < blocks ? room : (blocks > 0 ? blocks : 1)));
 }
 inline size_t score_pitch(const Args& a) { return ((size_t)a.keys + BKEY - 1) / BKEY * BKEY; }
+// Of the scores: rows one by one, or tiles of 128.
+inline size_t score_bytes(const Args& a) {
+    const int tile_tokens = BQ / (a.heads / a.kv_heads);
+    const size_t rows = takes_few(a) ? (size_t)a.episodes * a.tokens * a.heads : (size_t)a.episodes * a.kv_heads * ((a.tokens + tile_tokens - 1) / tile_tokens) * BQ;
+    return rows * score_pitch(a) * sizeof(float);
+}
 inline size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 inline size_t workspace_bytes(const Args& a) {
     const int splits = plan_splits(a);
     const size_t rows = (size_t)a.episodes * a.tokens * a.heads;
     size_t n = a.q_docs ? align256((size_t)a.episodes * ((a.keys + BKEY - 1) / BKEY) * sizeof(int2)) : 0;
-    if (a.weights) n += rows * score_pitch(a) * sizeof(float);
+    if (a.weights) n += score_bytes(a);
     if (splits > (takes_few(a) ? CLUSTER : 1)) n += align256(splits * rows * sizeof(float2)) + splits * rows * padded_dim(a) * sizeof(float);
     return n;
 }
@@ -344,9 +404,10 @@ inline int launch_attention(const Args& a, void* ws, int* status, cudaStream_t s
     }
     p.scores = nullptr;
     p.pitch = (long long)score_pitch(a);
+    p.key_blocks = blocks;
     if (a.weights) {
         p.scores = reinterpret_cast<float*>(at);
-        at += rows * p.pitch * sizeof(float);
+        at += score_bytes(a);
     }
     p.part_ml = reinterpret_cast<float2*>(at);
     p.part_o = reinterpret_cast<float*>(at + align256(p.splits * rows * sizeof(float2)));
@@ -384,8 +445,13 @@ inline int launch_attention(const Args& a, void* ws, int* status, cudaStream_t s
         rc = hdp == 64 ? launch_tile<64, false>(p, tmQ, tmK, tmV, st) : (hdp == 128 ? launch_tile<128, false>(p, tmQ, tmK, tmV, st) : launch_tile<256, false>(p, tmQ, tmK, tmV, st));
     }
     if (rc || a.weights == nullptr || a.keys == 0) return rc;
-    const int rows_each = a.tokens * a.heads, warps = rows_each < 4 * WEIGHT_WARPS ? (rows_each + 3) / 4 : WEIGHT_WARPS;      // four rows or more for a warp
-    const cudaError_t e = launch_pdl(key_weights_kernel, dim3((a.keys + 31) / 32, a.episodes), dim3(32 * warps), 0, st, p);
+    cudaError_t e;
+    if (few) {
+        const int rows_each = a.tokens * a.heads, warps = rows_each < 4 * WEIGHT_WARPS ? (rows_each + 3) / 4 : WEIGHT_WARPS;      // four rows or more for a warp
+        e = launch_pdl(key_weights_kernel, dim3((a.keys + 31) / 32, a.episodes), dim3(32 * warps), 0, st, p);
+    } else {
+        e = launch_pdl(tile_weights_kernel, dim3(2 * blocks, a.episodes), dim3(32 * WEIGHT_WARPS), 0, st, p);
+    }
     if (e != cudaSuccess) { set_error("key_weights_kernel: %s", cudaGetErrorString(e)); return FVLA_ERR_LAUNCH; }
     return check_launch("key_weights_kernel");
 }

@@ -262,8 +262,8 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
                 const size_t at = (size_t)(min(j, a.keys - 1) >> shift) * a.kv_heads;
                 kf = __ldg(ks + at);
                 const float x = __ldg(vs + at);
-                lv = (float)((int)(__float_as_uint(x) >> 23) - 127);
-                iv = q8::inverse_pow2(x);
+                lv = q8::log2_of_scale(x);
+                iv = __frcp_rn(x);
             }
             const int kp = a.k_pos ? __ldg(a.k_pos + (size_t)e * a.keys + min(j, a.keys - 1)) : j;
             ok = ok && mbar_wait(s_full(b), (uint32_t)((n >> 1) & 1), abort_flag);

@@ -4,7 +4,7 @@
 //
 // e4m3 is a floating format: a power-of-two scale loses none of its precision (it only moves the exponents), and division by it is exact, so a value
 // is rounded once, to e4m3, and a block whose scale has to grow later moves its old values by a power of two, exact down to the subnormals.
-// Values that are not finite are held as NaN and do not take part in amax.
+// Values that are not finite are held as NaN and do not take part in amax. (Reciprocals below are exact for powers of two.)
 #pragma once
 
 #include "common.cuh"
@@ -21,8 +21,12 @@ __device__ __forceinline__ float scale_of(uint32_t amax) {
     const int e = x - ((amax & 0x7fu) <= 0x60u ? 8 : 7);
     return __int_as_float((max(e, kMinExponent) + 127) << 23);
 }
-// 1 / s of a power of two s within [2^-120, 2^121].
-__device__ __forceinline__ float inverse_pow2(float s) { return __int_as_float((254 << 23) - __float_as_int(s)); }
+// log2 of a positive scale, exact for a power of two. (Scales that this file makes are powers of two; a program may bring others.)
+__device__ __forceinline__ float log2_of_scale(float s) {
+    const uint32_t u = __float_as_uint(s), m = u & 0x7fffffu;
+    const float whole = (float)((int)(u >> 23) - 127);
+    return m == 0 ? whole : whole + __log2f(__uint_as_float(m | 0x3f800000u));
+}
 
 __device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
     uint16_t r;
@@ -118,14 +122,14 @@ __global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const __gr
     const float now = fmaxf(was, scale_of(amax));
     if (threadIdx.x == 0) *scale = now;
     if (now != was) {
-        const float ratio = was * inverse_pow2(now);
+        const float ratio = was * __frcp_rn(now);
         for (int i = threadIdx.x; i < old * chunks; i += threads) {
             uint4* at = reinterpret_cast<uint4*>(held + (long long)(i / chunks) * p.hs[kv][1] + (i % chunks) * 16);
             const uint4 v = *at;
             *at = make_uint4(rescale4(v.x, ratio), rescale4(v.y, ratio), rescale4(v.z, ratio), rescale4(v.w, ratio));
         }
     }
-    const float inv = inverse_pow2(now);
+    const float inv = __frcp_rn(now);
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
         const int i = first * chunks + k * threads + threadIdx.x;
@@ -339,7 +343,7 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const __grid_c
     __syncthreads();
     const float now = fmaxf(fmaxf(warp_top[0], warp_top[1]), fmaxf(warp_top[2], warp_top[3]));
     if (tid == 0) p.out_scale[kv][((size_t)e * p.out_blocks + b) * p.kv_heads + head] = now;
-    const float inv = inverse_pow2(now);
+    const float inv = __frcp_rn(now);
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
         const int i = k * MOVE_THREADS + tid, r = i / chunks;

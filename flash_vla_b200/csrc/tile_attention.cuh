@@ -12,7 +12,7 @@
 // of an e4m3 term and an e5m2 term (what rounding to 4 bits leaves of 8 has at most 3; below 2^-16, 2^-23 of the largest, is lost), a probability the sum
 // of two e4m3 terms and an e5m2 term (11 bits; the last holds what is below e4m3's range). Probabilities stand against the running maximum at 2^6
 // and are rescaled when it has grown by 2^2, so that what falls below the last term is under 2^-24 of the largest. The scale of K multiplies the scores in fp32; the
-// scale of V, a power of two, moves into the exponent of P (w = log2 p + log2 V_scale, P = 2^(w - max w)), and the row sum takes it back.
+// scale of V moves into the exponent of P (w = log2 p + log2 V_scale, P = 2^(w - max w)), and the row sum takes it back.
 #pragma once
 
 namespace fvla {
@@ -391,13 +391,13 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
         if (g == 1 && i < walk.count) { i = walk.next(i + 1); n = 1; }
         while (i < walk.count) {
             const int after_i = walk.next(i + 1), key0 = walk.block(i) * BKEY;
-            float kf[8], lv[8];                                        // (8-bit cache) per 16 keys: factor of the scores, log2 of V's scale
+            float kf[8], lv[8];                                        // (8-bit cache) per 16 keys: factor of the scores; log2 of V's scale
             if (Q8 && busy) {
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                     const size_t at = ((size_t)e * (a.keys >> shift) + (min(key0 + c * 16, a.keys - 1) >> shift)) * a.kv_heads + kv;
                     kf[c] = factor * __ldg(a.k_scale + at);
-                    lv[c] = (float)((int)(__float_as_uint(__ldg(a.v_scale + at)) >> 23) - 127);
+                    lv[c] = q8::log2_of_scale(__ldg(a.v_scale + at));
                 }
             }
             const uint32_t t_s = tmem + t_lane + buffer * BKEY;

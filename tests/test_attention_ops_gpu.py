@@ -98,6 +98,9 @@ def test_documents_in_any_order(D, H, HK, causal):
         K[:, ids[0] < 0], V[:, ids[0] < 0] = INF, NAN
         out, want = check(Q, K, V, D ** -0.5, causal=causal, q_docs=ids, k_docs=ids)
         assert (out[:, ids[0] < 0] == 0).all()
+    for T in (1, 3):                                                        # few rows
+        q_docs = ids[:, 460:460 + T].contiguous()
+        check(randn(7, 1, T, H, D), K, V, D ** -0.5, q_docs=q_docs, k_docs=ids)
     other = torch.full_like(ids, 9)
     out, lse = attend(Q, K, V, 1.0, q_docs=other, k_docs=ids)            # a document that no key has
     assert (out == 0).all() and (lse == -INF).all()
@@ -338,6 +341,46 @@ def test_cache_attention_with_uneven_scales():
         big, small = (Q.float() * size).to(bf16), 0.02 / size
         op_table().cache_attention(big, cache, lengths, small, out)
         A.check_out(out, A.attention(big, A.widened(cache.K, cache.K_scale), A.widened(cache.V, cache.V_scale), small, k_lens=lengths), 128, P_FP16)
+
+
+@pytest.mark.parametrize("T", [1, 30])
+def test_cache_attention_with_scales_of_any_size(T):
+    """Scales that a program brings need not be powers of two."""
+    cache, _, _ = filled(19, 2, 512, 2, 128, 32, 0.3)
+    for scale in cache[2:]:
+        scale.mul_(torch.rand(scale.shape, device="cuda", generator=torch.Generator("cuda").manual_seed(5)) + 0.7)
+    Q, lengths = randn(20, 2, T, 8, 128), A.ints([512, 300])
+    out, w = torch.zeros_like(Q), torch.zeros(2, 512, device="cuda")
+    op_table().cache_attention(Q, cache, lengths, 0.08, out, weights=w, decay=0.0)
+    want = A.attention(Q, A.widened(cache.K, cache.K_scale), A.widened(cache.V, cache.V_scale), 0.08, k_lens=lengths)
+    A.check_out(out, want, 128, P_FP16)
+    A.check_weights(w, want, 128, lengths, torch.zeros_like(w), 0.0)
+
+
+def test_cache_rows_far_apart():
+    """Rows 32 KB apart, 2.3 GB of them: byte offsets pass 31 bits in all four operators."""
+    rows, HK, D, keep = 70016, 1, 64, 64
+    store = torch.zeros(2, rows, 1, 32768, dtype=torch.uint8, device="cuda").view(e4m3)
+    scales = [torch.ones(1, rows // 64, HK, device="cuda") for _ in range(2)]
+    cache = QuantizedCache(store[:1, :, :, :D], store[1:, :, :, -D:], *scales)
+    K, V = randn(58, 1, rows, HK, D), randn(59, 1, rows, HK, D)
+    op_table().cache_append(K, V, cache, A.ints([0]))
+    dense = allocate_quantized_cache(1, rows, HK, D, "cuda")
+    op_table().cache_append(K, V, dense, A.ints([0]))
+    for a, b in zip(cache, dense):
+        assert A.same_bits(a.contiguous(), b)
+    for T in (1, 40):
+        Q = randn(60, 1, T, 2, D)
+        outs = [torch.zeros_like(Q) for _ in range(2)]
+        for c, o in zip((cache, dense), outs):
+            op_table().cache_attention(Q, c, A.ints([rows - 5]), 0.1, o)
+        assert torch.equal(*outs)
+    w = torch.zeros(1, rows, device="cuda")
+    w[0, rows - 200:] = 1.0
+    small = allocate_quantized_cache(1, keep, HK, D, "cuda")
+    op_table().cache_evict(cache, A.ints([rows]), w, keep, small, A.ints([0]))
+    assert A.same_bits(small.K, cache.K[:, rows - 200:rows - 200 + keep].contiguous()) or not torch.equal(small.K_scale, cache.K_scale[:, :1])
+    assert torch.equal(A.widened(small.V, small.V_scale), A.widened(cache.V.contiguous(), cache.V_scale)[:, rows - 200:rows - 200 + keep])
 
 
 @pytest.mark.parametrize("positions", ["evicted", "shuffled"])

@@ -111,13 +111,25 @@ __global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const __gr
 #pragma unroll
         for (int h = 0; h < 2; ++h) u[k][h] = mine ? __ldg(src + h) : make_uint4(0, 0, 0, 0);
     }
+    // two magnitudes at a time; a block with a value that is not finite (all but none) is looked through again, and rounded with care below
+    uint32_t both = 0;
 #pragma unroll
     for (int k = 0; k < PER; ++k)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) amax = amax_pair(amax_pair(amax_pair(amax_pair(amax, u[k][h].x), u[k][h].y), u[k][h].z), u[k][h].w);
+        for (int h = 0; h < 2; ++h)
+            both = __vmaxu2(__vmaxu2(both, __vmaxu2(u[k][h].x & 0x7fff7fffu, u[k][h].y & 0x7fff7fffu)), __vmaxu2(u[k][h].z & 0x7fff7fffu, u[k][h].w & 0x7fff7fffu));
+    amax = max(both & 0xffffu, both >> 16);
+    const bool odd = __syncthreads_or(amax >= 0x7f80u);          // and every thread has read the old scale
+    if (odd) {
+        amax = 0;
+#pragma unroll
+        for (int k = 0; k < PER; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) amax = amax_pair(amax_pair(amax_pair(amax_pair(amax, u[k][h].x), u[k][h].y), u[k][h].z), u[k][h].w);
+    }
     amax = __reduce_max_sync(0xffffffffu, amax);
     if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = amax;
-    __syncthreads();                                             // and every thread has read the old scale
+    __syncthreads();
     for (int i = 0; i < threads / 32; ++i) amax = max(amax, warp_max[i]);
     const float now = fmaxf(was, scale_of(amax));
     if (threadIdx.x == 0) *scale = now;
@@ -135,10 +147,19 @@ __global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const __gr
         const int i = first * chunks + k * threads + threadIdx.x;
         if (i >= last * chunks) break;
         uint32_t o[4];
+        if (odd) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            o[2 * h] = quantize_pair(u[k][h].x, inv) | (quantize_pair(u[k][h].y, inv) << 16);
-            o[2 * h + 1] = quantize_pair(u[k][h].z, inv) | (quantize_pair(u[k][h].w, inv) << 16);
+            for (int h = 0; h < 2; ++h) {
+                o[2 * h] = quantize_pair(u[k][h].x, inv) | (quantize_pair(u[k][h].y, inv) << 16);
+                o[2 * h + 1] = quantize_pair(u[k][h].z, inv) | (quantize_pair(u[k][h].w, inv) << 16);
+            }
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float2 a = unpack_bf16x2(u[k][h].x), b2 = unpack_bf16x2(u[k][h].y), c = unpack_bf16x2(u[k][h].z), d = unpack_bf16x2(u[k][h].w);
+                o[2 * h] = to_e4m3x2(a.x * inv, a.y * inv) | (to_e4m3x2(b2.x * inv, b2.y * inv) << 16);
+                o[2 * h + 1] = to_e4m3x2(c.x * inv, c.y * inv) | (to_e4m3x2(d.x * inv, d.y * inv) << 16);
+            }
         }
         *reinterpret_cast<uint4*>(held + (long long)(i / chunks) * p.hs[kv][1] + (i % chunks) * 16) = make_uint4(o[0], o[1], o[2], o[3]);
     }

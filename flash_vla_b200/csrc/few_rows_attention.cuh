@@ -45,7 +45,7 @@ __device__ __forceinline__ void st16(uint32_t taddr, const float* v) {
           "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]) : "memory");
 }
 
-constexpr int FEW_THREADS = 192;
+constexpr int FEW_THREADS = 192, CLUSTER = 8;      // shares that a cluster puts together
 
 template <int HDP, bool Q8, int NR>
 struct FewCfg {
@@ -61,8 +61,8 @@ struct FewCfg {
     static constexpr int SLOTS = TILE == 16384 ? 4 : 3;
     static constexpr int PER_SM = NR == 32 ? (TILE == 16384 ? 2 : 1) : (TILE == 16384 ? 3 : (TILE == 32768 ? 2 : 1));
     static constexpr int OFF_Q = 0, OFF_P = OFF_Q + Q_BYTES, OFF_T = OFF_P + P_BYTES;
-    static constexpr int OFF_F = OFF_T + SLOTS * TILE;                   // per row: factor, slope (floats), position, limit (ints)
-    static constexpr int OFF_M = OFF_F + 4 * NR * 4;                     // maxima of the four warps, twice
+    static constexpr int OFF_F = OFF_T + SLOTS * TILE;                   // per row: factor, slope (floats), position, limit, number (ints)
+    static constexpr int OFF_M = OFF_F + 5 * NR * 4;                     // maxima of the four warps, twice
     static constexpr int OFF_W = OFF_M + 2 * 4 * NR * 4;                 // of each warp, per row: the maximum in use, the factor of what is accumulated
     static constexpr int OFF_BAR = OFF_W + 4 * 2 * NR * 4;
     static constexpr int SMEM = 1024 + OFF_BAR + 160;
@@ -110,6 +110,20 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
+    // Q's rows are asked for before the lengths are known: a warp of the softmax has every fourth
+    constexpr int PER = HDP / 32, Q_ROWS = NR / 4;                             // elements of a lane: 4 or 8; rows of a warp
+    uint2 q_raw[Q_ROWS][PER / 4];
+    if (warp >= 2) {
+#pragma unroll
+        for (int i = 0; i < Q_ROWS; ++i) {
+            const int r = i * 4 + (warp & 3), t = r / p.group, h = kv * p.group + r - t * p.group, d = lane * PER;
+#pragma unroll
+            for (int k = 0; k < PER / 4; ++k) {
+                q_raw[i][k] = make_uint2(0, 0);
+                if (t < a.tokens && d + 4 * k < a.dim) q_raw[i][k] = __ldg(reinterpret_cast<const uint2*>(static_cast<const bf16*>(a.q) + e * a.qs[0] + t * a.qs[1] + h * a.qs[2] + d + 4 * k));
+            }
+        }
+    }
     const Episode s = episode_of(a, e);
     int most = s.n > 0 ? s.L : 0;
     if (a.causal && a.k_pos == nullptr) most = max(0, min(most, max(s.start + s.n, s.prefix)));
@@ -181,6 +195,7 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
         float* row_slope = row_f + NR;
         int* row_pos = reinterpret_cast<int*>(row_f + 2 * NR);
         int* row_limit = row_pos + NR;
+        int* row_number = row_limit + NR;                                      // in the log-sum-exps and scores of the episode
         float* maxima = reinterpret_cast<float*>(gen + C::OFF_M);
         float* in_use = reinterpret_cast<float*>(gen + C::OFF_W) + quad * 2 * NR;
         float* rescale = in_use + NR;
@@ -189,19 +204,17 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
         bool ok = true;
 
         if (count > 0) {
-            // Q as the K-major operand, and what the rows have of their own
-            constexpr int PER = HDP / 32;                                      // elements of a lane: 4 or 8
-            for (int r = quad; r < C::NS / C::QT; r += 4) {
-                const int t = r / group, h = kv * group + r - t * group;
+            // Q as the K-major operand, and what the rows have of their own (rows of the operand behind NR, and their columns of S^T, are never looked at)
+#pragma unroll
+            for (int i = 0; i < Q_ROWS; ++i) {
+                const int r = i * 4 + quad, t = r / group, h = kv * group + r - t * group;
                 float q[PER];
                 uint32_t amax = 0;
 #pragma unroll
-                for (int i = 0; i < PER; i += 4) {
-                    uint2 u = make_uint2(0, 0);
-                    const int d = lane * PER + i;
-                    if (r < rows && d < a.dim) u = __ldg(reinterpret_cast<const uint2*>(static_cast<const bf16*>(a.q) + e * a.qs[0] + t * a.qs[1] + h * a.qs[2] + d));
+                for (int k = 0; k < PER / 4; ++k) {
+                    const uint2 u = r < rows ? q_raw[i][k] : make_uint2(0, 0);
                     const float2 x = unpack_bf16x2(u.x), y = unpack_bf16x2(u.y);
-                    q[i] = x.x; q[i + 1] = x.y; q[i + 2] = y.x; q[i + 3] = y.y;
+                    q[4 * k] = x.x; q[4 * k + 1] = x.y; q[4 * k + 2] = y.x; q[4 * k + 3] = y.y;
                     amax = max(max(amax, max(u.x & 0x7fffu, (u.x >> 16) & 0x7fffu)), max(u.y & 0x7fffu, (u.y >> 16) & 0x7fffu));
                 }
                 float f = capped ? a.scale / a.cap : a.scale * kLog2e;
@@ -214,31 +227,26 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
                     const float up = __int_as_float((134 - ex) << 23);
                     f *= __int_as_float((120 + ex) << 23);
                     if (amax >= 0x7f80u) f = __int_as_float(0x7fffffff);        // an infinity or NaN: the row is NaN
-                    uint32_t one[PER / 4], two[PER / 4];
 #pragma unroll
-                    for (int i = 0; i < PER; i += 4) {
-                        const float x[4] = {q[i] * up, q[i + 1] * up, q[i + 2] * up, q[i + 3] * up};
+                    for (int k = 0; k < PER / 4; ++k) {
+                        const float x[4] = {q[4 * k] * up, q[4 * k + 1] * up, q[4 * k + 2] * up, q[4 * k + 3] * up};
                         const uint32_t lo = q8::to_e4m3x2(x[0], x[1]), hi = q8::to_e4m3x2(x[2], x[3]);
                         const float2 a0 = q8::from_e4m3x2(lo), a1 = q8::from_e4m3x2(hi);
-                        one[i / 4] = lo | hi << 16;
-                        two[i / 4] = q8::to_e4m3x2((x[0] - a0.x) * 32.f, (x[1] - a0.y) * 32.f) | q8::to_e4m3x2((x[2] - a1.x) * 32.f, (x[3] - a1.y) * 32.f) << 16;
-                    }
-#pragma unroll
-                    for (int i = 0; i < PER / 4; ++i) {
-                        *reinterpret_cast<uint32_t*>(line + r * 128 + ((piece ^ (r & 7)) << 4) + in + 4 * i) = one[i];
-                        *reinterpret_cast<uint32_t*>(line + (NR + r) * 128 + ((piece ^ ((NR + r) & 7)) << 4) + in + 4 * i) = two[i];
+                        *reinterpret_cast<uint32_t*>(line + r * 128 + ((piece ^ (r & 7)) << 4) + in + 4 * k) = lo | hi << 16;
+                        *reinterpret_cast<uint32_t*>(line + (NR + r) * 128 + ((piece ^ ((NR + r) & 7)) << 4) + in + 4 * k) =
+                            q8::to_e4m3x2((x[0] - a0.x) * 32.f, (x[1] - a0.y) * 32.f) | q8::to_e4m3x2((x[2] - a1.x) * 32.f, (x[3] - a1.y) * 32.f) << 16;
                     }
                 } else {
 #pragma unroll
-                    for (int i = 0; i < PER; i += 4)
-                        *reinterpret_cast<uint2*>(line + r * 128 + ((piece ^ (r & 7)) << 4) + in + 2 * i) = make_uint2(pack_bf16x2(q[i], q[i + 1]), pack_bf16x2(q[i + 2], q[i + 3]));
+                    for (int k = 0; k < PER / 4; ++k) *reinterpret_cast<uint2*>(line + r * 128 + ((piece ^ (r & 7)) << 4) + in + 8 * k) = r < rows ? q_raw[i][k] : make_uint2(0, 0);
                 }
-                if (r < NR && lane == 0) {
+                if (lane == 0) {
                     const int pos = s.start + t;
                     row_f[r] = f;
                     row_slope[r] = a.slopes && r < rows ? a.slopes[h] * kLog2e : 0.f;
                     row_pos[r] = pos;
                     row_limit[r] = a.causal ? max(pos, s.prefix - 1) : 0x7fffffff;
+                    row_number[r] = h * a.tokens + t;
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -254,18 +262,25 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
         const float* ks = a.k_scale + (size_t)e * (Q8 ? a.keys / a.block : 0) * a.kv_heads + kv;
         const float* vs = a.v_scale + (size_t)e * (Q8 ? a.keys / a.block : 0) * a.kv_heads + kv;
         const int shift = Q8 ? 31 - __clz(a.block) : 0;                        // blocks are powers of two
+        // a key's scales and position, fetched a block ahead
+        float next_k = 1.f, next_v = 1.f;
+        int next_pos = 0;
+        auto fetch = [&](int n) {
+            const int j = min((first + n) * BKEY + key, a.keys - 1);
+            if (Q8) {
+                next_k = __ldg(ks + (size_t)(j >> shift) * a.kv_heads);
+                next_v = __ldg(vs + (size_t)(j >> shift) * a.kv_heads);
+            }
+            if (a.k_pos) next_pos = __ldg(a.k_pos + (size_t)e * a.keys + j);
+        };
+        if (count > 0) fetch(0);
+        float* scores = p.scores + (size_t)e * a.heads * a.tokens * p.pitch;
         for (int n = 0; n < count; ++n) {
             const int b = n & 1, j = (first + n) * BKEY + key;
             const bool inside = j < s.L;
-            float kf = 1.f, lv = 0.f, iv = 1.f;                                // K's scale; log2 of V's and its inverse
-            if (Q8) {
-                const size_t at = (size_t)(min(j, a.keys - 1) >> shift) * a.kv_heads;
-                kf = __ldg(ks + at);
-                const float x = __ldg(vs + at);
-                lv = q8::log2_of_scale(x);
-                iv = __frcp_rn(x);
-            }
-            const int kp = a.k_pos ? __ldg(a.k_pos + (size_t)e * a.keys + min(j, a.keys - 1)) : j;
+            const float kf = next_k, lv = Q8 ? q8::log2_of_scale(next_v) : 0.f, iv = Q8 ? __frcp_rn(next_v) : 1.f;      // K's scale; log2 of V's and its inverse
+            const int kp = a.k_pos ? next_pos : j;
+            if (n + 1 < count) fetch(n + 1);
             ok = ok && mbar_wait(s_full(b), (uint32_t)((n >> 1) & 1), abort_flag);
             __syncwarp();
             tc5::tc_fence_after();
@@ -295,10 +310,7 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
             if (Q8 && p.scores != nullptr) {
 #pragma unroll
                 for (int r = 0; r < NR; ++r)
-                    if (r < rows) {
-                        const int t = r / group;
-                        p.scores[(((size_t)e * a.heads + kv * group + r - t * group) * a.tokens + t) * p.pitch + j] = v[r];
-                    }
+                    if (r < rows) scores[(size_t)row_number[r] * p.pitch + j] = v[r];
             }
             float mine = -INFINITY;
 #pragma unroll
@@ -433,28 +445,28 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
             const int group = p.group, rows = s.n * group, me = tid - 64;
             for (int i = split * 128 + me; i < rows * HDP; i += p.splits * 128) {
                 const int r = i / HDP, d = i % HDP;
-                float2 ml[8];
-                float top = -INFINITY, sum = 0.f, x = 0.f;
+                // all that the CTAs have of it at once; what a share that held nothing has left is dropped
+                float2 ml[CLUSTER];
+                float y[CLUSTER], top = -INFINITY, sum = 0.f, x = 0.f;
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
+                for (int c = 0; c < CLUSTER; ++c) {
                     ml[c] = make_float2(-INFINITY, 0.f);
                     if (c < p.splits) {
                         uint32_t at;
                         asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(base + C::OFF_F + r * 8), "r"(c));
                         asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(ml[c].x), "=f"(ml[c].y) : "r"(at) : "memory");
+                        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(base + C::OFF_T + i * 4), "r"(c));
+                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(y[c]) : "r"(at) : "memory");
                     }
-                    if (ml[c].y != 0.f) top = fmaxf(top, ml[c].x);
                 }
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    if (ml[c].y == 0.f) continue;                                       // this share held nothing that the row sees
-                    uint32_t at;
-                    float y;
-                    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(base + C::OFF_T + i * 4), "r"(c));
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(y) : "r"(at) : "memory");
-                    const float w = fast_exp2(ml[c].x - top);
+                for (int c = 0; c < CLUSTER; ++c)
+                    if (ml[c].y != 0.f) top = fmaxf(top, ml[c].x);
+#pragma unroll
+                for (int c = 0; c < CLUSTER; ++c) {
+                    const float w = ml[c].y == 0.f ? 0.f : fast_exp2(ml[c].x - top);
                     sum = fmaf(ml[c].y, w, sum);
-                    x = fmaf(y, w, x);
+                    x = ml[c].y == 0.f ? x : fmaf(y[c], w, x);
                 }
                 const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);
                 const int t = r / group, h = kv * group + r - t * group;

@@ -318,7 +318,6 @@ inline bool takes_few(const Args& a) { return (long long)a.tokens * (a.heads / a
 // Head dimension that the kernel is built for.
 inline int padded_dim(const Args& a) { return a.dim <= 64 && !takes_few(a) && a.k_scale == nullptr ? 64 : (a.dim <= 128 ? 128 : 256); }
 
-constexpr int CLUSTER = 8;      // shares that a cluster puts together
 // Shares of the key blocks: as many as bring the CTAs up to the number that are resident, at most one per block.
 inline int plan_splits(const Args& a) {
     const int group = a.heads / a.kv_heads, tile_tokens = BQ / group, blocks = (a.keys + BKEY - 1) / BKEY;

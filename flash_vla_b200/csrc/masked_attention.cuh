@@ -329,7 +329,10 @@ inline int plan_splits(const Args& a) {
         per_sm = few_rows(a) == 32 ? (tile_bytes == 16384 ? 2 : 1) : (tile_bytes == 16384 ? 3 : (tile_bytes == 32768 ? 2 : 1));
     }
     const long long room = (long long)tc5::num_sms() * per_sm * (few && tiles > tc5::num_sms() ? 2 : 1) / tiles;
-    if (few && room > CLUSTER && blocks <= 2 * CLUSTER) return blocks < CLUSTER ? (blocks > 0 ? blocks : 1) : CLUSTER;      // no second launch for two blocks each
+    // A cluster rather than a second launch that joins the shares, up to four blocks for each of its CTAs. (8 heads of 256 over 32 blocks of the 8-bit cache, eight shares
+    // in a cluster / as many as are resident: eight episodes 11.4 / 14.3 us, one 11.2 / 10.7; over 64 blocks 17.6 / 15.8 and 16.3 / 11.6. bf16, 32 blocks: eight episodes 14.0 / 15.3,
+    // two 12.2 / 11.6.)
+    if (few && room > CLUSTER && blocks <= 4 * CLUSTER) return blocks < CLUSTER ? (blocks > 0 ? blocks : 1) : CLUSTER;
     return (int)(room < 1 ? 1 : (room < blocks ? room : (blocks > 0 ? blocks : 1)));
 }
 inline size_t score_pitch(const Args& a) { return ((size_t)a.keys + BKEY - 1) / BKEY * BKEY; }
@@ -360,7 +363,7 @@ inline int launch_join(const Tile& p, int hdp, cudaStream_t st) {
 }
 
 template <int HDP, bool Q8>
-inline int launch_tile(const Tile& p, const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV, cudaStream_t st) {
+inline int launch_tile(const Tile& p, const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV, const CUtensorMap& tmO, cudaStream_t st) {
     using C = TileCfg<HDP, Q8>;
     auto kern = attention_tile_kernel<HDP, Q8>;
     static PerDeviceFlag configured;
@@ -370,7 +373,7 @@ inline int launch_tile(const Tile& p, const CUtensorMap& tmQ, const CUtensorMap&
         configured.set();
     }
     const Args& a = p.a;
-    cudaError_t e = launch_pdl(kern, dim3((unsigned)(p.tiles * p.splits * a.kv_heads * a.episodes)), dim3(C::THREADS), C::SMEM, st, p, tmQ, tmK, tmV);
+    cudaError_t e = launch_pdl(kern, dim3((unsigned)(p.tiles * p.splits * a.kv_heads * a.episodes)), dim3(C::THREADS), C::SMEM, st, p, tmQ, tmK, tmV, tmO);
     if (e != cudaSuccess) { set_error("attention_tile_kernel: %s", cudaGetErrorString(e)); return FVLA_ERR_LAUNCH; }
     int rc = check_launch("attention_tile_kernel");
     return rc || p.splits == 1 ? rc : launch_join(p, HDP, st);
@@ -410,7 +413,7 @@ inline int launch_attention(const Args& a, void* ws, int* status, cudaStream_t s
     }
     p.part_ml = reinterpret_cast<float2*>(at);
     p.part_o = reinterpret_cast<float*>(at + align256(p.splits * rows * sizeof(float2)));
-    CUtensorMap tmQ = {}, tmK = {}, tmV = {};
+    CUtensorMap tmQ = {}, tmK = {}, tmV = {}, tmO = {};
     const bool few = takes_few(a), q8 = a.k_scale != nullptr;
     p.q_mul[0] = 1;
     p.q_mul[1] = a.qs[0] != 0;
@@ -418,7 +421,11 @@ inline int launch_attention(const Args& a, void* ws, int* status, cudaStream_t s
         const uint64_t dims[5] = {(uint64_t)a.dim, (uint64_t)p.group, (uint64_t)a.tokens, (uint64_t)a.kv_heads, p.q_mul[1] ? (uint64_t)a.episodes : 1};
         const uint64_t strides[4] = {(uint64_t)a.qs[2], (uint64_t)a.qs[1], (uint64_t)a.qs[2] * p.group, p.q_mul[1] ? (uint64_t)a.qs[0] : 256};
         const uint32_t box[5] = {64, (uint32_t)p.group, (uint32_t)p.tile_tokens, 1, 1};
-        const int rc = make_map(&tmQ, a.q, 5, dims, strides, box);
+        int rc = make_map(&tmQ, a.q, 5, dims, strides, box);
+        if (rc) return rc;
+        const uint64_t out_dims[5] = {dims[0], dims[1], dims[2], dims[3], (uint64_t)a.episodes};
+        const uint64_t out_strides[4] = {(uint64_t)a.os[2], (uint64_t)a.os[1], (uint64_t)a.os[2] * p.group, (uint64_t)a.os[0]};
+        if (p.splits == 1) rc = make_map(&tmO, a.out, 5, out_dims, out_strides, box);
         if (rc) return rc;
     }
     p.k_mul[0] = a.ks[2] != 0; p.k_mul[1] = a.ks[0] != 0; p.v_mul[0] = a.vs[2] != 0; p.v_mul[1] = a.vs[0] != 0;
@@ -439,9 +446,9 @@ inline int launch_attention(const Args& a, void* ws, int* status, cudaStream_t s
         else rc = hdp == 128 ? launch_few<128, false>(p, tmK, tmV, st) : launch_few<256, false>(p, tmK, tmV, st);
         if (!rc && !p.cluster) rc = launch_join(p, hdp, st);
     } else if (q8) {
-        rc = hdp == 128 ? launch_tile<128, true>(p, tmQ, tmK, tmV, st) : launch_tile<256, true>(p, tmQ, tmK, tmV, st);
+        rc = hdp == 128 ? launch_tile<128, true>(p, tmQ, tmK, tmV, tmO, st) : launch_tile<256, true>(p, tmQ, tmK, tmV, tmO, st);
     } else {
-        rc = hdp == 64 ? launch_tile<64, false>(p, tmQ, tmK, tmV, st) : (hdp == 128 ? launch_tile<128, false>(p, tmQ, tmK, tmV, st) : launch_tile<256, false>(p, tmQ, tmK, tmV, st));
+        rc = hdp == 64 ? launch_tile<64, false>(p, tmQ, tmK, tmV, tmO, st) : (hdp == 128 ? launch_tile<128, false>(p, tmQ, tmK, tmV, tmO, st) : launch_tile<256, false>(p, tmQ, tmK, tmV, tmO, st));
     }
     if (rc || a.weights == nullptr || a.keys == 0) return rc;
     cudaError_t e;

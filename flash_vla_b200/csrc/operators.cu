@@ -40,6 +40,8 @@ static int check_attention(const struct fvla_attention* a) {
                  "attention: every row must start on 16 bytes");
     FVLA_REQUIRE((a->tokens == 1 || a->q_stride[1] > 0) && (a->heads == 1 || a->q_stride[2] > 0) && (a->keys <= 1 || (a->k_stride[1] > 0 && a->v_stride[1] > 0)),
                  "attention: tokens or query heads that share their memory");
+    FVLA_REQUIRE((a->episodes == 1 || a->out_stride[0] > 0) && (a->tokens == 1 || a->out_stride[1] > 0) && (a->heads == 1 || a->out_stride[2] > 0),
+                 "attention: rows of the result that share their memory");
     for (int i = 0; i < 3; ++i) FVLA_REQUIRE(a->q_stride[i] >= 0 && a->k_stride[i] >= 0 && a->v_stride[i] >= 0 && a->out_stride[i] >= 0, "attention: negative strides");
     FVLA_REQUIRE(!q8 || (block_ok(a->block) && a->keys % a->block == 0), "attention: blocks of %d rows in %d", a->block, a->keys);
     FVLA_REQUIRE((a->q_docs != nullptr) == (a->k_docs != nullptr), "attention: documents of queries and keys, or of neither");

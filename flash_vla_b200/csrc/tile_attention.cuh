@@ -120,7 +120,7 @@ struct TileCfg {
 template <int HDP, bool Q8>
 __global__ void __launch_bounds__(TileCfg<HDP, Q8>::THREADS, 1)
 attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                      const __grid_constant__ CUtensorMap tmV) {
+                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO) {
     using C = TileCfg<HDP, Q8>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -653,6 +653,9 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
             const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);             // NaN stays
             if (store && g == 0 && a.lse)
                 a.lse[((size_t)e * a.heads + h) * a.tokens + t0 + t] = l > 0.f ? (m_end + log2f(l)) * 0.6931471805599453f : (l == 0.f ? -INFINITY : l);
+            // Q's buffer takes the results in Q's layout, and the TMA stores them: all rows of the box, or all that the tensor has. A tile that ends at its
+            // episode's last query is stored by its threads (for four prefixes of 8 x 256, 37.1 us if all are).
+            const bool whole = tokens == p.tile_tokens || t0 + tokens == a.tokens;
             bf16* dst = a.out + e * a.os[0] + (t0 + (mine ? t : 0)) * a.os[1] + h * a.os[2];
 #pragma unroll 1
             for (int c = 0; c < (busy ? SPAN : 0); c += 32) {
@@ -661,14 +664,26 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                 if (any) tc5::tmem_ld32(tmem + t_lane + C::O_COL + col, o);
 #pragma unroll
                 for (int k = 0; k < 32; ++k) o[k] = any ? o[k] * inv : 0.f;
-                if (store) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (col + k * 8 < a.dim)
-                            *reinterpret_cast<uint4*>(dst + col + k * 8) = make_uint4(pack_bf16x2(o[8 * k], o[8 * k + 1]), pack_bf16x2(o[8 * k + 2], o[8 * k + 3]),
-                                                                                    pack_bf16x2(o[8 * k + 4], o[8 * k + 5]), pack_bf16x2(o[8 * k + 6], o[8 * k + 7]));
+                for (int k = 0; k < 4; ++k) {
+                    const uint4 u = make_uint4(pack_bf16x2(o[8 * k], o[8 * k + 1]), pack_bf16x2(o[8 * k + 2], o[8 * k + 3]), pack_bf16x2(o[8 * k + 4], o[8 * k + 5]),
+                                               pack_bf16x2(o[8 * k + 6], o[8 * k + 7]));
+                    const int piece = (col >> 3) + k;
+                    if (whole) *reinterpret_cast<uint4*>(gen + C::OFF_Q + (piece >> 3) * 16384 + row * 128 + (((piece & 7) ^ (row & 7)) << 4)) = u;
+                    else if (store && piece * 8 < a.dim) *reinterpret_cast<uint4*>(dst + piece * 8) = u;
                 }
                 __syncwarp();
+            }
+            if (whole && tokens > 0) {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                asm volatile("bar.sync 9, 256;" ::: "memory");
+                if (tid == 32 * SOFTMAX0 && ok) {
+#pragma unroll 1
+                    for (int c = 0; c * 64 < a.dim; ++c)
+                        asm volatile("cp.async.bulk.tensor.5d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5, %6}], [%1];"
+                                     ::"l"(reinterpret_cast<uint64_t>(&tmO)), "r"(sQ + c * 16384), "r"(c * 64), "r"(0), "r"(t0), "r"(kv), "r"(e) : "memory");
+                    asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group 0;" ::: "memory");
+                }
             }
         } else {
             // Sums of a share, 32 bits wide, by way of the rings, which are idle now: a thread leaves its half of a row there (pieces of 16 bytes, exchanged

@@ -151,14 +151,14 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) attention_join_kernel(const _
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const Args& a = p.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % warps, col0 = blockIdx.y * 32 * PER + lane;
-    const long long row = (long long)blockIdx.x * (JOIN_WARPS / warps) + warp / warps, rows = (long long)a.episodes * a.tokens * a.heads;
-    const int h = (int)(row % a.heads), t = (int)(row / a.heads % a.tokens), e = (int)min(row / a.heads / a.tokens, (long long)a.episodes - 1);
+    const int row = blockIdx.x * (JOIN_WARPS / warps) + warp / warps, rows = a.episodes * a.tokens * a.heads;      // (below 2^31: checked on the host)
+    const int h = row % a.heads, t = row / a.heads % a.tokens, e = min(row / a.heads / a.tokens, a.episodes - 1);
     const bool mine = row < rows && t < episode_of(a, e).n;
     // no load waits for another, but for the maxima: shares that held nothing are read as well, and dropped
     float m = -INFINITY;
 #pragma unroll 4
     for (int s = lane; s < p.splits; s += 32) {
-        const float2 ml = mine ? p.part_ml[s * rows + row] : make_float2(0.f, 0.f);
+        const float2 ml = mine ? p.part_ml[(size_t)s * rows + row] : make_float2(0.f, 0.f);
         if (ml.y != 0.f) m = fmaxf(m, ml.x);
     }
     m = warp_max(m);
@@ -166,12 +166,12 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) attention_join_kernel(const _
     float acc[PER], l = 0.f;                                                         // columns lane, lane + 32, ...
 #pragma unroll
     for (int c = 0; c < PER; ++c) acc[c] = 0.f;
-    const float* o = p.part_o + (mine ? row : 0) * hdp + col0;
+    const float* o = p.part_o + (size_t)(mine ? row : 0) * hdp + col0;
     const size_t pitch = (size_t)rows * hdp;
     for (int s0 = part; s0 < p.splits; s0 += 32 * warps) {
         // lane i: the factor of share s0 + i * warps
         const int s = s0 + lane * warps;
-        const float2 ml = mine && s < p.splits ? p.part_ml[s * rows + row] : make_float2(0.f, 0.f);
+        const float2 ml = mine && s < p.splits ? p.part_ml[(size_t)s * rows + row] : make_float2(0.f, 0.f);
         const float w = ml.y == 0.f ? 0.f : (ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - top));
         l += warp_sum(ml.y == 0.f ? 0.f : ml.y * w);
         const int have = min(32, (p.splits - s0 + warps - 1) / warps);
@@ -355,7 +355,7 @@ inline size_t workspace_bytes(const Args& a) {
 inline int launch_join(const Tile& p, int hdp, cudaStream_t st) {
     const long long rows = (long long)p.a.episodes * p.a.tokens * p.a.heads;
     // many shares: eight warps for 32 columns of a row; few: a warp or some for the whole row
-    const int warps = p.splits >= 16 ? 8 : (p.splits >= 8 ? 4 : (p.splits >= 4 ? 2 : 1)), each = JOIN_WARPS / warps, per = p.splits >= 16 ? 1 : hdp / 32;
+    const int warps = p.splits >= 16 ? 8 : (p.splits >= 8 ? 4 : 1), each = JOIN_WARPS / warps, per = p.splits >= 16 ? 1 : hdp / 32;
     const auto kern = per == 1 ? attention_join_kernel<1> : (per == 2 ? attention_join_kernel<2> : (per == 4 ? attention_join_kernel<4> : attention_join_kernel<8>));
     const cudaError_t e = launch_pdl(kern, dim3((unsigned)((rows + each - 1) / each), hdp / (32 * per)), dim3(32 * JOIN_WARPS), 0, st, p, hdp, warps);
     if (e != cudaSuccess) { set_error("attention_join_kernel: %s", cudaGetErrorString(e)); return FVLA_ERR_LAUNCH; }

@@ -113,7 +113,7 @@ def _attention_plan(q, k, v, out, cache):
         raise ValueError(f"attention: head_dim {D} (a multiple of {dim_multiple} up to 256)")
     if HK == 0 or H % HK or not 0 < H // HK <= 128:
         raise ValueError(f"attention: {H} query heads over {HK} K/V heads")
-    if T * H >= 1 << 31 or E * HK >= 1 << 16 or S >= 1 << 31 or E >= 1 << 16:
+    if E * T * H >= 1 << 31 or E * HK >= 1 << 16 or S >= 1 << 31 or E >= 1 << 16:
         raise ValueError(f"attention: {E} episodes of {T} queries of {H} heads over {S} keys: too many")
     a.episodes, a.tokens, a.keys, a.heads, a.kv_heads, a.head_dim = E, T, S, H, HK, D
     nbytes = [0, 0]

@@ -20,7 +20,7 @@ STAMP = ROOT / "libfvla_b200.so.stamp"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-    "--shared", "-Xcompiler", "-fPIC", "-Xptxas", "-v",
+    "--shared", "-Xcompiler", "-fPIC", "-Xptxas", "-v", "--threads", "2",
 ]
 
 

@@ -1,4 +1,7 @@
-// Attention of few rows: a decoding step of at most 32 rows (tokens x the query heads of a K/V head), bound by the bytes of the cache.
+// Attention of few rows: a decoding step of at most 32 rows (tokens x the query heads of a K/V head), bound by the bytes of the cache: 32 episodes of
+// up to 16 384 rows of 8 heads of 128, 805 MB, in 130 us, 0.95 of the measured copy rate (144 us at the clocks of a long run); with the cache converted
+// to fp16 operands by warps of their own 730 us. One token over 819 rows is a chain of latencies, 8 us: lengths, Q, the tiles' first bytes, two products,
+// the cluster's exchange.
 //
 // The keys are the 128-row operand of both products, so that every thread of the softmax has one key and all rows of it:
 //   S^T (128 keys x rows) = K Q^T,      O^T (128 dims x rows, one or two halves) += V^T P^T

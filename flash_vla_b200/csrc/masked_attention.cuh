@@ -4,6 +4,10 @@
 //
 // The query of token t of an episode with n queries and L keys stands at p = q_start + t (L - n + t when none is given), key j at kp = j or k_pos[j].
 // Visible: j < L, with `causal` kp <= max(p, prefix - 1), with documents equal ids that are not negative. A query without a visible key gets zeros.
+//
+// Two kernels: tile_attention.cuh (128 rows of tokens x heads against 128 keys at a time; bound by the softmax's instructions, or at head dim 256 by
+// how fast keys and values arrive) and few_rows_attention.cuh (up to 32 rows; bound by the bytes of the cache, or where there are few by a chain of
+// latencies). Here: what both are given, masks and scores, the join of keys shared out over CTAs, the weights of keys, and the choice between them.
 #pragma once
 
 #include "common.cuh"
@@ -124,7 +128,7 @@ __device__ __forceinline__ void ld32_nowait(uint32_t taddr, uint32_t* r) {
         : "r"(taddr) : "memory");
 }
 // What a CTA's rows may see, block by block. Every role evaluates it from the same memory. The last block comes first: where scores fall with distance
-// the maximum is found at once, and nothing is rescaled (every block otherwise: 241 us against 180 at head dim 128, 4 096 causal keys, 32 heads).
+// the maximum is found at once, and nothing is rescaled (every block otherwise: 241 us against 178 at head dim 128, 4 096 causal keys, 32 heads).
 struct Walk {
     int first, count;                 // key blocks of this CTA (of its split), some of which may hold nothing that is seen
     int q_low, q_high;                // documents of the tile's queries

@@ -3,11 +3,14 @@
 //   warps 0, 3  TMA: the Q tile and K, and V, each in granules of 16 KB through a ring (K: 128 bytes of the head dimension of 128 keys; V: some
 //               keys, whole): what is in flight is then limited by shared memory alone, not by tile sizes
 //   warps 1, 2  one lane of each issues S = Q K^T into one of BUFFERS TMEM score buffers, and O += P V (TMEM). (An issue takes 50 to 100 clocks with
-//               its waits; one lane for both was the bottleneck, 2 070 clocks a block at head dim 128.)
+//               its waits; one lane for both was the bottleneck at head dim 128: 301 us against 281.)
 //   warps 4-11  softmax: two groups of 128 threads, thread = row, which take the blocks in turn. P goes back to TMEM over the scores, as the A operand
 //               of P V, so that nothing crosses shared memory. All that one block needs from the one before is the running maximum: the other group
 //               hands it on (per warp, 32 rows) before it begins its exponentials, and those of one block run beside the other's
 //               loads and maxima. The accumulator is rescaled only where the maximum has grown by more than a threshold.
+// 4 096 keys, 32 query heads of 128 or 16 of 256 with two to a K/V head: 270 us (1 018 TFLOP/s) and 112 us (1 231 TFLOP/s). A block of 128 keys takes 2 200 to
+// 2 500 clocks: at head dim 128 the softmax's instructions (128 exponentials of a row at 16 clocks a warp among them), at 256 the arrival of 128 KB of
+// keys and values through 128 KB of rings. A CTA's two ends, 7 000 and 5 000 clocks, are the rest of short walks.
 // The 8-bit cache runs in 8 bits (kind::f8f6f4), its values straight from TMA: a bf16 row of Q, brought to 2^7..2^8 by its own power of two, is the sum
 // of an e4m3 term and an e5m2 term (what rounding to 4 bits leaves of 8 has at most 3; below 2^-16, 2^-23 of the largest, is lost), a probability the sum
 // of two e4m3 terms and an e5m2 term (11 bits; the last holds what is below e4m3's range). Probabilities stand against the running maximum at 2^6

@@ -309,11 +309,12 @@ int fvla_embed_rows(const void* table, const long long* ids, void* out, int rows
  *
  * Token t of an episode stands at p = q_start[e] + t, or k_lens[e] - q_lens[e] + t; key j at kp = k_pos[e][j], or j. A query sees key
  * j < k_lens[e]; with `causal` only where kp <= max(p, prefix[e] - 1); with documents only where q_docs[e][t] == k_docs[e][j] >= 0. A query that
- * sees nothing gets zeros and a log-sum-exp of -infinity; rows behind q_lens[e] stay as they were. With k_scale / v_scale (fp32 powers of two,
+ * sees nothing gets zeros and a log-sum-exp of -infinity; rows behind q_lens[e] stay as they were. With k_scale / v_scale (fp32, positive,
  * (episodes, keys / block, kv_heads) contiguous; block 16, 32, 64 or 128) k and v hold e4m3 values, else bf16. lse: (episodes, heads,
  * tokens) fp32. weights: (episodes, keys) fp32, weights[e][j] = decay * weights[e][j] + the probabilities that key j < k_lens[e] got from all queries;
- * needs lse and the 8-bit cache, and 4 bytes of ws for every score. What a query does not see may hold any bits, infinities and NaN among them, where no query of its 128-row tile sees it: rows behind
- * k_lens, and rows of a negative document. head_dim: a multiple of 8 (e4m3: 16) up to 256; up to 128 query heads per K/V head. */
+ * needs lse and the 8-bit cache, and 4 bytes of ws for every score. Rows of k and v behind k_lens, and rows of a negative document, may hold any bits. All
+ * others have to be finite: a value of v that is not can reach every query that is processed beside one that sees it. ws:
+ * fvla_attention_workspace_bytes of these arguments, any contents, not shared by calls that may run at the same time. out may be q, unless weights are asked for. head_dim: a multiple of 8 (e4m3: 16) up to 256; up to 128 query heads per K/V head. */
 struct fvla_attention {
     const void *q, *k, *v, *k_scale, *v_scale;
     void *out, *lse, *weights, *ws;

@@ -134,7 +134,7 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
     const int first = (int)((long long)blocks * split / p.splits), count = (int)((long long)blocks * (split + 1) / p.splits) - first;
 
     if (warp == 0) {
-        if (lane == 0) {
+        if (lane == 0 && count > 0) {
             tc5::prefetch_tensormap(&tmK);
             tc5::prefetch_tensormap(&tmV);
             for (int i = 0; i < 2 * count; ++i) {

@@ -193,6 +193,8 @@ def _attend(Q, K, V, cache, scale, out, causal, prefix, q_lens, k_lens, q_start,
     q, k, v, o = _address("Q", Q, device), _address("K", K, device), _address("V", V, device), _address("out", out, device)
     if E == 0 or T == 0:
         return out
+    if S == 0:                                  # no key: documents of none have no address
+        q_docs = k_docs = 0
     if weights and o == q:
         raise ValueError("attention: the weights are taken from Q, which out would overwrite")
     if weights and not lse:

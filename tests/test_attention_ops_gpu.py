@@ -19,6 +19,14 @@ NAN, INF = math.nan, math.inf
 P_BF16, P_FP16 = 2.0 ** -8, 2.0 ** -11      # half a step of the probabilities' type
 
 
+@pytest.fixture(autouse=True)
+def no_wait_has_run_out():
+    """A kernel that gives up on a wait leaves a code in the device's health word."""
+    yield
+    torch.cuda.synchronize()
+    assert _lib.load().fvla_device_status(None) == 0
+
+
 def randn(seed, *shape, dtype=bf16):
     return torch.randn(shape, device="cuda", generator=torch.Generator("cuda").manual_seed(seed)).to(dtype)
 
@@ -106,6 +114,13 @@ def test_documents_in_any_order(D, H, HK, causal):
     assert (out == 0).all() and (lse == -INF).all()
 
 
+def test_no_keys_and_documents():
+    Q, K = randn(7, 2, 3, 4, 64), randn(8, 2, 0, 2, 64)
+    ids = torch.zeros(2, 3, dtype=i32, device="cuda")
+    out, lse = attend(Q, K, K, 0.1, q_docs=ids, k_docs=ids[:, :0].contiguous())
+    assert (out == 0).all() and (lse == -INF).all()
+
+
 def test_prefix_mask():
     E, T, S, H, D = 4, 200, 300, 8, 256
     Q, K, V = randn(10, E, T, H, D), randn(11, E, S, 1, D), randn(12, E, S, 1, D)
@@ -149,6 +164,18 @@ def test_large_and_growing_scores(D):
 def test_caps(cap):
     Q, K, V = randn(21, 1, 130, 4, 128) * 3, randn(22, 1, 260, 2, 128) * 3, randn(23, 1, 260, 2, 128)
     check(Q, K, V, 0.5, cap=cap)
+
+
+@pytest.mark.parametrize("H,HK,D", [(8, 4, 256), (4, 4, 128), (4, 2, 64)])
+def test_long_walks(H, HK, D):
+    """Thirty blocks and more to a tile, the last tile almost empty, with every score function; results repeat to the bit."""
+    T = S = 4099
+    Q, K, V = randn(63, 1, T, H, D), randn(64, 1, S, HK, D), randn(65, 1, S, HK, D)
+    for kw in ({}, {"causal": True}, {"causal": True, "cap": 20.0}, {"causal": True, "slopes": slopes_of(H)}):
+        outs = [attend(Q, K, V, D ** -0.5, **kw)[0] for _ in range(4)]
+        assert all(torch.equal(o, outs[0]) for o in outs[1:])
+        want = A.attention(Q, K, V, D ** -0.5, **kw)
+        A.check_out(outs[0], want, D, P_BF16)
 
 
 def test_a_row_of_nan_stays_in_its_row():
@@ -383,9 +410,10 @@ def test_cache_rows_far_apart():
     assert torch.equal(A.widened(small.V, small.V_scale), A.widened(cache.V.contiguous(), cache.V_scale)[:, rows - 200:rows - 200 + keep])
 
 
+@pytest.mark.parametrize("T", [5, 20])
 @pytest.mark.parametrize("positions", ["evicted", "shuffled"])
-def test_cache_attention_with_positions(positions):
-    E, T, rows, H, HK, D = 2, 5, 384, 8, 2, 64
+def test_cache_attention_with_positions(positions, T):
+    E, rows, H, HK, D = 2, 384, 8, 2, 64
     cache, _, _ = filled(27, E, rows, HK, D)
     gen = torch.Generator("cuda").manual_seed(3)
     k_pos = torch.stack([torch.randperm(2000, device="cuda", generator=gen)[:rows] for _ in range(E)]).to(i32)
@@ -462,6 +490,42 @@ def test_evict_refuses_its_own_memory():
         op_table().cache_evict(cache, n, w, 64, cache, A.ints([0]))
     with pytest.raises(ValueError, match="lies over"):
         op_table().cache_evict(cache, n, w, 64, allocate_quantized_cache(1, 128, 1, 64, "cuda"), n)
+
+
+def test_a_captured_step_of_all_of_them():
+    """Append, attention with weights and eviction in one graph: replays on rewritten inputs give what the calls themselves give."""
+    E, rows, H, HK, D, keep = 2, 256, 8, 2, 128, 64
+    ops = op_table()
+
+    def state(seed):
+        cache, _, _ = filled(seed, E, rows, HK, D)
+        return {"cache": cache, "q": randn(seed, E, 2, H, D), "k": randn(seed + 1, E, 2, HK, D), "v": randn(seed + 2, E, 2, HK, D), "n": A.ints([200, 111]),
+                "out": torch.zeros(E, 2, H, D, dtype=bf16, device="cuda"), "w": torch.rand(E, rows, device="cuda", generator=torch.Generator("cuda").manual_seed(seed)),
+                "small": allocate_quantized_cache(E, keep, HK, D, "cuda"), "m": A.ints([0, 0]), "pos": torch.zeros(E, keep, dtype=i32, device="cuda")}
+
+    def step(s):
+        ops.cache_append(s["k"], s["v"], s["cache"], s["n"])
+        ops.cache_attention(s["q"], s["cache"], s["n"] + 2, 0.08, s["out"], causal=True, weights=s["w"], decay=0.5)
+        ops.cache_evict(s["cache"], s["n"] + 2, s["w"], keep, s["small"], s["m"], out_positions=s["pos"], sinks=1, recent=4)
+
+    held = state(200)
+    step(held)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step(held)
+    for seed in (300, 400):
+        fresh, same = state(seed), state(seed)
+        for name in ("q", "k", "v", "n", "w", "out", "m", "pos"):
+            held[name].copy_(same[name])
+        for name in ("cache", "small"):
+            for a, b in zip(held[name], same[name]):
+                a.view(torch.uint8).copy_(b.view(torch.uint8))
+        g.replay()
+        step(fresh)
+        for name in ("out", "w", "m", "pos"):
+            assert torch.equal(held[name], fresh[name]), name
+        for a, b in zip((*held["cache"], *held["small"]), (*fresh["cache"], *fresh["small"])):
+            assert A.same_bits(a, b)
 
 
 def test_a_server_uses_them_together():

@@ -38,20 +38,24 @@ def attention(Q, K, V, scale, causal=False, prefix=None, q_lens=None, k_lens=Non
     size = (q.abs() @ k.abs().mT * abs(scale)).masked_fill(~see[:, None], 0.0).amax(-1) if S else x.new_zeros(E, H, T)
     if cap:
         x = cap * torch.tanh(x / cap)
+    bias = 0.0
     if slopes is not None:
+        far = (pos[:, :, None] - kp[:, None, :]).abs().masked_fill(~see, 0).amax(-1) if S else pos * 0       # (E, T)
+        bias = slopes.double().abs()[None, :, None] * far[:, None, :]
         x = x - slopes.double()[None, :, None, None] * (pos[:, :, None] - kp[:, None, :]).abs()[:, None]
     x = x.masked_fill(~see[:, None], -math.inf)
     lse = torch.logsumexp(x, -1) if S else x.new_full((E, H, T), -math.inf)
     p = torch.where(see[:, None], torch.exp(x - torch.where(lse == -math.inf, 0.0, lse)[..., None]), 0.0)
     p = p * (torch.arange(T, device=dev) < n[:, None])[:, None, :, None]
     back = lambda y: y.permute(0, 2, 1, 3)                                                    # noqa: E731
-    return {"out": back(p @ v), "lse": lse, "p": p, "spread": back(p @ v.abs()), "size": size, "rows": torch.arange(T, device=dev) < n[:, None],
+    return {"out": back(p @ v), "lse": lse, "p": p, "spread": back(p @ v.abs()), "size": size, "bias": bias, "rows": torch.arange(T, device=dev) < n[:, None],
             "weights": p.sum((1, 2))}
 
 
 def score_error(want, D):
-    """Bound on a score's error in 32 bits: D products and sums of half a step each (2^-24), and cap, bias and exponential on top (2^-19)."""
-    return want["size"] * D * 2.0 ** -24 + 2.0 ** -19
+    """Bound on a score's error in 32 bits: D products and sums of half a step each (2^-24), cap and exponential on top (2^-19), and of the bias four half
+    steps: the slope in units of log2, its product with the distance, that product's sum with the score, and the maximum's subtraction."""
+    return want["size"] * D * 2.0 ** -24 + 2.0 ** -19 + want["bias"] * 2.0 ** -22
 
 
 def check_out(got, want, D, p_step):

@@ -215,15 +215,16 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) attention_join_kernel(const _
     if (a.lse && lane == 0 && blockIdx.y == 0) a.lse[((size_t)e * a.heads + h) * a.tokens + t] = l > 0.f ? (top + log2f(l)) * 0.6931471805599453f : (l == 0.f ? -INFINITY : l);
 }
 
-// weights[e][j] = decay * weights[e][j] + the probabilities that key j got, from the scores that the attention left and the rows' log-sum-exps. A CTA
-// has 32 keys; its warps share out the rows, and their sums are added in the order of the warps.
+// weights[e][j] = decay * weights[e][j] + the probabilities that key j got, from the scores that the attention left and the rows' log-sum-exps. `share`
+// warps have 32 keys together; they share out the rows, and their sums are added in the order of the warps.
 constexpr int WEIGHT_WARPS = 16;
-__global__ void __launch_bounds__(32 * WEIGHT_WARPS) key_weights_kernel(const __grid_constant__ Tile p) {
+__global__ void __launch_bounds__(32 * WEIGHT_WARPS) key_weights_kernel(const __grid_constant__ Tile p, int share) {
     __shared__ float part[WEIGHT_WARPS][32];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const Args& a = p.a;
-    const int e = blockIdx.y, j = blockIdx.x * 32 + (threadIdx.x & 31), warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const int e = blockIdx.y, lane = threadIdx.x & 31, all = blockDim.x >> 5, warp = (threadIdx.x >> 5) % share, warps = share;
+    const int j = (blockIdx.x * (all / share) + (threadIdx.x >> 5) / share) * 32 + lane;
     const Episode s = episode_of(a, e);
     const bool inside = j < s.L, by_number = a.causal && a.k_pos == nullptr;
     const int rows = a.heads * s.n;
@@ -240,16 +241,19 @@ __global__ void __launch_bounds__(32 * WEIGHT_WARPS) key_weights_kernel(const __
             const int r = min(r0 + k * warps, rows - 1), h = r / s.n, t = r - h * s.n;
             const size_t row = row0 + (size_t)h * a.tokens + t;
             z[k] = a.lse[row];
-            x[k] = p.scores[row * p.pitch + j];                                      // what was not left is read as well (j < pitch), and dropped
+            x[k] = p.scores[row * p.pitch + min((long long)j, p.pitch - 1)];         // what was not left is read as well, and dropped
             seen[k] = r0 + k * warps < rows && inside && t >= from;
         }
 #pragma unroll
         for (int k = 0; k < BATCH; ++k) sum += seen[k] && z[k] != -INFINITY ? fast_exp2(fmaf(z[k], -kLog2e, x[k])) : 0.f;
     }
-    part[warp][threadIdx.x & 31] = sum;
-    __syncthreads();
-    if (warp != 0 || !inside) return;
-    for (int w = 1; w < warps; ++w) sum += part[w][threadIdx.x];
+    if (warps > 1) {
+        part[threadIdx.x >> 5][lane] = sum;
+        __syncthreads();
+        if (warp != 0) return;
+        for (int w = 1; w < warps; ++w) sum += part[(threadIdx.x >> 5) + w][lane];
+    }
+    if (!inside) return;
     float* at = a.weights + (size_t)e * a.keys + j;
     *at = (a.decay != 0.f ? a.decay * *at : 0.f) + sum;
 }
@@ -457,8 +461,12 @@ inline int launch_attention(const Args& a, void* ws, int* status, cudaStream_t s
     if (rc || a.weights == nullptr || a.keys == 0) return rc;
     cudaError_t e;
     if (few) {
-        const int rows_each = a.tokens * a.heads, warps = rows_each < 4 * WEIGHT_WARPS ? (rows_each + 3) / 4 : WEIGHT_WARPS;      // four rows or more for a warp
-        e = launch_pdl(key_weights_kernel, dim3((a.keys + 31) / 32, a.episodes), dim3(32 * warps), 0, st, p);
+        // a warp for up to 16 rows, sixteen for the most: eight rows or more for each; CTAs of four warps at least
+        const int rows_each = a.tokens * a.heads;
+        int share = 1;
+        while (share < WEIGHT_WARPS && rows_each > 16 * share) share *= 2;
+        const int all = share < 4 ? 4 : share, keys_each = 32 * (all / share);
+        e = launch_pdl(key_weights_kernel, dim3((a.keys + keys_each - 1) / keys_each, a.episodes), dim3(32 * all), 0, st, p, share);
     } else {
         e = launch_pdl(tile_weights_kernel, dim3(2 * blocks, a.episodes), dim3(32 * WEIGHT_WARPS), 0, st, p);
     }

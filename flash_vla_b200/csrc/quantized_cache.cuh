@@ -225,6 +225,9 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const __gr
     const int wanted = n - low - (L - high);                              // and so many of them stay (sinks + recent <= keep)
     const int run = ((L + ctas * WARPS - 1) / (ctas * WARPS) + 31) / 32 * 32, begin = (int)min((long long)(rank * WARPS + warp) * run, (long long)L), end = min(begin + run, L);
     const bool choose = L > p.keep;
+    // a run of at most 64 rows stays in registers: two rows a lane
+    const float held0 = begin + lane < end ? w[begin + lane] : 0.f, held1 = begin + 32 + lane < end ? w[begin + 32 + lane] : 0.f;
+    auto weight = [&](int j0) { return j0 == begin ? held0 : (j0 == begin + 32 ? held1 : (j0 + lane < end ? w[j0 + lane] : 0.f)); };
     uint32_t threshold = 0xffffffffu, ties = 0;                           // nothing lies above the largest order
     if (choose && wanted > 0) {
         uint32_t prefix = 0, left = wanted;
@@ -236,7 +239,8 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const __gr
             for (int j0 = begin; j0 < end; j0 += 32) {
                 const int j = j0 + lane;
                 const bool free = j < end && j >= low && j < high;
-                const uint32_t u = free ? order_of(w[j]) : 0;
+                const float x = weight(j0);
+                const uint32_t u = free ? order_of(x) : 0;
                 const bool counts = free && (shift == 24 || (u >> (shift + 8)) == prefix);
                 const uint32_t digit = counts ? (u >> shift) & 255u : 256u;
                 const uint32_t same = __match_any_sync(0xffffffffu, digit);
@@ -281,7 +285,8 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const __gr
     for (int j0 = begin; j0 < end; j0 += 32) {
         const int j = j0 + lane;
         const bool inside = j < end, free = inside && choose && j >= low && j < high;
-        const uint32_t u = free ? order_of(w[j]) : 0;
+        const float x = weight(j0);
+        const uint32_t u = free ? order_of(x) : 0;
         tied += __popc(__ballot_sync(0xffffffffu, free && u == threshold));
         kept += __popc(__ballot_sync(0xffffffffu, inside && (!free || u > threshold)));
     }
@@ -312,7 +317,7 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const __gr
     for (int j0 = begin; j0 < end; j0 += 32) {
         const int j = j0 + lane;
         const bool inside = j < end, free = inside && choose && j >= low && j < high;
-        const float x = inside ? w[j] : 0.f;
+        const float x = weight(j0);
         const uint32_t u = free ? order_of(x) : 0, below = (1u << lane) - 1u;
         const bool tie = free && u == threshold;
         const uint32_t tie_mask = __ballot_sync(0xffffffffu, tie);

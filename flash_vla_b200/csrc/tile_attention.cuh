@@ -173,6 +173,13 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
+    // Q is asked for before the lengths are known
+    if (tid == 0) {
+        tc5::prefetch_tensormap(&tmQ);
+        mbar_expect_tx(q_full, C::Q_ATOMS * 128 * p.group * p.tile_tokens);
+#pragma unroll
+        for (int c = 0; c < C::Q_ATOMS; ++c) tma_load_5d(sQ + c * 16384, &tmQ, q_full, c * 64, 0, t0, kv * p.q_mul[0], e * p.q_mul[1]);
+    }
     const Episode s = episode_of(a, e);
     const int tokens = min(p.tile_tokens, s.n - t0);      // of this tile; none: nothing to write
     Walk walk;
@@ -208,6 +215,7 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
     walk.first = first + (int)((long long)(last - first) * split / p.splits);
     walk.count = first + (int)((long long)(last - first) * (split + 1) / p.splits) - walk.first;
     const bool any = walk.next(0) < walk.count;
+    if (!any) mbar_wait(q_full, 0, abort_flag);           // nobody else waits for it: neither Q's buffer nor this CTA may go before it has come
 
     // 384 threads start with 168 registers each: 56 + 2 x 224 = 504 = 3 x 168
     if (warp < SOFTMAX0) {
@@ -218,11 +226,7 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
         auto advance = [&]() { if (++at == C::SLOTS) { at = 0; phase ^= 1u; } };
         if (warp == 0) {
             if (lane == 0 && any) {
-                tc5::prefetch_tensormap(&tmQ);
                 tc5::prefetch_tensormap(&tmK);
-                mbar_expect_tx(q_full, C::Q_ATOMS * 128 * p.group * p.tile_tokens);
-#pragma unroll
-                for (int c = 0; c < C::Q_ATOMS; ++c) tma_load_5d(sQ + c * 16384, &tmQ, q_full, c * 64, 0, t0, kv * p.q_mul[0], e * p.q_mul[1]);
                 bool ok = true;
                 for (int i = walk.next(0); i < walk.count && ok; i = walk.next(i + 1)) {
 #pragma unroll 1

@@ -306,7 +306,7 @@ inline int make_map(CUtensorMap* map, const void* base, int rank, const uint64_t
     cuuint32_t b[5], step[5];
     for (int i = 0; i < rank; ++i) { gdim[i] = dims[i]; b[i] = box[i]; step[i] = 1; }
     for (int i = 0; i + 1 < rank; ++i) gstride[i] = strides[i] * elem;
-    const CUresult r = fn(map, elem == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), gdim, gstride, b, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    const CUresult r = fn(map, elem == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : (elem == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32), rank, const_cast<void*>(base), gdim, gstride, b, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) { set_error("attention: cuTensorMapEncodeTiled failed with CUresult %d", (int)r); return FVLA_ERR_ARG; }
     return FVLA_OK;
@@ -433,7 +433,14 @@ inline int launch_attention(const Args& a, void* ws, int* status, cudaStream_t s
         if (rc) return rc;
         const uint64_t out_dims[5] = {dims[0], dims[1], dims[2], dims[3], (uint64_t)a.episodes};
         const uint64_t out_strides[4] = {(uint64_t)a.os[2], (uint64_t)a.os[1], (uint64_t)a.os[2] * p.group, (uint64_t)a.os[0]};
-        if (p.splits == 1) rc = make_map(&tmO, a.out, 5, out_dims, out_strides, box);
+        if (p.splits == 1) {
+            rc = make_map(&tmO, a.out, 5, out_dims, out_strides, box);
+        } else {
+            const uint64_t wide = hdp, row = wide * a.heads;
+            const uint64_t part_dims[5] = {wide, dims[1], dims[2], dims[3], (uint64_t)a.episodes * p.splits}, part_strides[4] = {wide, row, wide * p.group, row * a.tokens};
+            const uint32_t part_box[5] = {32, box[1], box[2], 1, 1};
+            rc = make_map(&tmO, p.part_o, 5, part_dims, part_strides, part_box, 4);
+        }
         if (rc) return rc;
     }
     p.k_mul[0] = a.ks[2] != 0; p.k_mul[1] = a.ks[0] != 0; p.v_mul[0] = a.vs[2] != 0; p.v_mul[1] = a.vs[0] != 0;

@@ -584,7 +584,8 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                         st32_nowait(t_s + 32, r + 32);
                     }
                 } else {
-                    // three terms of four values to a word, 32 columns each
+                    // three terms of four values to a word, 32 columns each (the rest of a term by Veltkamp's splitting instead of a conversion back: 7 300 clocks
+                    // against 4 300)
                     uint32_t w[3][32];
 #pragma unroll
                     for (int q = 0; q < 8; ++q) {
@@ -597,24 +598,12 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                             for (int k = 0; k < 4; ++k) { x[k] = fast_exp2(v[c + k] + off); sum += x[k]; }
 #pragma unroll
                             for (int term = 0; term < 3; ++term) {
-                                // what e4m3 holds of x: 4 bits, or a multiple of 2^-9 below 2^-6, by adding and taking off a larger number of its sign (Veltkamp's splitting);
-                                // 2 to 3 clocks a value where converting back from e4m3 took 9
-                                float hold[4];
+                                const uint32_t lo = term < 2 ? q8::to_e4m3x2(x[0], x[1]) : q8::to_e5m2x2(x[0], x[1]);
+                                const uint32_t hi = term < 2 ? q8::to_e4m3x2(x[2], x[3]) : q8::to_e5m2x2(x[2], x[3]);
+                                w[term][c / 4] = lo | hi << 16;
                                 if (term < 2) {
-#pragma unroll
-                                    for (int k = 0; k < 4; k += 2) {
-                                        float c0 = x[k], c1 = x[k + 1];
-                                        mul2(c0, c1, 1048576.f);
-                                        c0 = copysignf(fmaxf(fabsf(c0), 16384.f), x[k]);
-                                        c1 = copysignf(fmaxf(fabsf(c1), 16384.f), x[k + 1]);
-                                        hold[k] = x[k]; hold[k + 1] = x[k + 1];
-                                        add2(hold[k], hold[k + 1], c0, c1);
-                                        add2(hold[k], hold[k + 1], -c0, -c1);
-                                        add2(x[k], x[k + 1], -hold[k], -hold[k + 1]);
-                                    }
-                                    w[term][c / 4] = q8::to_e4m3x2(hold[0], hold[1]) | q8::to_e4m3x2(hold[2], hold[3]) << 16;
-                                } else {
-                                    w[term][c / 4] = q8::to_e5m2x2(x[0], x[1]) | q8::to_e5m2x2(x[2], x[3]) << 16;
+                                    const float2 b0 = q8::from_e4m3x2(lo), b1 = q8::from_e4m3x2(hi);
+                                    x[0] -= b0.x; x[1] -= b0.y; x[2] -= b1.x; x[3] -= b1.y;
                                 }
                             }
                         }
@@ -705,10 +694,8 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                 }
             }
         } else {
-            // Sums of a share, 32 bits wide, by way of the rings, which are idle now: a thread leaves its half of a row there (pieces of 16 bytes, exchanged
-            // by row against bank conflicts), then a warp takes whole rows, so that stores are contiguous (51.8 us against 39.1 for the chunk of 51 tokens
-            // of eight episodes). bf16 results are stored by their threads above: by this way they took longer (37.1 / 41.0 us for four prefixes).
-            uint8_t* stage = gen + C::OFF_R;
+            // Sums of a share, 32 bits wide, by way of the rings, which are idle now, and the TMA, 32 columns at a time. (Rows behind the episode's last query
+            // are written as well: nobody reads them.)
             if (store && g == 0)
                 p.part_ml[((size_t)split * a.episodes + e) * a.tokens * a.heads + (size_t)(t0 + t) * a.heads + h] = make_float2(l == 0.f ? -INFINITY : m_end, l);
 #pragma unroll 1
@@ -718,16 +705,18 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                 tc5::tmem_ld32(tmem + t_lane + C::O_COL + col, o);
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
-                    *reinterpret_cast<float4*>(stage + row * (HDP * 4) + (((col >> 2) + k) ^ (row & 7)) * 16) = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                    *reinterpret_cast<float4*>(gen + C::OFF_R + (col >> 5) * 16384 + row * 128 + ((k ^ (row & 7)) << 4)) = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
             }
-            asm volatile("bar.sync 9, 256;" ::: "memory");
-            for (int r = warp - SOFTMAX0; r < (ok && any ? tokens * p.group : 0); r += SOFTMAX_WARPS) {
-                const int rt = r / p.group, rh = kv * p.group + r - rt * p.group;
-                const uint8_t* from = stage + r * (HDP * 4);
-                float* to = p.part_o + (((size_t)split * a.episodes + e) * a.tokens * a.heads + (size_t)(t0 + rt) * a.heads + rh) * HDP;
-#pragma unroll
-                for (int k = 0; k < HDP / 4; k += 32)
-                    if (HDP / 4 >= 32 || lane < HDP / 4) *reinterpret_cast<uint4*>(to + (k + lane) * 4) = *reinterpret_cast<const uint4*>(from + ((k + lane) ^ (r & 7)) * 16);
+            if (any) {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                asm volatile("bar.sync 9, 256;" ::: "memory");
+                if (tid == 32 * SOFTMAX0 && ok) {
+#pragma unroll 1
+                    for (int c = 0; c < HDP / 32; ++c)
+                        asm volatile("cp.async.bulk.tensor.5d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5, %6}], [%1];"
+                                     ::"l"(reinterpret_cast<uint64_t>(&tmO)), "r"(ring + c * 16384), "r"(c * 32), "r"(0), "r"(t0), "r"(kv), "r"(split * a.episodes + e) : "memory");
+                    asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group 0;" ::: "memory");
+                }
             }
         }
     }

@@ -103,10 +103,6 @@ __device__ __forceinline__ float tanh_far(float y) {
     const float near = fmaf(y * y2, fmaf(y2, fmaf(y2, kTanh7, kTanh5), kTanh3), y);
     return y2 < 0.04f ? near : far;
 }
-__device__ __forceinline__ float tanh_near(float y) {
-    const float y2 = y * y;
-    return y * fmaf(y2, fmaf(y2, fmaf(y2, fmaf(y2, fmaf(y2, fmaf(y2, kTanh13, kTanh11), kTanh9), kTanh7), kTanh5), kTanh3), 1.f);
-}
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int w) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
                  ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");

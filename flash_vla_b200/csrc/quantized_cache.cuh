@@ -193,7 +193,7 @@ __device__ __forceinline__ uint32_t order_of(float w) {
 // A cluster of `ctas` CTAs per episode: the threshold by a radix select of 8 bits at a time, then the rows that stay, in order. For both each warp has
 // a run of rows of its own; lanes with equal digits add to the histogram together (weights are alike in their leading bits). The CTAs read
 // one another's histograms (two in turn, so that one barrier per digit is enough) and, at last, counts. Bound by latencies: a digit takes a load,
-// the votes, the barrier and a scan of 256 sums (eight episodes of 16 384 rows 18 us; one CTA each 41).
+// the votes, the barrier and a scan of 256 sums (eight episodes of 16 384 rows 16 us; one CTA each 41).
 __device__ __forceinline__ uint32_t remote(const void* shared, int rank) {
     uint32_t r;
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(shared)), "r"(rank));

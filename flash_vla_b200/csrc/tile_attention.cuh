@@ -8,7 +8,7 @@
 //               of P V, so that nothing crosses shared memory. All that one block needs from the one before is the running maximum: the other group
 //               hands it on (per warp, 32 rows) before it begins its exponentials, and those of one block run beside the other's
 //               loads and maxima. The accumulator is rescaled only where the maximum has grown by more than a threshold.
-// 4 096 keys, 32 query heads of 128 or 16 of 256 with two to a K/V head: 270 us (1 018 TFLOP/s) and 112 us (1 231 TFLOP/s). A block of 128 keys takes 2 200 to
+// 4 096 keys, 32 query heads of 128, or 8 of 256 over 4 K/V heads: 270 us (1 018 TFLOP/s) and 112 us (1 231 TFLOP/s). A block of 128 keys takes 2 200 to
 // 2 500 clocks: at head dim 128 the softmax's instructions (128 exponentials of a row at 16 clocks a warp among them), at 256 the arrival of 128 KB of
 // keys and values through 128 KB of rings. A CTA's two ends, 7 000 and 5 000 clocks, are the rest of short walks.
 // The 8-bit cache runs in 8 bits (kind::f8f6f4), its values straight from TMA: a bf16 row of Q, brought to 2^7..2^8 by its own power of two, is the sum

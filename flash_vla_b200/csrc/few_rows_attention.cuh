@@ -9,6 +9,9 @@
 // into e4m3 terms, each a row of the other operand. A bf16 q brought to 2^7..2^8 by its row's power of two is the sum of two terms of 4 bits
 // (the second times 2^5; what falls below the subnormals is under 2^-22 of the row's largest element), a probability the sum of three (times 2^4 and
 // 2^8: 12 bits). Probabilities stand against the running maximum at 2^4, which leaves 2^-22 of it above the last term's half step.
+// The scale of V moves into their exponent, and the row sum takes it back: by its inverse over the first key's scale while all scales of a share lie
+// within 2^30 of that, and from there on by exponentials of the scores themselves against a maximum of their own (a block of zeros has
+// the scale 2^-120, and its inverse would end fp32's range). What a share leaves is its maximum, its sums and the log2 of its row sum.
 //   warp 0      TMA: K and V tiles of 128 keys in turn through a ring of SLOTS
 //   warp 1      one lane issues the MMAs, S^T a block ahead
 //   warps 2-5   softmax: thread = key. The rows' maxima by redux and through shared memory, sums kept per thread until the end.
@@ -24,6 +27,7 @@ __device__ __forceinline__ float redux_max(float x) {
     asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
     return r;
 }
+constexpr int SCALE_RANGE = 30 << 23;              // either side of the first scale, where P times a scale's inverse may be summed: as the difference of their bits
 // N consecutive columns (a multiple of 16) of this thread's TMEM lane.
 template <int N>
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[N]) {
@@ -204,6 +208,11 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
         float* rescale = in_use + NR;
         const bool capped = a.cap > 0.f;
         auto barrier = []() { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+        auto barrier_or = [](bool x) {
+            uint32_t r;
+            asm volatile("{.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;}" : "=r"(r) : "r"((uint32_t)x) : "memory");
+            return r != 0;
+        };
         bool ok = true;
 
         if (count > 0) {
@@ -277,12 +286,18 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
             if (a.k_pos) next_pos = __ldg(a.k_pos + (size_t)e * a.keys + j);
         };
         if (count > 0) fetch(0);
+        // the sums l stand against `in_use` over `scale0` until a scale has been found far from that, then (lane r: row r) against m_score
+        const float scale0 = Q8 && count > 0 ? __ldg(vs + (size_t)(first * BKEY >> shift) * a.kv_heads) : 1.f;
+        float m_score = -INFINITY;
+        bool wide = false;
         float* scores = p.scores + (size_t)e * a.heads * a.tokens * p.pitch;
         for (int n = 0; n < count; ++n) {
             const int b = n & 1, j = (first + n) * BKEY + key;
             const bool inside = j < s.L;
-            const float kf = next_k, lv = Q8 ? q8::log2_of_scale(next_v) : 0.f, iv = Q8 ? __frcp_rn(next_v) : 1.f;      // K's scale; log2 of V's and its inverse
+            const float kf = next_k, lv = Q8 ? q8::log2_of_scale(next_v) : 0.f;      // K's scale; log2 of V's
             const int kp = a.k_pos ? next_pos : j;
+            float iv = Q8 ? scale0 * __frcp_rn(next_v) : 1.f;                  // what a probability counts in the row sum
+            const bool far = Q8 && inside && abs(__float_as_int(next_v) - __float_as_int(scale0)) > SCALE_RANGE;
             if (n + 1 < count) fetch(n + 1);
             ok = ok && mbar_wait(s_full(b), (uint32_t)((n >> 1) & 1), abort_flag);
             __syncwarp();
@@ -324,7 +339,32 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
             }
             float* board = maxima + b * 4 * NR;
             if (lane < NR) board[quad * NR + lane] = mine;
-            barrier();
+            if (!Q8) barrier();
+            else if (barrier_or(far) || wide) {                                // (the same for every warp)
+                // the row sums by exponentials of their own, with the maxima's other half and the arrays that the probabilities take below
+                if (!wide) m_score = m_lane == -INFINITY ? -INFINITY : m_lane - C::SHIFT - q8::log2_of_scale(scale0);
+                wide = true;
+                iv = 0.f;
+                float* scored = maxima + (b ^ 1) * 4 * NR;
+                float most = -INFINITY;
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                    const float x = redux_max(v[r] - lv);
+                    if (lane == r) most = x;
+                }
+                if (lane < NR) scored[quad * NR + lane] = most;
+                barrier();
+                if (lane < NR) {
+                    const float was = m_score;
+                    m_score = fmaxf(m_score, fmaxf(fmaxf(scored[lane], scored[NR + lane]), fmaxf(scored[2 * NR + lane], scored[3 * NR + lane])));
+                    rescale[lane] = was == m_score || was == -INFINITY ? 1.f : fast_exp2(was - m_score);
+                    in_use[lane] = m_score == -INFINITY ? 0.f : m_score;
+                }
+                __syncwarp();
+#pragma unroll
+                for (int r = 0; r < NR; ++r) l[r] = fmaf(l[r], rescale[r], fast_exp2(v[r] - lv - in_use[r]));
+                barrier();                                                     // the maxima have been read
+            }
             bool grow = false;
             if (lane < NR) {
                 const float mx = fmaxf(fmaxf(board[lane], board[NR + lane]), fmaxf(board[2 * NR + lane], board[3 * NR + lane]));
@@ -353,8 +393,10 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
                     }
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc5::tc_fence_before();
+                if (!wide) {
 #pragma unroll
-                for (int r = 0; r < NR; ++r) l[r] *= rescale[r];
+                    for (int r = 0; r < NR; ++r) l[r] *= rescale[r];
+                }
             }
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
@@ -420,7 +462,8 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
         };
         if (quad == 0 && lane < NR) {
             const float sum = count > 0 ? maxima[lane] + maxima[NR + lane] + maxima[2 * NR + lane] + maxima[3 * NR + lane] : 0.f;
-            const float2 ml = make_float2(count > 0 ? in_use[lane] : -INFINITY, sum);
+            float2 ml = make_float2(count > 0 ? in_use[lane] : -INFINITY, sum);
+            if (Q8) ml.y = sum == 0.f ? -INFINITY : log2f(sum) + (wide ? (m_score == -INFINITY ? 0.f : m_score) : ml.x - q8::log2_of_scale(scale0));
             if (p.cluster) reinterpret_cast<float2*>(gen + C::OFF_F)[lane] = ml;      // (the rows' factors are no longer needed)
             else if (lane < rows) p.part_ml[flat(lane)] = ml;
         }
@@ -449,11 +492,12 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
             for (int i = split * 128 + me; i < rows * HDP; i += p.splits * 128) {
                 const int r = i / HDP, d = i % HDP;
                 // all that the CTAs have of it at once; what a share that held nothing has left is dropped
+                constexpr float NOTHING = Q8 ? -INFINITY : 0.f;
                 float2 ml[CLUSTER];
-                float y[CLUSTER], top = -INFINITY, sum = 0.f, x = 0.f;
+                float y[CLUSTER], top = -INFINITY, top_sum = -INFINITY, sum = 0.f, x = 0.f;
 #pragma unroll
                 for (int c = 0; c < CLUSTER; ++c) {
-                    ml[c] = make_float2(-INFINITY, 0.f);
+                    ml[c] = make_float2(-INFINITY, NOTHING);
                     if (c < p.splits) {
                         uint32_t at;
                         asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(base + C::OFF_F + r * 8), "r"(c));
@@ -464,17 +508,19 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
                 }
 #pragma unroll
                 for (int c = 0; c < CLUSTER; ++c)
-                    if (ml[c].y != 0.f) top = fmaxf(top, ml[c].x);
+                    if (ml[c].y != NOTHING) { top = fmaxf(top, ml[c].x); top_sum = fmaxf(top_sum, ml[c].y); }
+                if (!Q8) top_sum = top;
 #pragma unroll
                 for (int c = 0; c < CLUSTER; ++c) {
-                    const float w = ml[c].y == 0.f ? 0.f : fast_exp2(ml[c].x - top);
-                    sum = fmaf(ml[c].y, w, sum);
-                    x = ml[c].y == 0.f ? x : fmaf(y[c], w, x);
+                    const float w = ml[c].y == NOTHING ? 0.f : fast_exp2(ml[c].x - top);
+                    sum = Q8 ? sum + (ml[c].y == NOTHING ? 0.f : fast_exp2(ml[c].y - top_sum)) : fmaf(ml[c].y, w, sum);
+                    x = ml[c].y == NOTHING ? x : fmaf(y[c], w, x);
                 }
                 const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);
+                const float half = Q8 && sum > 0.f ? fast_exp2(0.5f * (top - top_sum)) : 1.f;      // the two maxima may lie beyond fp32's range of one another
                 const int t = r / group, h = kv * group + r - t * group;
-                if (d < a.dim) a.out[e * a.os[0] + t * a.os[1] + h * a.os[2] + d] = __float2bfloat16_rn(x * inv);
-                if (a.lse && d == 0) a.lse[((size_t)e * a.heads + h) * a.tokens + t] = sum > 0.f ? (top + log2f(sum)) * 0.6931471805599453f : (sum == 0.f ? -INFINITY : sum);
+                if (d < a.dim) a.out[e * a.os[0] + t * a.os[1] + h * a.os[2] + d] = __float2bfloat16_rn(x * half * (inv * half));
+                if (a.lse && d == 0) a.lse[((size_t)e * a.heads + h) * a.tokens + t] = sum > 0.f ? (top_sum + log2f(sum)) * 0.6931471805599453f : (sum == 0.f ? -INFINITY : sum);
             }
         }
         __syncwarp();

@@ -57,7 +57,7 @@ struct Tile {
     int group, tile_tokens, tiles, splits;      // query heads per K/V head, tokens per tile
     int q_mul[2], k_mul[2], v_mul[2];           // 0 where an axis (K/V head, episode) is broadcast: its coordinate stays 0
     float* part_o;                              // [split][row][HDP] fp32, row = ((e * tokens + t) * heads + h)
-    float2* part_ml;                            // [split][row] maximum (log2) and sum
+    float2* part_ml;                            // [split][row] maximum (log2) and row sum; of the 8-bit cache, whose row sums have a maximum of their own, the sum's log2
     float* scores;                              // log2 units, or null: what the keys' weights are made of
     long long pitch;                            // few rows: [row][pitch]
     int key_blocks;                             // many: [episode, K/V head, tile][key block][4 keys][128 rows][4]
@@ -141,7 +141,7 @@ struct Walk {
     }
 };
 
-// The shares' sums against the largest of their maxima. `warps` of a CTA take 32 * PER columns of a row together (grid.y: which): each adds up every
+// The shares' sums against the largest of their maxima (the row sums of the 8-bit cache against the largest of theirs). `warps` of a CTA take 32 * PER columns of a row together (grid.y: which): each adds up every
 // warps-th share, and the first adds up the warps in their order.
 constexpr int JOIN_WARPS = 8;
 template <int PER>
@@ -154,15 +154,19 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) attention_join_kernel(const _
     const int row = blockIdx.x * (JOIN_WARPS / warps) + warp / warps, rows = a.episodes * a.tokens * a.heads;      // (below 2^31: checked on the host)
     const int h = row % a.heads, t = row / a.heads % a.tokens, e = min(row / a.heads / a.tokens, a.episodes - 1);
     const bool mine = row < rows && t < episode_of(a, e).n;
+    const bool logs = a.k_scale != nullptr;
+    const float nothing = logs ? -INFINITY : 0.f;
     // no load waits for another, but for the maxima: shares that held nothing are read as well, and dropped
-    float m = -INFINITY;
+    float m = -INFINITY, m_sum = -INFINITY;
 #pragma unroll 4
     for (int s = lane; s < p.splits; s += 32) {
-        const float2 ml = mine ? p.part_ml[(size_t)s * rows + row] : make_float2(0.f, 0.f);
-        if (ml.y != 0.f) m = fmaxf(m, ml.x);
+        const float2 ml = mine ? p.part_ml[(size_t)s * rows + row] : make_float2(0.f, nothing);
+        if (ml.y != nothing) { m = fmaxf(m, ml.x); m_sum = fmaxf(m_sum, ml.y); }
     }
     m = warp_max(m);
     const float top = m == -INFINITY ? 0.f : m;
+    m_sum = logs ? warp_max(m_sum) : top;
+    const float top_sum = m_sum == -INFINITY ? 0.f : m_sum;
     float acc[PER], l = 0.f;                                                         // columns lane, lane + 32, ...
 #pragma unroll
     for (int c = 0; c < PER; ++c) acc[c] = 0.f;
@@ -171,9 +175,10 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) attention_join_kernel(const _
     for (int s0 = part; s0 < p.splits; s0 += 32 * warps) {
         // lane i: the factor of share s0 + i * warps
         const int s = s0 + lane * warps;
-        const float2 ml = mine && s < p.splits ? p.part_ml[(size_t)s * rows + row] : make_float2(0.f, 0.f);
-        const float w = ml.y == 0.f ? 0.f : (ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - top));
-        l += warp_sum(ml.y == 0.f ? 0.f : ml.y * w);
+        const float2 ml = mine && s < p.splits ? p.part_ml[(size_t)s * rows + row] : make_float2(0.f, nothing);
+        const bool held = ml.y != nothing;
+        const float w = !held ? 0.f : (ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - top));
+        l += warp_sum(!held ? 0.f : (logs ? fast_exp2(ml.y - top_sum) : ml.y * w));
         const int have = min(32, (p.splits - s0 + warps - 1) / warps);
         constexpr int BATCH = PER == 1 ? 16 : 4;                                     // loads in flight before the first is used
         for (int i = 0; i < have; i += BATCH) {
@@ -184,9 +189,10 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) attention_join_kernel(const _
                 for (int c = 0; c < PER; ++c) x[k][c] = o[(size_t)(s0 + min(i + k, have - 1) * warps) * pitch + 32 * c];
 #pragma unroll
             for (int k = 0; k < BATCH; ++k) {
-                const float f = __shfl_sync(0xffffffffu, w, i + k & 31), used = __shfl_sync(0xffffffffu, ml.y, i + k & 31);
+                const float f = __shfl_sync(0xffffffffu, w, i + k & 31);
+                const bool used = __shfl_sync(0xffffffffu, held, i + k & 31);
 #pragma unroll
-                for (int c = 0; c < PER; ++c) acc[c] = fmaf(i + k < have ? f : 0.f, i + k < have && used != 0.f ? x[k][c] : 0.f, acc[c]);
+                for (int c = 0; c < PER; ++c) acc[c] = fmaf(i + k < have ? f : 0.f, i + k < have && used ? x[k][c] : 0.f, acc[c]);
             }
         }
     }
@@ -204,11 +210,12 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) attention_join_kernel(const _
     }
     if (!mine) return;
     const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
+    const float half = logs ? fast_exp2(0.5f * (top - top_sum)) : 1.f;               // the two maxima may lie beyond fp32's range of one another
     bf16* dst = a.out + e * a.os[0] + t * a.os[1] + h * a.os[2];
 #pragma unroll
     for (int c = 0; c < PER; ++c)
-        if (col0 + 32 * c < a.dim) dst[col0 + 32 * c] = __float2bfloat16_rn(acc[c] * inv);
-    if (a.lse && lane == 0 && blockIdx.y == 0) a.lse[((size_t)e * a.heads + h) * a.tokens + t] = l > 0.f ? (top + log2f(l)) * 0.6931471805599453f : (l == 0.f ? -INFINITY : l);
+        if (col0 + 32 * c < a.dim) dst[col0 + 32 * c] = __float2bfloat16_rn(acc[c] * half * (inv * half));
+    if (a.lse && lane == 0 && blockIdx.y == 0) a.lse[((size_t)e * a.heads + h) * a.tokens + t] = l > 0.f ? (top_sum + log2f(l)) * 0.6931471805599453f : (l == 0.f ? -INFINITY : l);
 }
 
 // weights[e][j] = decay * weights[e][j] + the probabilities that key j got, from the scores that the attention left and the rows' log-sum-exps. `share`

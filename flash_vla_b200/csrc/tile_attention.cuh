@@ -15,7 +15,9 @@
 // of an e4m3 term and an e5m2 term (what rounding to 4 bits leaves of 8 has at most 3; below 2^-16, 2^-23 of the largest, is lost), a probability the sum
 // of two e4m3 terms and an e5m2 term (11 bits; the last holds what is below e4m3's range). Probabilities stand against the running maximum at 2^6
 // and are rescaled when it has grown by 2^2, so that what falls below the last term is under 2^-24 of the largest. The scale of K multiplies the scores in fp32; the
-// scale of V moves into the exponent of P (w = log2 p + log2 V_scale, P = 2^(w - max w)), and the row sum takes it back.
+// scale of V moves into the exponent of P (w = log2 p + log2 V_scale, P = 2^(w - max w)), and the row sum takes it back: the sum of 16 keys' P times one
+// power of two, against a maximum of the scores alone, so that no scale can carry it beyond fp32. Where a scale lies more than 2^60 below what the maxima
+// have between them (a block of zeros has 2^-120), P may have lost what the row sum needs, and exponentials of the scores take its place.
 #pragma once
 
 namespace fvla {
@@ -117,7 +119,7 @@ struct TileCfg {
     static constexpr int SMEM = 1024 + OFF_BAR + 344;
     static constexpr int THREADS = 32 * (SOFTMAX0 + SOFTMAX_WARPS);
     static constexpr uint32_t O_COL = BUFFERS * BKEY;
-    static constexpr float SHIFT = Q8 ? 6.f : 0.f, THRESHOLD = Q8 ? 2.f : RESCALE_THRESHOLD;
+    static constexpr float SHIFT = Q8 ? 6.f : 0.f, THRESHOLD = Q8 ? 2.f : RESCALE_THRESHOLD, SCALE_RANGE = 60.f;
 };
 
 template <int HDP, bool Q8>
@@ -387,7 +389,7 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
             if (lane == 0) tc5::mbar_arrive(q_ready);
         }
 
-        float m_used = -INFINITY, l = 0.f;                             // what this group's sum stands against
+        float m_used = -INFINITY, l = 0.f;                             // what this group's sum stands against (8-bit cache: a maximum of the scores)
         const int shift = Q8 ? 31 - __clz(a.block) : 0;                // blocks are powers of two
         const bool plain = !capped && a.slopes == nullptr && (factor > 1e-30f || !mine);
         const bool fast = !Q8 && __all_sync(0xffffffffu, plain);       // the factor goes into the exponential's argument
@@ -515,16 +517,21 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
 #pragma unroll
                     for (int c = 0; c < BKEY; c += 4) dst[c / 4 * BQ] = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
                 }
-                float top[8];
+                float top[8], m_score = -INFINITY;
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
                     float x = fmaxf(v[16 * q], v[16 * q + 1]);
 #pragma unroll
                     for (int c = 2; c < 16; c += 2) x = max3(x, v[16 * q + c], v[16 * q + c + 1]);
+                    if (Q8) m_score = fmaxf(m_score, x);
                     top[q] = Q8 ? x + lv[q] : x;
                 }
                 float mx = max3(max3(top[0], top[1], top[2]), max3(top[3], top[4], top[5]), fmaxf(top[6], top[7]));
                 if (fast) mx *= factor;
+                if (Q8 && m_score > m_used) {
+                    l *= m_used == -INFINITY ? 1.f : fast_exp2(m_used - m_score);
+                    m_used = m_score;
+                }
                 // the maximum that the blocks before have left, and what becomes of it
                 if (n > 0) asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + quad) : "memory");
                 const float m_old = n > 0 ? m_shared[row] : -INFINITY;
@@ -550,7 +557,7 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                 }
                 m_shared[row] = m_new;
                 if (after_i < walk.count) asm volatile("bar.arrive %0, 64;" ::"r"(1 + (g ^ 1) * 4 + quad) : "memory");
-                if (m_new != m_used) {
+                if (!Q8 && m_new != m_used) {
                     l *= m_used == -INFINITY ? 1.f : fast_exp2(m_used - m_new);
                     m_used = m_new;
                 }
@@ -587,6 +594,17 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                     // three terms of four values to a word, 32 columns each (the rest of a term by Veltkamp's splitting instead of a conversion back: 7 300 clocks
                     // against 4 300)
                     uint32_t w[3][32];
+                    const float m_sum = m_used == -INFINITY ? 0.f : m_used, between = m - m_sum;
+                    const float least = fminf(fminf(fminf(lv[0], lv[1]), fminf(lv[2], lv[3])), fminf(fminf(lv[4], lv[5]), fminf(lv[6], lv[7])));
+                    if (__any_sync(0xffffffffu, between - least > C::SCALE_RANGE)) {
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) {
+                            float sum = 0.f;
+#pragma unroll
+                            for (int c = q * 16; c < q * 16 + 16; ++c) sum += fast_exp2(v[c] - m_sum);
+                            if (between - lv[q] > C::SCALE_RANGE) l += sum;
+                        }
+                    }
 #pragma unroll
                     for (int q = 0; q < 8; ++q) {
                         float sum = 0.f;
@@ -607,7 +625,8 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                                 }
                             }
                         }
-                        l = fmaf(sum, fast_exp2(-lv[q]), l);
+                        const float to_scores = between - lv[q];
+                        l = fmaf(sum, to_scores > C::SCALE_RANGE ? 0.f : fast_exp2(to_scores), l);
                     }
 #pragma unroll
                     for (int term = 0; term < 3; ++term) st32_nowait(t_s + 32 * term, w[term]);
@@ -650,17 +669,29 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
         tc5::tc_fence_after();
         // the row's sum from its two threads, then half of the columns each
         const float m_all = any && busy ? m_shared[row] : -INFINITY;
-        if (m_used != -INFINITY) l *= fast_exp2(m_used - m_all);
-        xch[g * BQ + row] = l;
-        asm volatile("bar.sync 9, 256;" ::: "memory");
-        l = xch[row] + xch[BQ + row];
         const float m_end = (m_all == -INFINITY ? 0.f : m_all) - C::SHIFT;
+        float m_sum = m_end, half = 1.f;                               // what l stands against; root of what lies between the accumulator's maximum and that
+        if (!Q8) {
+            if (m_used != -INFINITY) l *= fast_exp2(m_used - m_all);
+            xch[g * BQ + row] = l;
+            asm volatile("bar.sync 9, 256;" ::: "memory");
+            l = xch[row] + xch[BQ + row];
+        } else {
+            float* maxima = reinterpret_cast<float*>(gen + C::OFF_R + (2 * C::SLOTS - 1) * C::GRANULE);      // (the rings are idle; results take their first slots at most)
+            xch[g * BQ + row] = l;
+            maxima[g * BQ + row] = m_used;
+            asm volatile("bar.sync 9, 256;" ::: "memory");
+            const float m0 = maxima[row], m1 = maxima[BQ + row], m_both = fmaxf(m0, m1);
+            m_sum = m_both == -INFINITY ? 0.f : m_both;
+            l = xch[row] * fast_exp2(m0 - m_sum) + xch[BQ + row] * fast_exp2(m1 - m_sum);
+            half = fast_exp2(0.5f * (m_end - m_sum));
+        }
         const bool store = ok && mine;
         constexpr int SPAN = HDP / 2;                                  // columns of a thread
         if (p.splits == 1) {
-            const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);             // NaN stays
+            const float inv = (l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l)) * half;    // NaN stays
             if (store && g == 0 && a.lse)
-                a.lse[((size_t)e * a.heads + h) * a.tokens + t0 + t] = l > 0.f ? (m_end + log2f(l)) * 0.6931471805599453f : (l == 0.f ? -INFINITY : l);
+                a.lse[((size_t)e * a.heads + h) * a.tokens + t0 + t] = l > 0.f ? (m_sum + log2f(l)) * 0.6931471805599453f : (l == 0.f ? -INFINITY : l);
             // Q's buffer takes the results in Q's layout, and the TMA stores them: all rows of the box, or all that the tensor has. A tile that ends at its
             // episode's last query is stored by its threads (for four prefixes of 8 x 256, 37.1 us if all are).
             const bool whole = tokens == p.tile_tokens || t0 + tokens == a.tokens;
@@ -671,7 +702,7 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                 const int col = g * SPAN + c;
                 if (any) tc5::tmem_ld32(tmem + t_lane + C::O_COL + col, o);
 #pragma unroll
-                for (int k = 0; k < 32; ++k) o[k] = any ? o[k] * inv : 0.f;
+                for (int k = 0; k < 32; ++k) o[k] = any ? (Q8 ? o[k] * half : o[k]) * inv : 0.f;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const uint4 u = make_uint4(pack_bf16x2(o[8 * k], o[8 * k + 1]), pack_bf16x2(o[8 * k + 2], o[8 * k + 3]), pack_bf16x2(o[8 * k + 4], o[8 * k + 5]),
@@ -697,7 +728,7 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
             // Sums of a share, 32 bits wide, by way of the rings, which are idle now, and the TMA, 32 columns at a time. (Rows behind the episode's last query
             // are written as well: nobody reads them.)
             if (store && g == 0)
-                p.part_ml[((size_t)split * a.episodes + e) * a.tokens * a.heads + (size_t)(t0 + t) * a.heads + h] = make_float2(l == 0.f ? -INFINITY : m_end, l);
+                p.part_ml[((size_t)split * a.episodes + e) * a.tokens * a.heads + (size_t)(t0 + t) * a.heads + h] = make_float2(l == 0.f ? -INFINITY : m_end, !Q8 ? l : (l == 0.f ? -INFINITY : m_sum + log2f(l)));
 #pragma unroll 1
             for (int c = 0; c < (busy && any ? SPAN : 0); c += 32) {
                 float o[32];

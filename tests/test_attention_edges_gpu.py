@@ -1,0 +1,128 @@
+"""Masked attention and the 8-bit cache on the GPU where their arithmetic, their plans and their operands have edges, against plain 64-bit forms."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import attention_cases as A
+from flash_vla_b200 import op_table
+from flash_vla_b200.hardware.nvidia.b200.pi0.backends.cuda import _lib
+from flash_vla_b200.hardware.nvidia.b200.pi0.buffers import QuantizedCache, allocate_quantized_cache
+
+pytestmark = pytest.mark.gpu
+bf16, f32, i32, e4m3 = torch.bfloat16, torch.float32, torch.int32, torch.float8_e4m3fn
+NAN, INF = math.nan, math.inf
+P_8BIT = 2.0 ** -11      # half a step of the probabilities over the 8-bit cache
+
+
+@pytest.fixture(autouse=True)
+def no_wait_has_run_out():
+    """A kernel that gives up on a wait leaves a code in the device's health word."""
+    yield
+    torch.cuda.synchronize()
+    assert _lib.load().fvla_device_status(None) == 0
+
+
+def randn(seed, *shape, dtype=bf16):
+    return torch.randn(shape, device="cuda", generator=torch.Generator("cuda").manual_seed(seed)).to(dtype)
+
+
+def cache_of(K, V, block=64):
+    E, rows, HK, D = K.shape
+    cache = allocate_quantized_cache(E, rows, HK, D, "cuda", block)
+    op_table().cache_append(K, V, cache, A.ints([0] * E))
+    return cache
+
+
+def check_cached(Q, cache, lengths, scale, **kw):
+    """Result, log-sum-exp and weights against the 64-bit form, and the result without the two.
+
+    P, a probability times V's scale, is held in three 8-bit terms against the largest P of the row, which stands at 2^6 or more (few rows: 2^4). Two terms of
+    e4m3 leave P 2^-8 or, among its subnormals (steps of 2^-9), 2^-10; a third of e5m2 at most 2^-3 of that: P 2^-11, or 2^-13, which is 2^-19 of the largest.
+    (Few rows, where the terms are e4m3 times 1, 2^-4 and 2^-8: 2^-10, then 2^-14, then 2^-18 are left, 2^-22 of the largest.) So the probabilities' half
+    step is on top of one term for each key: 2^-19 (2^-22) of the largest P, times the value that the cache holds."""
+    D, rows = Q.shape[3], cache.K.shape[1]
+    want = A.attention(Q, A.widened(cache.K, cache.K_scale), A.widened(cache.V, cache.V_scale), scale, k_lens=lengths, **kw)
+    HK = cache.K.shape[2]
+    group = Q.shape[2] // HK
+    lowest = 2.0 ** (-22 if Q.shape[1] * group <= 32 else -19)
+    per_row = cache.V_scale.double().repeat_interleave(rows // cache.V_scale.shape[1], 1).transpose(1, 2).repeat_interleave(group, 1)        # (E, H, rows)
+    top = (want["p"] * per_row[:, :, None]).amax(-1)                                                                                    # (E, H, T)
+    held = cache.V.double().abs().permute(0, 2, 1, 3).repeat_interleave(group, 1)
+    want["spread"] = want["spread"] + (top[..., None] * ((want["p"] > 0).double() @ held)).permute(0, 2, 1, 3) * (lowest / P_8BIT)
+    out, lse, bare = torch.full_like(Q, 7.0), torch.full((Q.shape[0], Q.shape[2], Q.shape[1]), 7.0, device="cuda"), torch.full_like(Q, 7.0)
+    before = randn(9, Q.shape[0], rows, dtype=f32).abs()
+    w = before.clone()
+    op_table().cache_attention(Q, cache, lengths, scale, out, lse=lse, weights=w, decay=0.5, **kw)
+    A.check_out(out, want, D, P_8BIT)
+    A.check_lse(lse, want, D)
+    A.check_weights(w, want, D, lengths, before, 0.5)
+    op_table().cache_attention(Q, cache, lengths, scale, bare, **kw)
+    assert torch.equal(bare, out)
+    return out, want
+
+
+# Both kernels, with the shares of a row in one CTA, in a cluster and in scratch (the comments: shares of a row at 148 SMs)
+SHARED_OUT = [  # episodes, tokens, rows, heads, kv heads, dim, block
+    (1, 1, 128, 8, 1, 64, 16),      # few rows: 1
+    (2, 1, 1024, 8, 1, 256, 64),    # 8, a cluster
+    (1, 2, 4096, 16, 2, 128, 32),   # 8 of four blocks
+    (1, 4, 1024, 8, 1, 256, 128),   # 32 rows, 8
+    (32, 1, 640, 8, 8, 128, 64),    # 3
+    (1, 1, 12800, 8, 1, 256, 64),   # 100, in scratch
+    (2, 51, 832, 8, 1, 256, 64),    # 128-row tiles: 7
+    (1, 40, 640, 8, 2, 64, 16),     # 5
+    (8, 160, 512, 8, 1, 128, 64),   # 80 tiles: 1
+    (8, 160, 512, 8, 1, 256, 16)]   # 1
+
+
+@pytest.mark.parametrize("where", ["first", "middle", "last", "all", "all but one", "every other"])
+@pytest.mark.parametrize("shape", SHARED_OUT)
+def test_values_that_are_zero(shape, where):
+    """Blocks of V that are all zero get the smallest scale there is. Their keys count in the row sums like any others."""
+    E, T, rows, H, HK, D, block = shape
+    K, V = randn(31, E, rows, HK, D), randn(32, E, rows, HK, D)
+    middle = rows // 256 * 128
+    at = {"first": slice(0, 128), "middle": slice(middle, middle + 128), "last": slice(rows - 128, rows), "all": slice(0, rows), "all but one": slice(0, rows - block),
+          "every other": None}[where]
+    if at is None:
+        V.view(E, rows // block, block, HK, D)[:, ::2] = 0.0
+    else:
+        V[:, at] = 0.0
+    cache = cache_of(K, V, block)
+    assert (cache.V_scale == 2.0 ** -120).any()
+    lengths = A.ints([rows - 3 * (e % 3) for e in range(E)])
+    check_cached(randn(33, E, T, H, D), cache, lengths, D ** -0.5, causal=True)
+
+
+@pytest.mark.parametrize("T", [1, 4, 40])
+@pytest.mark.parametrize("size", [1e-36, 1e-20, 1e30])
+def test_values_of_every_size(T, size):
+    """V of one small or large size throughout, beside zeros, and beside values of another size that the scores tell apart."""
+    E, rows, H, HK, D = 2, 512, 8, 1, 128
+    Q, K, V = randn(41, E, T, H, D), randn(42, E, rows, HK, D), randn(43, E, rows, HK, D)
+    lengths = A.ints([512, 301])
+    V = (V.float() * size).to(bf16)
+    check_cached(Q, cache_of(K, V), lengths, D ** -0.5)
+    V[:, 128:256] = 0.0
+    check_cached(Q, cache_of(K, V), lengths, D ** -0.5)
+    V[:, 384:] = randn(44, E, 128, HK, D)
+    V[:, 64:128] = randn(45, E, 64, HK, D)
+    for scale in (D ** -0.5, 4.0):
+        check_cached(Q, cache_of(K, V), lengths, scale)
+
+
+@pytest.mark.parametrize("T", [1, 4, 40])
+@pytest.mark.parametrize("gap", [8.0, 20.0, 70.0, 140.0])
+def test_many_small_probabilities_of_zero_values(T, gap):
+    """4 032 keys whose V is zero, each `gap` log2 units below (and above) the 64 that have values: together they count in every row sum."""
+    rows, H, D = 4096, 8, 128
+    Q, K, V = torch.zeros(1, T, H, D, dtype=bf16, device="cuda"), torch.zeros(1, rows, 1, D, dtype=bf16, device="cuda"), torch.zeros(1, rows, 1, D, dtype=bf16, device="cuda")
+    Q[..., 0] = 1.0
+    V[:, 2048:2112] = randn(51, 1, 64, 1, D)
+    for sign in (1.0, -1.0):
+        K[..., 0] = 0.0
+        K[:, 2048:2112, :, 0] = sign
+        check_cached(Q, cache_of(K, V), A.ints([rows]), gap * math.log(2.0))

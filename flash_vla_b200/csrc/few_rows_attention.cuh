@@ -9,9 +9,9 @@
 // into e4m3 terms, each a row of the other operand. A bf16 q brought to 2^7..2^8 by its row's power of two is the sum of two terms of 4 bits
 // (the second times 2^5; what falls below the subnormals is under 2^-22 of the row's largest element), a probability the sum of three (times 2^4 and
 // 2^8: 12 bits). Probabilities stand against the running maximum at 2^4, which leaves 2^-22 of it above the last term's half step.
-// The scale of V moves into their exponent, and the row sum takes it back: by its inverse over the first key's scale while all scales of a share lie
-// within 2^30 of that, and from there on by exponentials of the scores themselves against a maximum of their own (a block of zeros has
-// the scale 2^-120, and its inverse would end fp32's range). What a share leaves is its maximum, its sums and the log2 of its row sum.
+// The scale of V moves into their exponent, and the row sum takes it back; where a share has very small or large scales (a block of zeros has 2^-120, and
+// its inverse would end fp32's range), the row sum is taken from the scores themselves against a maximum of its own. What a share leaves is its maximum, its
+// sums and the log2 of its row sum.
 //   warp 0      TMA: K and V tiles of 128 keys in turn through a ring of SLOTS
 //   warp 1      one lane issues the MMAs, S^T a block ahead
 //   warps 2-5   softmax: thread = key. The rows' maxima by redux and through shared memory, sums kept per thread until the end.
@@ -27,7 +27,6 @@ __device__ __forceinline__ float redux_max(float x) {
     asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
     return r;
 }
-constexpr int SCALE_RANGE = 30 << 23;              // either side of the first scale, where P times a scale's inverse may be summed: as the difference of their bits
 // N consecutive columns (a multiple of 16) of this thread's TMEM lane.
 template <int N>
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[N]) {
@@ -94,6 +93,7 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
     auto empty = [&](int s) { return bars + 88 + s * 8; };
     volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(gen + C::OFF_BAR + 120);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + C::OFF_BAR + 124);
+    volatile int* odd_scales = reinterpret_cast<volatile int*>(gen + C::OFF_BAR + 128);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const Args& a = p.a;
@@ -104,6 +104,7 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
         for (int b = 0; b < 2; ++b) { mbar_init(s_full(b), 1); mbar_init(s_empty(b), 4); }
         for (int s = 0; s < C::SLOTS; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
         *abort_flag = 0;
+        *odd_scales = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -208,14 +209,24 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
         float* rescale = in_use + NR;
         const bool capped = a.cap > 0.f;
         auto barrier = []() { asm volatile("bar.sync 1, 128;" ::: "memory"); };
-        auto barrier_or = [](bool x) {
-            uint32_t r;
-            asm volatile("{.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;}" : "=r"(r) : "r"((uint32_t)x) : "memory");
-            return r != 0;
-        };
         bool ok = true;
 
+        const float* ks = a.k_scale + (size_t)e * (Q8 ? a.keys / a.block : 0) * a.kv_heads + kv;
+        const float* vs = a.v_scale + (size_t)e * (Q8 ? a.keys / a.block : 0) * a.kv_heads + kv;
+        const int shift = Q8 ? 31 - __clz(a.block) : 0;                        // blocks are powers of two
+        // a key's scales and position, fetched a block ahead
+        float next_k = 1.f, next_v = 1.f;
+        int next_pos = 0;
+        auto fetch = [&](int n) {
+            const int j = min((first + n) * BKEY + key, a.keys - 1);
+            if (Q8) {
+                next_k = __ldg(ks + (size_t)(j >> shift) * a.kv_heads);
+                next_v = __ldg(vs + (size_t)(j >> shift) * a.kv_heads);
+            }
+            if (a.k_pos) next_pos = __ldg(a.k_pos + (size_t)e * a.keys + j);
+        };
         if (count > 0) {
+            fetch(0);
             // Q as the K-major operand, and what the rows have of their own (rows of the operand behind NR, and their columns of S^T, are never looked at)
 #pragma unroll
             for (int i = 0; i < Q_ROWS; ++i) {
@@ -264,6 +275,14 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             barrier();
             if (lane == 0) tc5::mbar_arrive(q_ready);
+            if (Q8) {
+                // while the scores are made: whether a scale of V in this share is very small or large
+                const int end = (min((first + count) * BKEY, s.L) + a.block - 1) >> shift;
+                bool odd = false;
+                for (int i = (first * BKEY >> shift) + key; i < end; i += BKEY) odd |= odd_scale(__ldg(vs + (size_t)i * a.kv_heads));
+                if (odd) *odd_scales = 1;
+                barrier();
+            }
         }
 
         float m_lane = -INFINITY;                                              // lane r: the maximum that row r's sums stand against
@@ -271,33 +290,19 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
 #pragma unroll
         for (int r = 0; r < NR; ++r) l[r] = 0.f;
         const float cap2 = a.cap * kLog2e;
-        const float* ks = a.k_scale + (size_t)e * (Q8 ? a.keys / a.block : 0) * a.kv_heads + kv;
-        const float* vs = a.v_scale + (size_t)e * (Q8 ? a.keys / a.block : 0) * a.kv_heads + kv;
-        const int shift = Q8 ? 31 - __clz(a.block) : 0;                        // blocks are powers of two
-        // a key's scales and position, fetched a block ahead
-        float next_k = 1.f, next_v = 1.f;
-        int next_pos = 0;
-        auto fetch = [&](int n) {
-            const int j = min((first + n) * BKEY + key, a.keys - 1);
-            if (Q8) {
-                next_k = __ldg(ks + (size_t)(j >> shift) * a.kv_heads);
-                next_v = __ldg(vs + (size_t)(j >> shift) * a.kv_heads);
-            }
-            if (a.k_pos) next_pos = __ldg(a.k_pos + (size_t)e * a.keys + j);
-        };
-        if (count > 0) fetch(0);
-        // the sums l stand against `in_use` over `scale0` until a scale has been found far from that, then (lane r: row r) against m_score
-        const float scale0 = Q8 && count > 0 ? __ldg(vs + (size_t)(first * BKEY >> shift) * a.kv_heads) : 1.f;
+        // the sums l stand against `in_use`, or, where a scale is very small or large, against (lane r: row r) m_score
         float m_score = -INFINITY;
-        bool wide = false;
         float* scores = p.scores + (size_t)e * a.heads * a.tokens * p.pitch;
-        for (int n = 0; n < count; ++n) {
+        // The walk twice, each form in a loop of its own (32 episodes of 16 K rows: 149 us where one loop has a branch, 144 without).
+        const bool odd = Q8 && count > 0 && *odd_scales;
+#pragma unroll
+        for (int form = 0; form < (Q8 ? 2 : 1); ++form)
+        for (int n = 0; n < count && (form == 1) == odd; ++n) {
             const int b = n & 1, j = (first + n) * BKEY + key;
             const bool inside = j < s.L;
             const float kf = next_k, lv = Q8 ? q8::log2_of_scale(next_v) : 0.f;      // K's scale; log2 of V's
             const int kp = a.k_pos ? next_pos : j;
-            float iv = Q8 ? scale0 * __frcp_rn(next_v) : 1.f;                  // what a probability counts in the row sum
-            const bool far = Q8 && inside && abs(__float_as_int(next_v) - __float_as_int(scale0)) > SCALE_RANGE;
+            const float iv = Q8 ? (form == 0 ? __frcp_rn(next_v) : 0.f) : 1.f;      // what a probability counts in the row sum
             if (n + 1 < count) fetch(n + 1);
             ok = ok && mbar_wait(s_full(b), (uint32_t)((n >> 1) & 1), abort_flag);
             __syncwarp();
@@ -330,6 +335,28 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
                 for (int r = 0; r < NR; ++r)
                     if (r < rows) scores[(size_t)row_number[r] * p.pitch + j] = v[r];
             }
+            float* board = maxima + b * 4 * NR;
+            if (form == 1) {
+                // the row sums by exponentials of their own, with the arrays that the probabilities take below
+                float most = -INFINITY;
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                    const float x = redux_max(v[r]);
+                    if (lane == r) most = x;
+                }
+                if (lane < NR) board[quad * NR + lane] = most;
+                barrier();
+                if (lane < NR) {
+                    const float was = m_score;
+                    m_score = fmaxf(m_score, fmaxf(fmaxf(board[lane], board[NR + lane]), fmaxf(board[2 * NR + lane], board[3 * NR + lane])));
+                    rescale[lane] = was == m_score || was == -INFINITY ? 1.f : fast_exp2(was - m_score);
+                    in_use[lane] = m_score == -INFINITY ? 0.f : m_score;
+                }
+                __syncwarp();
+#pragma unroll
+                for (int r = 0; r < NR; ++r) l[r] = fmaf(l[r], rescale[r], fast_exp2(v[r] - in_use[r]));
+                barrier();                                                     // the maxima have been read
+            }
             float mine = -INFINITY;
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
@@ -337,34 +364,8 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
                 const float x = redux_max(v[r]);
                 if (lane == r) mine = x;
             }
-            float* board = maxima + b * 4 * NR;
             if (lane < NR) board[quad * NR + lane] = mine;
-            if (!Q8) barrier();
-            else if (barrier_or(far) || wide) {                                // (the same for every warp)
-                // the row sums by exponentials of their own, with the maxima's other half and the arrays that the probabilities take below
-                if (!wide) m_score = m_lane == -INFINITY ? -INFINITY : m_lane - C::SHIFT - q8::log2_of_scale(scale0);
-                wide = true;
-                iv = 0.f;
-                float* scored = maxima + (b ^ 1) * 4 * NR;
-                float most = -INFINITY;
-#pragma unroll
-                for (int r = 0; r < NR; ++r) {
-                    const float x = redux_max(v[r] - lv);
-                    if (lane == r) most = x;
-                }
-                if (lane < NR) scored[quad * NR + lane] = most;
-                barrier();
-                if (lane < NR) {
-                    const float was = m_score;
-                    m_score = fmaxf(m_score, fmaxf(fmaxf(scored[lane], scored[NR + lane]), fmaxf(scored[2 * NR + lane], scored[3 * NR + lane])));
-                    rescale[lane] = was == m_score || was == -INFINITY ? 1.f : fast_exp2(was - m_score);
-                    in_use[lane] = m_score == -INFINITY ? 0.f : m_score;
-                }
-                __syncwarp();
-#pragma unroll
-                for (int r = 0; r < NR; ++r) l[r] = fmaf(l[r], rescale[r], fast_exp2(v[r] - lv - in_use[r]));
-                barrier();                                                     // the maxima have been read
-            }
+            barrier();
             bool grow = false;
             if (lane < NR) {
                 const float mx = fmaxf(fmaxf(board[lane], board[NR + lane]), fmaxf(board[2 * NR + lane], board[3 * NR + lane]));
@@ -393,7 +394,7 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
                     }
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc5::tc_fence_before();
-                if (!wide) {
+                if (form == 0) {
 #pragma unroll
                     for (int r = 0; r < NR; ++r) l[r] *= rescale[r];
                 }
@@ -463,7 +464,7 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
         if (quad == 0 && lane < NR) {
             const float sum = count > 0 ? maxima[lane] + maxima[NR + lane] + maxima[2 * NR + lane] + maxima[3 * NR + lane] : 0.f;
             float2 ml = make_float2(count > 0 ? in_use[lane] : -INFINITY, sum);
-            if (Q8) ml.y = sum == 0.f ? -INFINITY : log2f(sum) + (wide ? (m_score == -INFINITY ? 0.f : m_score) : ml.x - q8::log2_of_scale(scale0));
+            if (Q8) ml.y = sum == 0.f ? -INFINITY : log2f(sum) + (odd ? (m_score == -INFINITY ? 0.f : m_score) : ml.x);
             if (p.cluster) reinterpret_cast<float2*>(gen + C::OFF_F)[lane] = ml;      // (the rows' factors are no longer needed)
             else if (lane < rows) p.part_ml[flat(lane)] = ml;
         }

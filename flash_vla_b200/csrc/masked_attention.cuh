@@ -50,6 +50,9 @@ __device__ __forceinline__ Episode episode_of(const Args& p, int e) {
 
 constexpr int BQ = 128, BKEY = 128, SOFTMAX_WARPS = 8, SOFTMAX0 = 4;
 constexpr float RESCALE_THRESHOLD = 8.0f;      // log2 units
+// Row sums over the 8-bit cache add up P (a probability times V's scale, at most 2^8, flushed below 2^-126) over that scale: with all scales of V within these
+// 60 binades that neither leaves fp32 nor misses what is above 2^-60 of a row.
+__device__ __forceinline__ bool odd_scale(float s) { return !(s >= 0x1p-40f && s <= 0x1p20f); }
 
 struct Tile {
     Args a;

@@ -15,9 +15,8 @@
 // of an e4m3 term and an e5m2 term (what rounding to 4 bits leaves of 8 has at most 3; below 2^-16, 2^-23 of the largest, is lost), a probability the sum
 // of two e4m3 terms and an e5m2 term (11 bits; the last holds what is below e4m3's range). Probabilities stand against the running maximum at 2^6
 // and are rescaled when it has grown by 2^2, so that what falls below the last term is under 2^-24 of the largest. The scale of K multiplies the scores in fp32; the
-// scale of V moves into the exponent of P (w = log2 p + log2 V_scale, P = 2^(w - max w)), and the row sum takes it back: the sum of 16 keys' P times one
-// power of two, against a maximum of the scores alone, so that no scale can carry it beyond fp32. Where a scale lies more than 2^60 below what the maxima
-// have between them (a block of zeros has 2^-120), P may have lost what the row sum needs, and exponentials of the scores take its place.
+// scale of V moves into the exponent of P (w = log2 p + log2 V_scale, P = 2^(w - max w)), and the row sum takes it back, or, where a share has very
+// small or large scales (a block of zeros has 2^-120, and its inverse would end fp32's range), is taken from the scores themselves against a maximum of their own.
 #pragma once
 
 namespace fvla {
@@ -119,7 +118,7 @@ struct TileCfg {
     static constexpr int SMEM = 1024 + OFF_BAR + 344;
     static constexpr int THREADS = 32 * (SOFTMAX0 + SOFTMAX_WARPS);
     static constexpr uint32_t O_COL = BUFFERS * BKEY;
-    static constexpr float SHIFT = Q8 ? 6.f : 0.f, THRESHOLD = Q8 ? 2.f : RESCALE_THRESHOLD, SCALE_RANGE = 60.f;
+    static constexpr float SHIFT = Q8 ? 6.f : 0.f, THRESHOLD = Q8 ? 2.f : RESCALE_THRESHOLD;
 };
 
 template <int HDP, bool Q8>
@@ -144,6 +143,7 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
     uint8_t* after = gen + C::OFF_BAR + 120 + C::SLOTS * 32;
     volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(after);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(after + 4);
+    volatile int* odd_scales = reinterpret_cast<volatile int*>(after + 24);
     int* shared_int = reinterpret_cast<int*>(after + 8);      // smallest and largest document of the queries, first and last block seen
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -160,6 +160,7 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
         mbar_init(finished, 1);
         for (int s = 0; s < 2 * C::SLOTS; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
         *abort_flag = 0;
+        *odd_scales = 0;
         shared_int[0] = shared_int[2] = 0x7fffffff;
         shared_int[1] = shared_int[3] = -0x7fffffff - 1;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -387,9 +388,16 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             asm volatile("bar.sync 9, 256;" ::: "memory");                       // xch is free again
             if (lane == 0) tc5::mbar_arrive(q_ready);
+            // while the scores are made: whether a scale of V in this share is very small or large
+            const int shift = 31 - __clz(a.block), end = (min((walk.first + walk.count) * BKEY, s.L) + a.block - 1) >> shift;
+            bool odd = false;
+            for (int i = (walk.first * BKEY >> shift) + tid - 32 * SOFTMAX0; i < end; i += 32 * SOFTMAX_WARPS)
+                odd |= odd_scale(__ldg(a.v_scale + ((size_t)e * (a.keys >> shift) + i) * a.kv_heads + kv));
+            if (odd) *odd_scales = 1;
+            asm volatile("bar.sync 9, 256;" ::: "memory");
         }
 
-        float m_used = -INFINITY, l = 0.f;                             // what this group's sum stands against (8-bit cache: a maximum of the scores)
+        float m_used = -INFINITY, l = 0.f;                             // what this group's sum stands against
         const int shift = Q8 ? 31 - __clz(a.block) : 0;                // blocks are powers of two
         const bool plain = !capped && a.slopes == nullptr && (factor > 1e-30f || !mine);
         const bool fast = !Q8 && __all_sync(0xffffffffu, plain);       // the factor goes into the exponential's argument
@@ -398,13 +406,16 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
         const int nearest = __reduce_min_sync(0xffffffffu, mine ? pos : 0x7fffffff);                // and no row's position lies before a key
         int n = 0, buffer = g, parity = 0, i = walk.next(0);
         if (g == 1 && i < walk.count) { i = walk.next(i + 1); n = 1; }
-        while (i < walk.count) {
+        // each form of the row sum has a loop of its own, and which it is is read again where it matters: a register for it costs the loop 120 bytes of spills
+#pragma unroll
+        for (int form = 0; form < (Q8 ? 2 : 1); ++form)
+        if (!Q8 || (*odd_scales != 0) == (form == 1)) while (i < walk.count) {
             const int after_i = walk.next(i + 1), key0 = walk.block(i) * BKEY;
             float kf[8], lv[8];                                        // (8-bit cache) per 16 keys: factor of the scores; log2 of V's scale
             if (Q8 && busy) {
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
-                    const size_t at = ((size_t)e * (a.keys >> shift) + (min(key0 + c * 16, a.keys - 1) >> shift)) * a.kv_heads + kv;
+                    const size_t at = ((size_t)e * (a.keys >> shift) + (min(key0 + c * 16, s.L - 1) >> shift)) * a.kv_heads + kv;
                     kf[c] = factor * __ldg(a.k_scale + at);
                     lv[c] = q8::log2_of_scale(__ldg(a.v_scale + at));
                 }
@@ -517,21 +528,16 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
 #pragma unroll
                     for (int c = 0; c < BKEY; c += 4) dst[c / 4 * BQ] = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
                 }
-                float top[8], m_score = -INFINITY;
+                float top[8];
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
                     float x = fmaxf(v[16 * q], v[16 * q + 1]);
 #pragma unroll
                     for (int c = 2; c < 16; c += 2) x = max3(x, v[16 * q + c], v[16 * q + c + 1]);
-                    if (Q8) m_score = fmaxf(m_score, x);
                     top[q] = Q8 ? x + lv[q] : x;
                 }
                 float mx = max3(max3(top[0], top[1], top[2]), max3(top[3], top[4], top[5]), fmaxf(top[6], top[7]));
                 if (fast) mx *= factor;
-                if (Q8 && m_score > m_used) {
-                    l *= m_used == -INFINITY ? 1.f : fast_exp2(m_used - m_score);
-                    m_used = m_score;
-                }
                 // the maximum that the blocks before have left, and what becomes of it
                 if (n > 0) asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + quad) : "memory");
                 const float m_old = n > 0 ? m_shared[row] : -INFINITY;
@@ -557,7 +563,7 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                 }
                 m_shared[row] = m_new;
                 if (after_i < walk.count) asm volatile("bar.arrive %0, 64;" ::"r"(1 + (g ^ 1) * 4 + quad) : "memory");
-                if (!Q8 && m_new != m_used) {
+                if (form == 0 && m_new != m_used) {
                     l *= m_used == -INFINITY ? 1.f : fast_exp2(m_used - m_new);
                     m_used = m_new;
                 }
@@ -594,16 +600,16 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                     // three terms of four values to a word, 32 columns each (the rest of a term by Veltkamp's splitting instead of a conversion back: 7 300 clocks
                     // against 4 300)
                     uint32_t w[3][32];
-                    const float m_sum = m_used == -INFINITY ? 0.f : m_used, between = m - m_sum;
-                    const float least = fminf(fminf(fminf(lv[0], lv[1]), fminf(lv[2], lv[3])), fminf(fminf(lv[4], lv[5]), fminf(lv[6], lv[7])));
-                    if (__any_sync(0xffffffffu, between - least > C::SCALE_RANGE)) {
+                    if (form == 1) {
+                        // the row sum from the scores, against a maximum of theirs
+                        float most = m_used;
 #pragma unroll
-                        for (int q = 0; q < 8; ++q) {
-                            float sum = 0.f;
+                        for (int c = 0; c < BKEY; c += 2) most = max3(most, v[c], v[c + 1]);
+                        const float m_sum = most == -INFINITY ? 0.f : most;
+                        l *= m_used == -INFINITY ? 1.f : fast_exp2(m_used - m_sum);
+                        m_used = most;
 #pragma unroll
-                            for (int c = q * 16; c < q * 16 + 16; ++c) sum += fast_exp2(v[c] - m_sum);
-                            if (between - lv[q] > C::SCALE_RANGE) l += sum;
-                        }
+                        for (int c = 0; c < BKEY; ++c) l += fast_exp2(v[c] - m_sum);
                     }
 #pragma unroll
                     for (int q = 0; q < 8; ++q) {
@@ -625,8 +631,7 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
                                 }
                             }
                         }
-                        const float to_scores = between - lv[q];
-                        l = fmaf(sum, to_scores > C::SCALE_RANGE ? 0.f : fast_exp2(to_scores), l);
+                        if (form == 0) l = fmaf(sum, fast_exp2(-lv[q]), l);
                     }
 #pragma unroll
                     for (int term = 0; term < 3; ++term) st32_nowait(t_s + 32 * term, w[term]);
@@ -679,7 +684,7 @@ attention_tile_kernel(const __grid_constant__ Tile p, const __grid_constant__ CU
         } else {
             float* maxima = reinterpret_cast<float*>(gen + C::OFF_R + (2 * C::SLOTS - 1) * C::GRANULE);      // (the rings are idle; results take their first slots at most)
             xch[g * BQ + row] = l;
-            maxima[g * BQ + row] = m_used;
+            maxima[g * BQ + row] = *odd_scales ? m_used : m_used - C::SHIFT;
             asm volatile("bar.sync 9, 256;" ::: "memory");
             const float m0 = maxima[row], m1 = maxima[BQ + row], m_both = fmaxf(m0, m1);
             m_sum = m_both == -INFINITY ? 0.f : m_both;

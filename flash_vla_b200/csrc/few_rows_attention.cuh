@@ -218,7 +218,7 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
         float next_k = 1.f, next_v = 1.f;
         int next_pos = 0;
         auto fetch = [&](int n) {
-            const int j = min((first + n) * BKEY + key, a.keys - 1);
+            const int j = min((first + n) * BKEY + key, s.L - 1);             // (what lies behind the last row may be anything, scales too)
             if (Q8) {
                 next_k = __ldg(ks + (size_t)(j >> shift) * a.kv_heads);
                 next_v = __ldg(vs + (size_t)(j >> shift) * a.kv_heads);

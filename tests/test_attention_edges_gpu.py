@@ -126,3 +126,22 @@ def test_many_small_probabilities_of_zero_values(T, gap):
         K[..., 0] = 0.0
         K[:, 2048:2112, :, 0] = sign
         check_cached(Q, cache_of(K, V), A.ints([rows]), gap * math.log(2.0))
+
+
+@pytest.mark.parametrize("T", [1, 4, 40])
+@pytest.mark.parametrize("block", [16, 32, 64])
+@pytest.mark.parametrize("unused", [0.0, NAN, INF, 1e-40, -1.0])
+def test_scales_behind_the_lengths_may_be_anything(T, block, unused):
+    """Blocks that no row has reached (a cache whose scales were never initialised) have no part in either kernel."""
+    E, rows, H, HK, D = 3, 512, 8, 1, 128
+    cache = cache_of(randn(61, E, rows, HK, D), randn(62, E, rows, HK, D), block)
+    Q, lengths = randn(63, E, T, H, D), A.ints([512 - 3 * block, 129, 40])
+    kw = {"causal": True, "slopes": torch.full((H,), 0.01, device="cuda")}
+    want, w = torch.zeros_like(Q), torch.zeros(E, rows, device="cuda")
+    op_table().cache_attention(Q, cache, lengths, 0.1, want, weights=w, **kw)
+    for e, L in enumerate(lengths.tolist()):
+        for scale in cache[2:]:
+            scale[e, (L + block - 1) // block:] = unused
+    out, again = torch.zeros_like(Q), torch.zeros_like(w)
+    op_table().cache_attention(Q, cache, lengths, 0.1, out, weights=again, **kw)
+    assert torch.isfinite(out).all() and torch.equal(out, want) and torch.equal(again, w)

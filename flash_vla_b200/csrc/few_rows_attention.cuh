@@ -483,6 +483,15 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
             }
         }
     }
+    // Tensor memory goes back before the cluster meets: a CTA that held some while it waits for another could wait for ever, where that one waits for tensor memory
+    // that a cluster of another kernel (on another stream) holds in the same way.
+    __syncwarp();
+    tc5::tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc5::tc_fence_after();
+        tc5::tmem_dealloc(tmem, C::COLS);
+    }
     if (p.cluster) {
         auto cluster_barrier = []() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); };
         __syncwarp();
@@ -526,13 +535,6 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
         }
         __syncwarp();
         cluster_barrier();                                                              // nobody leaves while its sums may be read
-    }
-
-    tc5::tc_fence_before();
-    __syncthreads();
-    if (warp == 1) {
-        tc5::tc_fence_after();
-        tc5::tmem_dealloc(tmem, C::COLS);
     }
     if (tid == 0 && *abort_flag && p.status) atomicExch(p.status, 9);
 }

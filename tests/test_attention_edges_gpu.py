@@ -145,3 +145,23 @@ def test_scales_behind_the_lengths_may_be_anything(T, block, unused):
     out, again = torch.zeros_like(Q), torch.zeros_like(w)
     op_table().cache_attention(Q, cache, lengths, 0.1, out, weights=again, **kw)
     assert torch.isfinite(out).all() and torch.equal(out, want) and torch.equal(again, w)
+
+
+def test_clusters_of_two_streams_share_the_tensor_memory():
+    """Two kernels whose CTAs fit an SM together by their shared memory, but not by their tensor memory (512 and 64 of 512 columns), each of clusters that meet."""
+    rows = 4096
+    sets = []
+    for i, (E, T, H, HK, D) in enumerate([(16, 4, 8, 1, 256), (16, 1, 8, 2, 128)]):
+        cache = cache_of(randn(71 + i, E, rows, HK, D), randn(73 + i, E, rows, HK, D))
+        Q, lengths = randn(75 + i, E, T, H, D), A.ints([rows - 7 * e for e in range(E)])
+        want = torch.zeros_like(Q)
+        op_table().cache_attention(Q, cache, lengths, 0.1, want)
+        sets.append((torch.cuda.Stream(), cache, Q, lengths, torch.zeros_like(Q), want))
+    torch.cuda.synchronize()
+    for _ in range(100):
+        for stream, cache, Q, lengths, out, _ in sets:
+            with torch.cuda.stream(stream):
+                op_table().cache_attention(Q, cache, lengths, 0.1, out)
+    torch.cuda.synchronize()
+    for *_, out, want in sets:
+        assert torch.equal(out, want)

@@ -18,11 +18,16 @@ DEFAULT_FUSED_OPS = tuple(sorted(_cuda.FUSED_WRAPPERS))
 __all__ = ["BACKENDS", "DEFAULT_FUSED_OPS", "build_table"]
 
 
+def offered(module, kind: str) -> dict:
+    """`STAGES` or `OPERATORS` of a backend: none, where it has no such dict."""
+    return getattr(module, kind, {})
+
+
 def build_table(backend: str = "cuda", fused: bool = True) -> SimpleNamespace:
     """All call sites of one backend, with its fused overlays applied when `fused`."""
     module = BACKENDS[backend]
-    table = {**module.ALL_WRAPPERS, **module.OPERATORS}
+    table = {**module.ALL_WRAPPERS, **offered(module, "OPERATORS")}
     if fused:
         table.update(module.FUSED_WRAPPERS)
-        table.update(module.STAGES)
+        table.update(offered(module, "STAGES"))
     return SimpleNamespace(**table)

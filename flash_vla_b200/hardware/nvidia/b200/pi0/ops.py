@@ -10,7 +10,7 @@ from __future__ import annotations
 
 from types import SimpleNamespace
 
-from .backends import BACKENDS, build_table as _build_table
+from .backends import BACKENDS, build_table as _build_table, offered as _offered
 
 
 def op_table(fused: bool = True, backend: str = "cuda",
@@ -28,16 +28,16 @@ def op_table(fused: bool = True, backend: str = "cuda",
             table[name] = module.FUSED_WRAPPERS[name]
         elif name in module.ALL_WRAPPERS:
             table[name] = module.ALL_WRAPPERS[name]
-        elif name in module.OPERATORS:
+        elif name in _offered(module, "OPERATORS"):
             table[name] = module.OPERATORS[name]
     if fused and set(plan.values()) <= {backend}:      # a stage stands for ops of one backend only
-        table.update(BACKENDS[backend].STAGES)
+        table.update(_offered(BACKENDS[backend], "STAGES"))
     return SimpleNamespace(**table)
 
 
 def _op_names(backend: str) -> list[str]:
     module = BACKENDS[backend]
-    return sorted(set(module.ALL_WRAPPERS) | set(module.FUSED_WRAPPERS) | set(module.OPERATORS))
+    return sorted(set(module.ALL_WRAPPERS) | set(module.FUSED_WRAPPERS) | set(_offered(module, "OPERATORS")))
 
 
 def op_names(fused: bool = True, backend: str = "cuda") -> list[str]:

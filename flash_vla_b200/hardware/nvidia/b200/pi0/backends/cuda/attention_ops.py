@@ -195,8 +195,6 @@ def _attend(Q, K, V, cache, scale, out, causal, prefix, q_lens, k_lens, q_start,
         return out
     if S == 0:                                  # no key: documents of none have no address
         q_docs = k_docs = 0
-    if weights and o == q:
-        raise ValueError("attention: the weights are taken from Q, which out would overwrite")
     if weights and not lse:
         held = _scratch("attention_lse", 4 * E * H * T, Q.device)
         lse = held.data_ptr()
@@ -231,7 +229,7 @@ def cache_attention(Q, cache, lengths, scale, out, causal=False, prefix=None, q_
     q_start (E,): position of each episode's first query, by default lengths - q_lens. k_pos (E, rows): position of each cached row, by default its
     number; a cache that `cache_evict` has thinned out needs both for `causal`, `prefix` (then positions below `prefix`) and `slopes`.
     weights (E, rows) fp32: weights = decay * weights + the probability mass that each row received from all queries and heads; rows
-    behind `lengths` stay as they were. decay = 0 overwrites. `out` may be Q, unless weights are asked for."""
+    behind `lengths` stay as they were. decay = 0 overwrites. `out` may be Q."""
     return _attend(Q, None, None, cache, scale, out, causal, prefix, q_lens, lengths, q_start, None, None, k_pos, cap, slopes, lse, weights, decay)
 
 

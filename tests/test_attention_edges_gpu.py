@@ -165,3 +165,14 @@ def test_clusters_of_two_streams_share_the_tensor_memory():
     torch.cuda.synchronize()
     for *_, out, want in sets:
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("T,rows", [(1, 4096), (1, 12800), (51, 832)])
+def test_weights_where_the_result_replaces_the_queries(T, rows):
+    cache = cache_of(randn(81, 2, rows, 1, 256), randn(82, 2, rows, 1, 256))
+    Q, lengths = randn(83, 2, T, 8, 256), A.ints([rows, rows - 100])
+    out, w = torch.zeros_like(Q), torch.zeros(2, rows, device="cuda")
+    op_table().cache_attention(Q, cache, lengths, 0.06, out, weights=w)
+    again = torch.zeros_like(w)
+    op_table().cache_attention(Q, cache, lengths, 0.06, Q, weights=again)
+    assert torch.equal(Q, out) and torch.equal(w, again)

@@ -393,6 +393,23 @@ inline int launch_tile(const Tile& p, const CUtensorMap& tmQ, const CUtensorMap&
     return rc || p.splits == 1 ? rc : launch_join(p, HDP, st);
 }
 
+inline int launch_weights(const Tile& p, cudaStream_t st) {
+    const Args& a = p.a;
+    cudaError_t e;
+    if (takes_few(a)) {
+        // a warp for up to 16 rows, sixteen for the most: eight rows or more for each; CTAs of four warps at least
+        const int rows_each = a.tokens * a.heads;
+        int share = 1;
+        while (share < WEIGHT_WARPS && rows_each > 16 * share) share *= 2;
+        const int all = share < 4 ? 4 : share, keys_each = 32 * (all / share);
+        e = launch_pdl(key_weights_kernel, dim3((a.keys + keys_each - 1) / keys_each, a.episodes), dim3(32 * all), 0, st, p, share);
+    } else {
+        e = launch_pdl(tile_weights_kernel, dim3(2 * p.key_blocks, a.episodes), dim3(32 * WEIGHT_WARPS), 0, st, p);
+    }
+    if (e != cudaSuccess) { set_error("key_weights_kernel: %s", cudaGetErrorString(e)); return FVLA_ERR_LAUNCH; }
+    return check_launch("key_weights_kernel");
+}
+
 inline int launch_attention(const Args& a, void* ws, int* status, cudaStream_t st) {
     Tile p;
     p.a = a;
@@ -471,20 +488,14 @@ inline int launch_attention(const Args& a, void* ws, int* status, cudaStream_t s
     } else {
         rc = hdp == 64 ? launch_tile<64, false>(p, tmQ, tmK, tmV, tmO, st) : (hdp == 128 ? launch_tile<128, false>(p, tmQ, tmK, tmV, tmO, st) : launch_tile<256, false>(p, tmQ, tmK, tmV, tmO, st));
     }
-    if (rc || a.weights == nullptr || a.keys == 0) return rc;
-    cudaError_t e;
-    if (few) {
-        // a warp for up to 16 rows, sixteen for the most: eight rows or more for each; CTAs of four warps at least
-        const int rows_each = a.tokens * a.heads;
-        int share = 1;
-        while (share < WEIGHT_WARPS && rows_each > 16 * share) share *= 2;
-        const int all = share < 4 ? 4 : share, keys_each = 32 * (all / share);
-        e = launch_pdl(key_weights_kernel, dim3((a.keys + keys_each - 1) / keys_each, a.episodes), dim3(32 * all), 0, st, p, share);
-    } else {
-        e = launch_pdl(tile_weights_kernel, dim3(2 * blocks, a.episodes), dim3(32 * WEIGHT_WARPS), 0, st, p);
-    }
-    if (e != cudaSuccess) { set_error("key_weights_kernel: %s", cudaGetErrorString(e)); return FVLA_ERR_LAUNCH; }
-    return check_launch("key_weights_kernel");
+    return rc || a.weights == nullptr || a.keys == 0 ? rc : launch_weights(p, st);
+}
+
+// The decay of the weights alone, where there is no query.
+inline int launch_weights(const Args& a, cudaStream_t st) {
+    Tile p = {};
+    p.a = a;
+    return a.keys == 0 ? FVLA_OK : launch_weights(p, st);
 }
 
 }  // namespace mattn

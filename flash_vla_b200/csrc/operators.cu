@@ -28,25 +28,26 @@ static bool strides_ok(const long long (&s)[3], int multiple) { return s[0] % mu
 
 static int check_attention(const struct fvla_attention* a) {
     FVLA_REQUIRE(a != nullptr, "attention: null arguments");
-    FVLA_REQUIRE(a->episodes > 0 && a->tokens > 0 && a->keys >= 0 && a->heads > 0 && a->kv_heads > 0, "attention: empty shape");
+    const bool decay = a->tokens == 0 && a->weights != nullptr;            // no query: the weights decay, and nothing else is written
+    FVLA_REQUIRE(a->episodes > 0 && (a->tokens > 0 || decay) && a->keys >= 0 && a->heads > 0 && a->kv_heads > 0, "attention: empty shape");
     FVLA_REQUIRE(a->heads % a->kv_heads == 0 && a->heads / a->kv_heads <= 128, "attention: %d heads over %d K/V heads", a->heads, a->kv_heads);
     const bool q8 = a->k_scale != nullptr;
     const int multiple = q8 ? 16 : 8;
     FVLA_REQUIRE(a->head_dim > 0 && a->head_dim <= 256 && a->head_dim % multiple == 0, "attention: head_dim %d (a multiple of %d up to 256)", a->head_dim, multiple);
-    FVLA_REQUIRE(a->q != nullptr && a->out != nullptr && (a->keys == 0 || (a->k != nullptr && a->v != nullptr)), "attention: null pointer");
+    FVLA_REQUIRE((decay || (a->q != nullptr && a->out != nullptr)) && (a->keys == 0 || (a->k != nullptr && a->v != nullptr)), "attention: null pointer");
     FVLA_REQUIRE((a->v_scale != nullptr) == q8, "attention: scales of both K and V, or of neither");
     FVLA_REQUIRE(aligned16(a->q) && aligned16(a->k) && aligned16(a->v) && aligned16(a->out), "attention: every tensor must be 16-byte aligned");
     FVLA_REQUIRE(strides_ok(a->q_stride, 8) && strides_ok(a->out_stride, 8) && strides_ok(a->k_stride, multiple) && strides_ok(a->v_stride, multiple),
                  "attention: every row must start on 16 bytes");
-    FVLA_REQUIRE((a->tokens == 1 || a->q_stride[1] > 0) && (a->heads == 1 || a->q_stride[2] > 0) && (a->keys <= 1 || (a->k_stride[1] > 0 && a->v_stride[1] > 0)),
+    FVLA_REQUIRE((a->tokens <= 1 || a->q_stride[1] > 0) && (a->heads == 1 || a->q_stride[2] > 0) && (a->keys <= 1 || (a->k_stride[1] > 0 && a->v_stride[1] > 0)),
                  "attention: tokens or query heads that share their memory");
-    FVLA_REQUIRE((a->episodes == 1 || a->out_stride[0] > 0) && (a->tokens == 1 || a->out_stride[1] > 0) && (a->heads == 1 || a->out_stride[2] > 0),
+    FVLA_REQUIRE((a->episodes == 1 || a->out_stride[0] > 0) && (a->tokens <= 1 || a->out_stride[1] > 0) && (a->heads == 1 || a->out_stride[2] > 0),
                  "attention: rows of the result that share their memory");
     for (int i = 0; i < 3; ++i) FVLA_REQUIRE(a->q_stride[i] >= 0 && a->k_stride[i] >= 0 && a->v_stride[i] >= 0 && a->out_stride[i] >= 0, "attention: negative strides");
     FVLA_REQUIRE(!q8 || (block_ok(a->block) && a->keys % a->block == 0), "attention: blocks of %d rows in %d", a->block, a->keys);
     FVLA_REQUIRE((a->q_docs != nullptr) == (a->k_docs != nullptr), "attention: documents of queries and keys, or of neither");
     FVLA_REQUIRE(a->prefix == nullptr || a->causal, "attention: a prefix without the causal mask");
-    FVLA_REQUIRE(a->weights == nullptr || (a->lse != nullptr && q8), "attention: weights need the 8-bit cache and the log-sum-exp");
+    FVLA_REQUIRE(a->weights == nullptr || ((a->lse != nullptr || decay) && q8), "attention: weights need the 8-bit cache and the log-sum-exp");
     FVLA_REQUIRE(a->cap >= 0.f && a->scale == a->scale, "attention: scale and cap");
     FVLA_REQUIRE((long long)a->tokens * a->heads < (1ll << 31) && (long long)a->episodes * a->tokens * a->heads < (1ll << 31) && (long long)a->episodes * a->kv_heads < 65536, "attention: too many rows");
     FVLA_REQUIRE(((long long)a->tokens / (128 / (a->heads / a->kv_heads)) + 1) * a->kv_heads * a->episodes < (1ll << 30), "attention: too many rows");
@@ -80,6 +81,7 @@ int fvla_attention_run(const struct fvla_attention* a, void* stream) {
     int rc = check_attention(a);
     if (rc) return rc;
     const mattn::Args p = attention_args(a);
+    if (a->tokens == 0) return mattn::launch_weights(p, S(stream));
     const size_t need = mattn::workspace_bytes(p);
     if (need > 0 && (a->ws == nullptr || a->ws_bytes < need)) { set_error("attention: workspace of %zu bytes needed", need); return FVLA_ERR_WORKSPACE; }
     FVLA_REQUIRE(aligned16(a->ws), "attention: the workspace must be 16-byte aligned");

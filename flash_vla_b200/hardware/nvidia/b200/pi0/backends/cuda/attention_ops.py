@@ -191,11 +191,11 @@ def _attend(Q, K, V, cache, scale, out, causal, prefix, q_lens, k_lens, q_start,
     if cache is not None:
         K_scale, V_scale = _vector("cache.K_scale", K_scale, K_scale.shape, _F32, device), _vector("cache.V_scale", V_scale, V_scale.shape, _F32, device)
     q, k, v, o = _address("Q", Q, device), _address("K", K, device), _address("V", V, device), _address("out", out, device)
-    if E == 0 or T == 0:
+    if E == 0 or (T == 0 and not weights):      # (without queries the weights still decay)
         return out
     if S == 0:                                  # no key: documents of none have no address
         q_docs = k_docs = 0
-    if weights and not lse:
+    if weights and not lse and T:
         held = _scratch("attention_lse", 4 * E * H * T, Q.device)
         lse = held.data_ptr()
     need = nbytes[1 if q_docs or weights else 0]

@@ -176,3 +176,16 @@ def test_weights_where_the_result_replaces_the_queries(T, rows):
     again = torch.zeros_like(w)
     op_table().cache_attention(Q, cache, lengths, 0.06, Q, weights=again)
     assert torch.equal(Q, out) and torch.equal(w, again)
+
+
+def test_weights_decay_without_a_query():
+    """No token at all, as for a batch whose episodes all wait: the weights decay as with no query of an episode's own."""
+    cache, w = cache_of(randn(91, 2, 256, 1, 64), randn(92, 2, 256, 1, 64)), torch.full((2, 256), 2.0, device="cuda")
+    none = torch.empty(2, 0, 8, 64, dtype=bf16, device="cuda")
+    op_table().cache_attention(none, cache, A.ints([256, 100]), 0.1, none.clone(), weights=w, decay=0.25)
+    assert (w[0] == 0.5).all() and (w[1, :100] == 0.5).all() and (w[1, 100:] == 2).all()
+    w[1, 40] = NAN
+    op_table().cache_attention(none, cache, A.ints([0, 50]), 0.1, none.clone(), weights=w, decay=0.0, lse=torch.empty(2, 8, 0, device="cuda"))
+    assert (w[0] == 0.5).all() and (w[1, :50] == 0).all() and (w[1, 50:100] == 0.5).all()
+    op_table().cache_attention(none, cache, A.ints([256, 256]), 0.1, none.clone())
+    op_table().masked_attention(none, randn(93, 2, 5, 1, 64), randn(94, 2, 5, 1, 64), 0.1, none.clone())

@@ -17,6 +17,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import operator
 import struct
 
 import torch
@@ -67,6 +68,27 @@ def _cache_shapes(name, shapes, strides, dtypes):
     if k[3] % 16 or not 0 < k[3] <= 256:
         raise ValueError(f"{name}: head_dim {k[3]} (a multiple of 16 up to 256)")
     return k[1] // ks[1]
+
+
+def _footprint(shape, stride, size):
+    """(bytes from an operand's first to behind its last, bytes of a row, (elements, bytes apart) of the axes before the last)"""
+    if 0 in shape:
+        return 0, 0, ()
+    axes = tuple((n, s * size) for n, s in zip(shape[:-1], stride[:-1]) if n > 1 and s)
+    return sum((n - 1) * s for n, s in axes) + shape[-1] * size, shape[-1] * size, axes
+
+
+def _apart(p, a, q, b):
+    """Whether operands of the footprints a and b at p and q share no byte. Ones that interleave (K and V of one tensor, layers of a stack) do so with some
+    axis' stride as their period: each then has a part of it of its own."""
+    if p + a[0] <= q or q + b[0] <= p:
+        return True
+    for period in {s for f in (a, b) for _, s in f[2]}:
+        inner_a, inner_b = (f[1] + sum((n - 1) * s for n, s in f[2] if s % period) for f in (a, b))
+        ahead = (q - p) % period
+        if inner_a <= ahead and ahead + inner_b <= period:
+            return True
+    return False
 
 
 def _layout(t):
@@ -289,9 +311,17 @@ def _evict_plan(cache, out, keep, sinks, recent):
     if E >= 1 << 16 or rows >= 1 << 31 or HK == 0:
         raise ValueError(f"cache_evict: a cache of {tuple(cache[0][0])}")
     a.episodes, a.rows, a.out_rows, a.kv_heads, a.head_dim, a.keep, a.sinks, a.recent = E, rows, out_rows, HK, D, keep, sinks, recent
-    extent = lambda layout, i: 1 + sum((n - 1) * st for n, st in zip(layout[0][i], layout[1][i]))      # noqa: E731  bytes of an 8-bit operand
     return (_between(a, "k_stride", None), _lib.load().fvla_cache_evict_workspace_bytes(E, keep), E, rows, out_rows,
-            (extent(cache, 0), extent(cache, 1), extent(out, 0), extent(out, 1)))
+            tuple(_footprint(layout[0][i], layout[1][i], 1) for layout in (cache, out) for i in (0, 1)))
+
+
+_first = operator.itemgetter(0)
+
+
+def _all_apart(spans):
+    """Whether no destination among these spans shares a byte with another one of them."""
+    spans = [(p, whole or (last - p, last - p, ()), out) for p, last, out, whole in spans if last > p]
+    return all(_apart(p, a, q, b) for i, (p, a, out) in enumerate(spans) for q, b, other in spans[:i] if out or other)
 
 
 def cache_evict(cache, lengths, weights, keep, out_cache, out_lengths, out_weights=None, positions=None, out_positions=None, sinks=0, recent=0):
@@ -303,7 +333,7 @@ def cache_evict(cache, lengths, weights, keep, out_cache, out_lengths, out_weigh
     scale is the largest among its rows', and values are rounded again where theirs was smaller. What lies behind the last row stays as it was."""
     held_k, held_v, k_scale, v_scale = cache
     to_k, to_v, to_k_scale, to_v_scale = out_cache
-    rest, nbytes, E, rows, out_rows, extents = _evict_plan(_cache_layout(cache), _cache_layout(out_cache), int(keep), int(sinks), int(recent))
+    rest, nbytes, E, rows, out_rows, footprints = _evict_plan(_cache_layout(cache), _cache_layout(out_cache), int(keep), int(sinks), int(recent))
     device = _device()
     n, out_n = _vector("lengths", lengths, (E,), _INT32, device), _vector("out_lengths", out_lengths, (E,), _INT32, device)
     w = _vector("weights", weights, (E, rows), _F32, device)
@@ -317,16 +347,16 @@ def cache_evict(cache, lengths, weights, keep, out_cache, out_lengths, out_weigh
     to_k, to_v = _address("out_cache.K", to_k, device), _address("out_cache.V", to_v, device)
     if E == 0:
         return
-    # (first byte, byte behind the last, a destination)
-    small, large = 4 * k_scale.numel(), 4 * to_k_scale.numel()
-    spans = [(n, n + 4 * E, 0), (w, w + 4 * E * rows, 0), (pos, pos + 4 * E * rows if pos else 0, 0), (ks, ks + small, 0), (vs, vs + small, 0), (k, k + extents[0], 0),
-             (v, v + extents[1], 0), (out_n, out_n + 4 * E, 1), (out_w, out_w + 4 * E * out_rows if out_w else 0, 1),
-             (out_pos, out_pos + 4 * E * out_rows if out_pos else 0, 1), (to_ks, to_ks + large, 1), (to_vs, to_vs + large, 1), (to_k, to_k + extents[2], 1),
-             (to_v, to_v + extents[3], 1)]
-    spans.sort()
+    # (first byte, byte behind the last, a destination, footprint where it is not whole)
+    small, large, (fk, fv, to_fk, to_fv) = 4 * k_scale.numel(), 4 * to_k_scale.numel(), footprints
+    spans = [(n, n + 4 * E, 0, None), (w, w + 4 * E * rows, 0, None), (pos, pos + 4 * E * rows if pos else 0, 0, None), (ks, ks + small, 0, None), (vs, vs + small, 0, None),
+             (k, k + fk[0], 0, fk), (v, v + fv[0], 0, fv), (out_n, out_n + 4 * E, 1, None), (out_w, out_w + 4 * E * out_rows if out_w else 0, 1, None),
+             (out_pos, out_pos + 4 * E * out_rows if out_pos else 0, 1, None), (to_ks, to_ks + large, 1, None), (to_vs, to_vs + large, 1, None), (to_k, to_k + to_fk[0], 1, to_fk),
+             (to_v, to_v + to_fv[0], 1, to_fv)]
+    spans.sort(key=_first)
     read = written = 0                          # how far the operands so far reach
-    for first, last, out in spans:
-        if first < written or (out and first < read):
+    for first, last, out, _ in spans:
+        if (first < written or (out and first < read)) and not _all_apart(spans):
             raise ValueError("cache_evict: a destination lies over another operand")
         if out:
             written = last if last > written else written

@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes
+import random
 from types import SimpleNamespace
 
 import pytest
@@ -9,7 +10,7 @@ import torch
 
 from flash_vla_b200 import op_table
 from flash_vla_b200.hardware.nvidia.b200.pi0 import backends
-from flash_vla_b200.hardware.nvidia.b200.pi0.backends.cuda import _lib
+from flash_vla_b200.hardware.nvidia.b200.pi0.backends.cuda import _lib, attention_ops
 from flash_vla_b200.hardware.nvidia.b200.pi0.buffers import allocate_quantized_cache
 
 bf16, f32, i32 = torch.bfloat16, torch.float32, torch.int32
@@ -42,3 +43,30 @@ def test_the_entry_takes_no_tokens_only_with_weights():
     assert lib.fvla_attention_run(ctypes.byref(a), None) == -1 and b"null" in lib.fvla_last_error()
     a.tokens, a.q, a.lse = 1, P, None
     assert lib.fvla_attention_run(ctypes.byref(a), None) == -1 and b"log-sum-exp" in lib.fvla_last_error()
+
+
+def test_operands_that_interleave_are_apart_and_others_are_not():
+    """Against the bytes themselves."""
+    rng = random.Random(3)
+    seen = {True: 0, False: 0}
+    for _ in range(4000):
+        def operand():
+            shape = [rng.choice((1, 1, 2, 3)) for _ in range(3)] + [rng.choice((1, 2, 4))]
+            order, stride, reach = rng.sample(range(3), 3), [0] * 3 + [1], shape[3]
+            for axis in order:
+                stride[axis] = reach * rng.choice((1, 2, 3)) if rng.random() < 0.9 else 0
+                reach = max(reach, stride[axis] * shape[axis])
+            size = rng.choice((1, 2))
+            p = rng.randrange(0, 60)
+            at = {p + size * (i * stride[0] + j * stride[1] + k * stride[2] + d) + b for i in range(shape[0]) for j in range(shape[1]) for k in range(shape[2])
+                  for d in range(shape[3]) for b in range(size)}
+            return p, attention_ops._footprint(tuple(shape), tuple(stride), size), at
+        (p, a, x), (q, b, y) = operand(), operand()
+        assert a[0] == max(x) + 1 - p
+        apart = attention_ops._apart(p, a, q, b)
+        assert not (apart and x & y) and apart == attention_ops._apart(q, b, p, a)
+        seen[apart] += 1
+    assert min(seen.values()) > 500
+    kv = attention_ops._footprint((2, 5, 3, 8), (2 * 5 * 3 * 8, 2 * 3 * 8, 8, 1), 2)               # rows of (K, V)
+    assert attention_ops._apart(0, kv, 3 * 8 * 2, kv) and not attention_ops._apart(0, kv, 3 * 8 * 2 - 2, kv)
+    assert attention_ops._footprint((2, 0, 3, 8), (24, 24, 8, 1), 2) == (0, 0, ())

@@ -189,3 +189,46 @@ def test_weights_decay_without_a_query():
     assert (w[0] == 0.5).all() and (w[1, :50] == 0).all() and (w[1, 50:100] == 0.5).all()
     op_table().cache_attention(none, cache, A.ints([256, 256]), 0.1, none.clone())
     op_table().masked_attention(none, randn(93, 2, 5, 1, 64), randn(94, 2, 5, 1, 64), 0.1, none.clone())
+
+
+@pytest.mark.parametrize("layout", ["rows of K and V", "heads of K and V", "layers"])
+def test_evict_between_interleaved_tensors(layout):
+    """K and V of a cache as views of one tensor, and the source and the destination as two layers of one stack: what goes where is the same as between whole tensors."""
+    E, rows, HK, D, keep = 2, 256, 2, 64, 100
+
+    def views(n):
+        if layout == "rows of K and V":
+            t = torch.zeros(E, n, 2, HK, D, dtype=torch.uint8, device="cuda").view(e4m3)
+            return t[:, :, 0], t[:, :, 1], t
+        if layout == "heads of K and V":
+            t = torch.zeros(E, n, HK, 2, D, dtype=torch.uint8, device="cuda").view(e4m3)
+            return t[:, :, :, 0], t[:, :, :, 1], t
+        t = torch.zeros(2, E, 3, n, HK, D, dtype=torch.uint8, device="cuda").view(e4m3)
+        return t[0, :, 1], t[1, :, 1], t
+
+    K, V = randn(95, E, rows, HK, D), randn(96, E, rows, HK, D)
+    whole = cache_of(K, V)
+    k, v, _ = views(rows)
+    cache = QuantizedCache(k, v, *(torch.ones(E, rows // 64, HK, device="cuda") for _ in range(2)))
+    op_table().cache_append(K, V, cache, A.ints([0] * E))
+    w = randn(97, E, rows, dtype=f32)
+    k, v, _ = views(128)
+    out = QuantizedCache(k, v, *(torch.ones(E, 2, HK, device="cuda") for _ in range(2)))
+    want, n, m = allocate_quantized_cache(E, 128, HK, D, "cuda"), A.ints([0, 0]), A.ints([0, 0])
+    op_table().cache_evict(whole, A.ints([256, 90]), w, keep, want, n)
+    op_table().cache_evict(cache, A.ints([256, 90]), w, keep, out, m)
+    assert torch.equal(n, m)
+    for a, b in zip(out, want):
+        assert A.same_bits(a.contiguous(), b)
+    if layout == "layers":                                                     # from one layer to the next
+        store = [torch.zeros(E, 3, rows, HK, D, dtype=torch.uint8, device="cuda").view(e4m3) for _ in range(2)]
+        src = QuantizedCache(store[0][:, 0], store[1][:, 0], *(s.clone() for s in whole[2:]))
+        dst = QuantizedCache(store[0][:, 1], store[1][:, 1], *(torch.ones(E, 4, HK, device="cuda") for _ in range(2)))
+        for held, full in zip(src[:2], whole[:2]):
+            held.view(torch.uint8).copy_(full.view(torch.uint8))
+        op_table().cache_evict(src, A.ints([256, 90]), w, keep, dst, m)
+        for a, b in zip(dst[:2], want[:2]):
+            assert A.same_bits(a[:, :keep].contiguous()[0], b[0, :keep]) and A.same_bits(a[1, :90].contiguous(), b[1, :90])
+    with pytest.raises(ValueError, match="lies over"):                         # one row on: the source's rows in the destination
+        t = torch.zeros(E, rows + 128, HK, D, dtype=torch.uint8, device="cuda").view(e4m3)
+        op_table().cache_evict(whole._replace(K=t[:, :rows]), A.ints([256, 90]), w, keep, want._replace(K=t[:, rows - 1:rows + 127]), m)

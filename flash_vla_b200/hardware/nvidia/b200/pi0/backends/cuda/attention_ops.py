@@ -31,7 +31,7 @@ _INT32, _F32 = torch.int32, torch.float32
 
 def _rows(name, shape, stride, dtype, want, multiple, shared=()):
     """Element strides (episode, token, head) of a 4-D operand; an axis of one element gets a stride that any layout may have. `shared`: axes whose
-    elements may share their memory (stride 0)."""
+    elements may share their memory (stride 0); where there is none the operand is written, and no two of its rows may overlap."""
     if dtype != want:
         raise ValueError(f"{name}: expected {want}, got {dtype}")
     if len(shape) != 4:
@@ -47,6 +47,11 @@ def _rows(name, shape, stride, dtype, want, multiple, shared=()):
         if s == 0 and axis not in shared:
             raise ValueError(f"{name}: rows that share memory, strides {tuple(stride)}")
         out.append(s)
+    reach = shape[3]
+    for s, n in () if shared else sorted((s, n) for s, n in zip(stride[:3], shape[:3]) if n > 1):
+        if s < reach:
+            raise ValueError(f"{name}: rows that share memory, shape {tuple(shape)}, strides {tuple(stride)}")
+        reach += s * (n - 1)
     return out
 
 
@@ -116,7 +121,7 @@ def _between(block, first, last):
 @functools.lru_cache(maxsize=1024)
 def _attention_plan(q, k, v, out, cache):
     """What operands of these layouts determine of an attention's argument block: (strides, dimensions, scratch bytes without and with documents or
-    weights, episodes, tokens, keys, heads). `cache`: layout of a QuantizedCache, or None."""
+    weights, episodes, tokens, keys, heads, footprints of Q, K, V and out, whether out in Q's place has its rows). `cache`: layout of a QuantizedCache, or None."""
     a = _lib.Attention()
     if cache is None:
         multiple, want, dim_multiple = 8, torch.bfloat16, 8
@@ -145,7 +150,10 @@ def _attention_plan(q, k, v, out, cache):
             setattr(b, name, 16)                # an address that only says that there is a tensor
         if E and T:
             nbytes[i] = _lib.load().fvla_attention_workspace_bytes(ctypes.byref(b))
-    return _between(a, "q_stride", "scale"), _between(a, "episodes", "causal"), nbytes, E, T, S, H
+    held = 2 if cache is None else 1
+    footprints = _footprint(q[0], q[1], 2), _footprint(k[0], k[1], held), _footprint(v[0], v[1], held), _footprint(out[0], out[1], 2)
+    same = all(n <= 1 or s == o for n, s, o in zip(q[0], q[1], out[1]))
+    return _between(a, "q_stride", "scale"), _between(a, "episodes", "causal"), nbytes, E, T, S, H, footprints, same
 
 
 def _vector(name, t, shape, dtype, device):
@@ -161,13 +169,21 @@ def _vector(name, t, shape, dtype, device):
     raise ValueError(f"{name}: expected a tensor on the current CUDA device, got {t.device}")
 
 
+def _misplaced(device, **operands):
+    """Says which of four operands, whose layouts have been checked, is not on this device or not aligned."""
+    for name, t in operands.items():
+        name = name.replace("cache_", "cache.")
+        if t.get_device() != device:
+            raise ValueError(f"{name}: expected a CUDA tensor on the current device, got {t.device}")
+        if t.data_ptr() & 15:
+            raise ValueError(f"{name}: expected 16-byte alignment")
+
+
 def _address(name, t, device):
     """Address of an operand whose layout has been checked."""
-    if t.get_device() != device:
-        raise ValueError(f"{name}: expected a CUDA tensor on the current device, got {t.device}")
     p = t.data_ptr()
-    if p & 15:
-        raise ValueError(f"{name}: expected 16-byte alignment")
+    if p & 15 or t.get_device() != device:
+        _misplaced(device, **{name: t})
     return p
 
 
@@ -191,7 +207,7 @@ def _attend(Q, K, V, cache, scale, out, causal, prefix, q_lens, k_lens, q_start,
     else:
         K, V, K_scale, V_scale = cache
         plan = _attention_plan(_layout(Q), None, None, _layout(out), _cache_layout(cache))
-    strides, dims, nbytes, E, T, S, H = plan
+    strides, dims, nbytes, E, T, S, H, (fq, fk, fv, fo), same = plan
     scale, cap, decay = float(scale), float(cap or 0.0), float(decay)
     if not math.isfinite(scale) or not (0.0 <= cap < math.inf) or not math.isfinite(decay):
         raise ValueError(f"attention: scale {scale}, cap {cap}, decay {decay}: finite numbers, the cap not negative")
@@ -199,6 +215,11 @@ def _attend(Q, K, V, cache, scale, out, causal, prefix, q_lens, k_lens, q_start,
         raise ValueError("attention: a prefix without the causal mask")
     if (q_docs is None) != (k_docs is None):
         raise ValueError("attention: documents of queries and keys, or of neither")
+    q, k, v, o = Q.data_ptr(), K.data_ptr(), V.data_ptr(), out.data_ptr()
+    last = o + fo[0]
+    if (o < q + fq[0] and q < last and not (o == q and same) and not _apart(o, fo, q, fq)) or (o < k + fk[0] and k < last and not _apart(o, fo, k, fk)) or \
+            (o < v + fv[0] and v < last and not _apart(o, fo, v, fv)):
+        raise ValueError("attention: out lies over Q, K or V")
     device = _device()
     prefix = 0 if prefix is None else _vector("prefix", prefix, (E,), _INT32, device)
     q_lens = 0 if q_lens is None else _vector("q_lens", q_lens, (E,), _INT32, device)
@@ -212,7 +233,8 @@ def _attend(Q, K, V, cache, scale, out, causal, prefix, q_lens, k_lens, q_start,
     weights = 0 if weights is None else _vector("weights", weights, (E, S), _F32, device)
     if cache is not None:
         K_scale, V_scale = _vector("cache.K_scale", K_scale, K_scale.shape, _F32, device), _vector("cache.V_scale", V_scale, V_scale.shape, _F32, device)
-    q, k, v, o = _address("Q", Q, device), _address("K", K, device), _address("V", V, device), _address("out", out, device)
+    if (q | k | v | o) & 15 or not Q.get_device() == K.get_device() == V.get_device() == out.get_device() == device:
+        _misplaced(device, Q=Q, K=K, V=V, out=out)
     if E == 0 or (T == 0 and not weights):      # (without queries the weights still decay)
         return out
     if S == 0:                                  # no key: documents of none have no address
@@ -232,7 +254,8 @@ def masked_attention(Q, K, V, scale, out, causal=False, prefix=None, q_lens=None
                      lse=None):
     """out = softmax(bias(cap(scale * Q K^T))) V over the keys that each query sees.
 
-    Q, out (E, T, H, D); K, V (E, S, HK, D), H a multiple of HK; bf16, D a multiple of 8 up to 256. `out` may be Q.
+    Q, out (E, T, H, D); K, V (E, S, HK, D), H a multiple of HK; bf16, D a multiple of 8 up to 256. `out` may be Q, row by
+    row, and otherwise overlaps neither Q nor K nor V.
     cap > 0: scores become cap * tanh(score / cap). slopes (H,) fp32: slope * |distance| is taken off them.
     k_lens, q_lens (E,): keys and queries of each episode, all by default; rows of `out` (and of `lse`) behind q_lens stay as they were. The queries are the
     last tokens of their episode: token t stands at k_lens - q_lens + t.
@@ -272,7 +295,7 @@ def _append_plan(k, v, cache):
     if E >= 1 << 16 or rows >= 1 << 31 or HK == 0:
         raise ValueError(f"cache_append: a cache of {tuple(cache[0][0])}")
     a.episodes, a.tokens, a.rows, a.kv_heads, a.head_dim = E, T, rows, HK, D
-    return _between(a, "k_stride", None), E, T
+    return _between(a, "k_stride", None), E, T, _footprint(cache[0][0], cache[1][0], 1), _footprint(cache[0][1], cache[1][1], 1)
 
 
 def cache_append(K, V, cache, starts, counts=None):
@@ -282,13 +305,18 @@ def cache_append(K, V, cache, starts, counts=None):
     block holds rows before starts[e]; where it has grown, those rows are moved to it. Rows behind the new ones are taken to be unused. Values
     that are not finite become NaN and leave the scale alone. Rows that would lie outside the cache are left out (device status 8)."""
     held_k, held_v, k_scale, v_scale = cache
-    rest, E, T = _append_plan(_layout(K), _layout(V), _cache_layout(cache))
+    rest, E, T, fk, fv = _append_plan(_layout(K), _layout(V), _cache_layout(cache))
+    to_k, to_v = held_k.data_ptr(), held_v.data_ptr()
+    if (to_k < to_v + fv[0] and to_v < to_k + fk[0] and not _apart(to_k, fk, to_v, fv)) or abs(k_scale.data_ptr() - v_scale.data_ptr()) < 4 * k_scale.numel():
+        raise ValueError("cache_append: K and V of the cache share memory")
     device = _device()
     starts = _vector("starts", starts, (E,), _INT32, device)
     counts = 0 if counts is None else _vector("counts", counts, (E,), _INT32, device)
     k_scale, v_scale = _vector("cache.K_scale", k_scale, k_scale.shape, _F32, device), _vector("cache.V_scale", v_scale, v_scale.shape, _F32, device)
-    block = _APPEND_HEAD.pack(_address("K", K, device), _address("V", V, device), _address("cache.K", held_k, device), _address("cache.V", held_v, device),
-                              k_scale, v_scale, starts, counts) + rest
+    k, v = K.data_ptr(), V.data_ptr()
+    if (k | v | to_k | to_v) & 15 or not K.get_device() == V.get_device() == held_k.get_device() == held_v.get_device() == device:
+        _misplaced(device, K=K, V=V, cache_K=held_k, cache_V=held_v)
+    block = _APPEND_HEAD.pack(k, v, to_k, to_v, k_scale, v_scale, starts, counts) + rest
     if E and T:
         _lib.call("fvla_cache_append", block, torch._C._cuda_getCurrentRawStream(device))
 

@@ -70,3 +70,47 @@ def test_operands_that_interleave_are_apart_and_others_are_not():
     kv = attention_ops._footprint((2, 5, 3, 8), (2 * 5 * 3 * 8, 2 * 3 * 8, 8, 1), 2)               # rows of (K, V)
     assert attention_ops._apart(0, kv, 3 * 8 * 2, kv) and not attention_ops._apart(0, kv, 3 * 8 * 2 - 2, kv)
     assert attention_ops._footprint((2, 0, 3, 8), (24, 24, 8, 1), 2) == (0, 0, ())
+
+
+def test_attention_refuses_a_result_over_what_it_reads():
+    call = op_table().masked_attention
+    store = z(1 << 16)
+
+    def at(first, *shape, strides=None):
+        dense = [shape[1] * shape[2] * shape[3], shape[2] * shape[3], shape[3], 1]
+        return store.as_strided(shape, strides or dense, first)
+    Q, K, V = at(0, 2, 3, 4, 64), at(4096, 2, 5, 2, 64), at(8192, 2, 5, 2, 64)
+    for out in (at(64, 2, 3, 4, 64), at(0, 2, 3, 4, 64, strides=[64 * 4 * 3, 64, 64 * 3, 1]), at(4096 + 64, 2, 3, 4, 64), at(8192 - 8, 2, 3, 4, 64)):
+        with pytest.raises(ValueError, match="lies over"):
+            call(Q, K, V, 0.1, out)
+    with pytest.raises(ValueError, match="lies over"):                  # one Q for two episodes, in place of its first
+        call(Q[:1].expand(2, 3, 4, 64), K, V, 0.1, Q)
+    for out in (Q, at(16384, 2, 3, 4, 64)):                             # (as far as a machine without a GPU goes)
+        with pytest.raises(ValueError, match="CUDA"):
+            call(Q, K, V, 0.1, out)
+    qkv = store[:2 * 3 * 8 * 64].view(2, 3, 8, 64)
+    with pytest.raises(ValueError, match="CUDA"):                       # Q, K and V as parts of one projection's rows
+        call(qkv[:, :, :4], qkv[:, :, 4:6], qkv[:, :, 6:], 0.1, qkv[:, :, :4])
+    held = store.view(torch.uint8).view(torch.float8_e4m3fn)[:128 * 64].view(1, 64, 2, 64)
+    c = allocate_quantized_cache(1, 64, 2, 64, "cpu")._replace(V=held)
+    with pytest.raises(ValueError, match="lies over"):
+        op_table().cache_attention(at(8192, 1, 3, 4, 64), c, z(1, dtype=i32), 0.1, at(2048, 1, 3, 4, 64))
+
+
+def test_rows_of_a_result_may_not_overlap():
+    store, Q, K = z(1 << 14), z(2, 3, 4, 64), z(2, 5, 2, 64)
+    for strides in ((768, 256, 32, 1), (768, 128, 64, 1), (512, 256, 64, 1), (64, 256, 128, 1)):
+        with pytest.raises(ValueError, match="share memory"):
+            op_table().masked_attention(Q, K, K, 0.1, store.as_strided((2, 3, 4, 64), strides))
+    for strides in ((768, 64, 192, 1), (64, 1024, 128, 1), (2048, 512, 64, 1)):
+        with pytest.raises(ValueError, match="CUDA"):
+            op_table().masked_attention(Q, K, K, 0.1, store.as_strided((2, 3, 4, 64), strides))
+    with pytest.raises(ValueError, match="CUDA"):                       # keys may: a window that moves by a row
+        op_table().masked_attention(Q, z(1 << 12).as_strided((2, 5, 2, 64), (64, 64, 64, 1)), K, 0.1, z(2, 3, 4, 64))
+
+
+def test_append_refuses_a_cache_that_is_its_own_twin():
+    c, starts, new = allocate_quantized_cache(2, 128, 2, 64, "cpu"), z(2, dtype=i32), z(2, 3, 2, 64)
+    for twin in (c._replace(V=c.K), c._replace(V_scale=c.K_scale)):
+        with pytest.raises(ValueError, match="share memory"):
+            op_table().cache_append(new, new, twin, starts)

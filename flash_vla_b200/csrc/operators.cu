@@ -48,7 +48,9 @@ static int check_attention(const struct fvla_attention* a) {
     FVLA_REQUIRE((a->q_docs != nullptr) == (a->k_docs != nullptr), "attention: documents of queries and keys, or of neither");
     FVLA_REQUIRE(a->prefix == nullptr || a->causal, "attention: a prefix without the causal mask");
     FVLA_REQUIRE(a->weights == nullptr || ((a->lse != nullptr || decay) && q8), "attention: weights need the 8-bit cache and the log-sum-exp");
-    FVLA_REQUIRE(a->cap >= 0.f && a->scale == a->scale, "attention: scale and cap");
+    const auto finite = [](float x) { return x - x == 0.f; };
+    FVLA_REQUIRE(a->cap >= 0.f && finite(a->cap * kLog2e) && finite(a->scale * kLog2e) && finite(a->decay) && (a->cap == 0.f || finite(a->scale / a->cap)),
+                 "attention: scale, cap and decay must be finite, scale over cap as well, the cap not negative");
     FVLA_REQUIRE((long long)a->tokens * a->heads < (1ll << 31) && (long long)a->episodes * a->tokens * a->heads < (1ll << 31) && (long long)a->episodes * a->kv_heads < 65536, "attention: too many rows");
     FVLA_REQUIRE(((long long)a->tokens / (128 / (a->heads / a->kv_heads)) + 1) * a->kv_heads * a->episodes < (1ll << 30), "attention: too many rows");
     return FVLA_OK;

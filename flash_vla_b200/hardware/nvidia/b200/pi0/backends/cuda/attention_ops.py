@@ -16,7 +16,6 @@ from __future__ import annotations
 
 import ctypes
 import functools
-import math
 import operator
 import struct
 
@@ -209,8 +208,8 @@ def _attend(Q, K, V, cache, scale, out, causal, prefix, q_lens, k_lens, q_start,
         plan = _attention_plan(_layout(Q), None, None, _layout(out), _cache_layout(cache))
     strides, dims, nbytes, E, T, S, H, (fq, fk, fv, fo), same = plan
     scale, cap, decay = float(scale), float(cap or 0.0), float(decay)
-    if not math.isfinite(scale) or not (0.0 <= cap < math.inf) or not math.isfinite(decay):
-        raise ValueError(f"attention: scale {scale}, cap {cap}, decay {decay}: finite numbers, the cap not negative")
+    if not (abs(scale) < 2e38 and abs(decay) < 3.4e38 and (cap == 0.0 or (1.2e-38 < cap < 2e38 and abs(scale) < 3.4e38 * cap))):
+        raise ValueError(f"attention: scale {scale}, cap {cap}, decay {decay}: finite numbers within fp32, scale over cap as well, the cap not negative")
     if prefix is not None and not causal:
         raise ValueError("attention: a prefix without the causal mask")
     if (q_docs is None) != (k_docs is None):

@@ -114,3 +114,23 @@ def test_append_refuses_a_cache_that_is_its_own_twin():
     for twin in (c._replace(V=c.K), c._replace(V_scale=c.K_scale)):
         with pytest.raises(ValueError, match="share memory"):
             op_table().cache_append(new, new, twin, starts)
+
+
+@pytest.mark.parametrize("kw", [{"scale": 1e39}, {"scale": -1e300}, {"scale": float("nan")}, {"cap": 1e39}, {"cap": 1e-45}, {"cap": 1e-300}, {"scale": 1e10, "cap": 1e-30}, {"decay": 1e39},
+                                {"decay": -float("inf")}])
+def test_numbers_beyond_fp32_are_refused(kw):
+    """They would reach the kernels as infinities, or (a cap that rounds to zero) as another function."""
+    Q, c = z(1, 1, 2, 64), allocate_quantized_cache(1, 64, 2, 64, "cpu")
+    with pytest.raises(ValueError, match="finite numbers"):
+        op_table().cache_attention(Q, c, z(1, dtype=i32), kw.get("scale", 0.1), z(1, 1, 2, 64), cap=kw.get("cap", 0.0), decay=kw.get("decay", 1.0))
+
+
+@pytest.mark.parametrize("kw", [{"scale": float("inf")}, {"scale": float("nan")}, {"cap": float("inf")}, {"cap": 3e38}, {"scale": 1e10, "cap": 1e-30}, {"decay": float("nan")}])
+def test_the_entry_refuses_numbers_that_are_not_finite(kw):
+    a = _lib.Attention()
+    a.q = a.k = a.v = a.out = 1 << 20
+    a.q_stride[:] = a.out_stride[:] = a.k_stride[:] = a.v_stride[:] = (512, 512, 64)
+    a.episodes, a.tokens, a.keys, a.heads, a.kv_heads, a.head_dim, a.scale = 1, 1, 64, 8, 1, 64, 0.1
+    for name, value in kw.items():
+        setattr(a, name, value)
+    assert _lib.load().fvla_attention_run(ctypes.byref(a), None) == -1 and b"finite" in _lib.load().fvla_last_error()

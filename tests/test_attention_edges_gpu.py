@@ -232,3 +232,75 @@ def test_evict_between_interleaved_tensors(layout):
     with pytest.raises(ValueError, match="lies over"):                         # one row on: the source's rows in the destination
         t = torch.zeros(E, rows + 128, HK, D, dtype=torch.uint8, device="cuda").view(e4m3)
         op_table().cache_evict(whole._replace(K=t[:, :rows]), A.ints([256, 90]), w, keep, want._replace(K=t[:, rows - 1:rows + 127]), m)
+
+
+PROMPTS = [  # episodes, tokens, rows, heads, kv heads, dim, block: 128-row tiles over the 8-bit cache whose keys one CTA walks (75 tiles and more, or one block of keys)
+    (8, 160, 512, 8, 1, 256, 64), (10, 64, 384, 32, 8, 128, 32), (6, 300, 304, 12, 4, 80, 16), (1, 51, 128, 8, 1, 256, 128), (2, 70, 96, 4, 4, 64, 32), (5, 257, 640, 3, 1, 16, 64)]
+
+
+@pytest.mark.parametrize("shape", PROMPTS)
+@pytest.mark.parametrize("kind", ["plain", "all", "positions"])
+def test_prompts_over_the_cache(shape, kind):
+    E, T, rows, H, HK, D, block = shape
+    size = torch.exp2(torch.arange(rows, device="cuda").div(16, rounding_mode="floor").remainder(7).float() - 3)[None, :, None, None]      # blocks of unlike scales
+    cache = cache_of((randn(101, E, rows, HK, D).float() * size).to(bf16), (randn(102, E, rows, HK, D).float() * size.flip(1)).to(bf16), block)
+    Q = (randn(103, E, T, H, D).float() * 0.25).to(bf16)
+    lengths, q_lens = A.ints([max(1, rows - 37 * e) for e in range(E)]), A.ints([max(0, min(T, T + 10 - 29 * e)) for e in range(E)])
+    slopes = torch.tensor([2.0 ** (-4.0 * (h + 1) / H) for h in range(H)], device="cuda")
+    kw = {"plain": {}, "all": {"causal": True, "cap": 15.0, "slopes": slopes, "prefix": A.ints([rows // 3] * E), "q_lens": q_lens},
+          "positions": {"causal": True, "q_lens": q_lens, "q_start": A.ints([900 + e for e in range(E)]), "slopes": slopes * 0.01,
+                        "k_pos": torch.stack([torch.randperm(2 * rows, device="cuda", generator=torch.Generator("cuda").manual_seed(e))[:rows] + 500 for e in range(E)]).to(i32)}}[kind]
+    out, want = check_cached(Q, cache, lengths, D ** -0.5, **kw)
+    assert (out[~want["rows"]] == 7).all()
+
+
+@pytest.mark.parametrize("T", [1, 40])
+@pytest.mark.parametrize("D", [16, 48, 176])
+def test_small_and_odd_head_dims_over_the_cache(T, D):
+    cache = cache_of(randn(111, 2, 272, 2, D), randn(112, 2, 272, 2, D), 16)
+    check_cached(randn(113, 2, T, 6, D), cache, A.ints([272, 131]), D ** -0.5, causal=True)
+
+
+@pytest.mark.parametrize("T", [1, 40])
+def test_broadcast_queries_and_caches(T):
+    """One Q, and one K and V, for all episodes; heads that share theirs. Scales are whole, as the cache has them."""
+    E, rows, H, HK, D = 3, 192, 8, 2, 64
+    Q, one = randn(121, 1, T, H, D).expand(E, T, H, D), cache_of(randn(122, 1, rows, 1, D), randn(123, 1, rows, 1, D))
+    shared = QuantizedCache(*(t.expand(E, rows, HK, D) for t in one[:2]), *(t.expand(E, rows // 64, HK).contiguous() for t in one[2:]))
+    lengths = A.ints([192, 65, 1])
+    want = A.attention(Q, A.widened(shared.K, shared.K_scale), A.widened(shared.V, shared.V_scale), 0.1, k_lens=lengths, causal=True)
+    out = torch.zeros(E, T, H, D, dtype=bf16, device="cuda")
+    op_table().cache_attention(Q, shared, lengths, 0.1, out, causal=True)
+    A.check_out(out, want, D, P_8BIT)
+    K, V = randn(124, E, rows, HK, D), randn(125, E, rows, HK, D)
+    op_table().masked_attention(Q, K, V, 0.1, out, k_lens=lengths, causal=True)
+    A.check_out(out, A.attention(Q, K, V, 0.1, k_lens=lengths, causal=True), D, 2.0 ** -8)
+
+
+@pytest.mark.parametrize("T", [1, 24])
+def test_many_episodes(T):
+    """More episodes than SMs: a CTA has all keys of a tile."""
+    E, rows, H, D = 700, 144, 8, 64
+    cache = cache_of(randn(131, E, rows, 1, D), randn(132, E, rows, 1, D), 16)
+    check_cached(randn(133, E, T, H, D), cache, A.ints([1 + (e * 7) % rows for e in range(E)]), 0.1, causal=True)
+
+
+def test_evicted_rows_of_a_far_cache():
+    """Rows 32 KB apart, byte offsets past 31 bits: K and V of the rows that stay, bit for bit."""
+    rows, keep, D = 70016, 64, 64
+    store = torch.zeros(2, rows, 1, 32768, dtype=torch.uint8, device="cuda").view(e4m3)
+    cache = QuantizedCache(store[:1, :, :, :D], store[1:, :, :, -D:], *(torch.ones(1, rows // 64, 1, device="cuda") for _ in range(2)))
+    size = torch.exp2(torch.arange(rows, device="cuda").div(64, rounding_mode="floor").remainder(5).float() - 2)[None, :, None, None]
+    op_table().cache_append((randn(141, 1, rows, 1, D).float() * size).to(bf16), (randn(142, 1, rows, 1, D).float() * size).to(bf16), cache, A.ints([0]))
+    first = rows - 200
+    w = torch.zeros(1, rows, device="cuda")
+    w[0, first:] = 1.0                                                          # ties: the first 64 of them stay
+    small, n = allocate_quantized_cache(1, keep, 1, D, "cuda"), A.ints([0])
+    op_table().cache_evict(cache, A.ints([rows]), w, keep, small, n)
+    kept = torch.arange(first, first + keep, device="cuda")
+    assert n.tolist() == [keep]
+    for got, got_scale, held, scale in ((small.K, small.K_scale, cache.K, cache.K_scale), (small.V, small.V_scale, cache.V, cache.V_scale)):
+        source = scale[0, kept // 64, 0]
+        assert (source != source[0]).any() and got_scale[0, 0, 0] == source.max()
+        moved = A.to_e4m3(held[0, first:first + keep, 0].float() * (source / source.max())[:, None])
+        assert A.same_bits(got[0, :, 0].contiguous(), moved)

@@ -332,9 +332,10 @@ inline bool takes_few(const Args& a) { return (long long)a.tokens * (a.heads / a
 // Head dimension that the kernel is built for.
 inline int padded_dim(const Args& a) { return a.dim <= 64 && !takes_few(a) && a.k_scale == nullptr ? 64 : (a.dim <= 128 ? 128 : 256); }
 
-// Shares of the key blocks: as many as bring the CTAs up to the number that are resident, at most one per block.
+// Shares of the key blocks: as many as bring the CTAs up to the number that are resident, at most one per block. (Below: a token of 8 query heads per K/V head of
+// 256 unless said, both sides in us.)
 inline int plan_splits(const Args& a) {
-    const int group = a.heads / a.kv_heads, tile_tokens = BQ / group, blocks = (a.keys + BKEY - 1) / BKEY;
+    const int group = a.heads / a.kv_heads, tile_tokens = BQ / group, blocks = (a.keys + BKEY - 1) / BKEY, sms = tc5::num_sms();
     const bool few = takes_few(a);
     const long long tiles = (few ? 1ll : (long long)((a.tokens + tile_tokens - 1) / tile_tokens)) * a.kv_heads * a.episodes;
     int per_sm = 1;
@@ -342,11 +343,15 @@ inline int plan_splits(const Args& a) {
         const int tile_bytes = 128 * padded_dim(a) * (a.k_scale ? 1 : 2);
         per_sm = few_rows(a) == 32 ? (tile_bytes == 16384 ? 2 : 1) : (tile_bytes == 16384 ? 3 : (tile_bytes == 32768 ? 2 : 1));
     }
-    const long long room = (long long)tc5::num_sms() * per_sm * (few && tiles > tc5::num_sms() ? 2 : 1) / tiles;
-    // A cluster rather than a second launch that joins the shares, up to four blocks for each of its CTAs. (8 heads of 256 over 32 blocks of the 8-bit cache, eight shares
-    // in a cluster / as many as are resident: eight episodes 11.4 / 14.3 us, one 11.2 / 10.7; over 64 blocks 17.6 / 15.8 and 16.3 / 11.6. bf16, 32 blocks: eight episodes 14.0 / 15.3,
-    // two 12.2 / 11.6.)
-    if (few && room > CLUSTER && blocks <= 4 * CLUSTER) return blocks < CLUSTER ? (blocks > 0 ? blocks : 1) : CLUSTER;
+    // Few rows of more tiles than SMs: twice as many, which evens out the last round. 160 episodes over 2 048 / 8 192 rows 40.6 / 92 us, 44.1 / 125 without. At three CTAs
+    // an SM (8 bits, head dim 128, 8 K/V heads) from 64 blocks on: 24 episodes of 8 192 58.4 (60.5), 32 of 16 384 130 (155), but of 4 096 38.3 (35.5).
+    const bool twice = few && tiles > sms && (per_sm < 3 || blocks >= 64);
+    const long long room = (long long)sms * per_sm * (twice ? 2 : 1) / tiles;
+    // A cluster rather than a second launch that joins the shares, up to two blocks for each of its CTAs, and up to four where there are some tiles. 8 bits, 16 blocks: one
+    // episode 9.5 (11.1 with a join), 32 of them 11.7 (14.5); 32 blocks: one 12.0 (11.3), four 12.0 (12.2), 32 18.1 (21.8). bf16, 32 blocks: four 12.7 (11.0), twelve
+    // 15.0 (16.6). Where a CTA takes a whole SM, clusters of eight leave SMs over: 14 of them 9.6 (12.0), but 16 take a second round, 17.7 (12.2).
+    const bool fits = per_sm > 1 || 5 * CLUSTER * tiles <= 4 * sms;
+    if (few && fits && room > CLUSTER && blocks <= (tiles * per_sm >= 8 ? 4 : 2) * CLUSTER) return blocks < CLUSTER ? (blocks > 0 ? blocks : 1) : CLUSTER;
     return (int)(room < 1 ? 1 : (room < blocks ? room : (blocks > 0 ? blocks : 1)));
 }
 inline size_t score_pitch(const Args& a) { return ((size_t)a.keys + BKEY - 1) / BKEY * BKEY; }
@@ -368,8 +373,11 @@ inline size_t workspace_bytes(const Args& a) {
 
 inline int launch_join(const Tile& p, int hdp, cudaStream_t st) {
     const long long rows = (long long)p.a.episodes * p.a.tokens * p.a.heads;
-    // many shares: eight warps for 32 columns of a row; few: a warp or some for the whole row
-    const int warps = p.splits >= 16 ? 8 : (p.splits >= 8 ? 4 : 1), each = JOIN_WARPS / warps, per = p.splits >= 16 ? 1 : hdp / 32;
+    // From eight shares on several warps for a row; of a few rows also a CTA for 32 columns. Both sides in us, attention and join: 8 rows of 256, 296 shares 25.6 (28.0 with the
+    // whole row to a CTA), 24 rows, 98 shares 20.3 (20.9 with columns apart); 408 rows, 32 shares: eight warps 19.3, four 20.7, one 24.8, columns apart 38.6; 800 rows: 26.0,
+    // 23.7, 28.6, 61; 2 400 rows, 7 shares: one warp 57, four 62.
+    const bool columns = rows <= 12 && p.splits >= 16;
+    const int warps = p.splits < 8 ? 1 : (rows < 512 ? 8 : 4), each = JOIN_WARPS / warps, per = columns ? 1 : hdp / 32;
     const auto kern = per == 1 ? attention_join_kernel<1> : (per == 2 ? attention_join_kernel<2> : (per == 4 ? attention_join_kernel<4> : attention_join_kernel<8>));
     const cudaError_t e = launch_pdl(kern, dim3((unsigned)((rows + each - 1) / each), hdp / (32 * per)), dim3(32 * JOIN_WARPS), 0, st, p, hdp, warps);
     if (e != cudaSuccess) { set_error("attention_join_kernel: %s", cudaGetErrorString(e)); return FVLA_ERR_LAUNCH; }
@@ -397,7 +405,9 @@ inline int launch_weights(const Tile& p, cudaStream_t st) {
     const Args& a = p.a;
     cudaError_t e;
     if (takes_few(a)) {
-        // a warp for up to 16 rows, sixteen for the most: eight rows or more for each; CTAs of four warps at least
+        // A warp for up to 16 rows, sixteen for the most: eight rows or more for each; CTAs of four warps at least. Attention and weights, with 1 / 2 / 4 / 8 / 16 warps, us: 8 rows
+        // over 131 072 keys 31.6 / 32.0 / 36.0 / 44.4 / 50.0, 32 rows over 4 096 of eight episodes 25.0 / 21.6 / 20.1 / 20.6 / 24.2, over 16 384 of 32 146 / 146 / 150 / 181 / 249,
+        // 128 rows over 4 096 of two 40.0 / 30.1 / 25.2 / 22.0 / 20.0.
         const int rows_each = a.tokens * a.heads;
         int share = 1;
         while (share < WEIGHT_WARPS && rows_each > 16 * share) share *= 2;

@@ -227,6 +227,8 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
         };
         if (count > 0) {
             fetch(0);
+            const int scale_end = Q8 ? (min((first + count) * BKEY, s.L) + a.block - 1) >> shift : 0, scale0 = (first * BKEY >> shift) + key;
+            const float scale = scale0 < scale_end ? __ldg(vs + (size_t)scale0 * a.kv_heads) : 1.f;
             // Q as the K-major operand, and what the rows have of their own (rows of the operand behind NR, and their columns of S^T, are never looked at)
 #pragma unroll
             for (int i = 0; i < Q_ROWS; ++i) {
@@ -277,9 +279,8 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
             if (lane == 0) tc5::mbar_arrive(q_ready);
             if (Q8) {
                 // while the scores are made: whether a scale of V in this share is very small or large
-                const int end = (min((first + count) * BKEY, s.L) + a.block - 1) >> shift;
-                bool odd = false;
-                for (int i = (first * BKEY >> shift) + key; i < end; i += BKEY) odd |= odd_scale(__ldg(vs + (size_t)i * a.kv_heads));
+                bool odd = odd_scale(scale);
+                for (int i = scale0 + BKEY; i < scale_end; i += BKEY) odd |= odd_scale(__ldg(vs + (size_t)i * a.kv_heads));
                 if (odd) *odd_scales = 1;
                 barrier();
             }
@@ -423,6 +424,7 @@ attention_few_rows_kernel(const __grid_constant__ Tile p, const __grid_constant_
                     }
                 }
             } else {
+                // (the operand of the second product is bf16, as K and V are: half a step, 2^-8 of a probability; the row sum has all 24 bits)
 #pragma unroll
                 for (int r = 0; r < NR; ++r)
                     *reinterpret_cast<bf16*>(gen + C::OFF_P + (key >> 6) * (C::NO * 128) + r * 128 + ((((key & 63) >> 3) ^ (r & 7)) << 4) + (key & 7) * 2) = __float2bfloat16_rn(v[r]);

@@ -262,7 +262,7 @@ def masked_attention(Q, K, V, scale, out, causal=False, prefix=None, q_lens=None
     q_docs (E, T), k_docs (E, S): a query sees the keys of its own document; negative ids are padding.
     A query that sees no key gets zeros. lse (E, H, T) fp32 receives the natural log-sum-exp of the scores, -inf for such a query.
     One new token per episode (T = 1) is the same call. K and V behind k_lens, or under a negative document id, may hold anything; a value
-    of V elsewhere that is not finite can reach every query that is processed beside one that sees it."""
+    of V elsewhere that is not finite can reach queries that do not see it."""
     return _attend(Q, K, V, None, scale, out, causal, prefix, q_lens, k_lens, None, q_docs, k_docs, None, cap, slopes, lse, None, 1.0)
 
 

@@ -312,9 +312,11 @@ int fvla_embed_rows(const void* table, const long long* ids, void* out, int rows
  * sees nothing gets zeros and a log-sum-exp of -infinity; rows behind q_lens[e] stay as they were. With k_scale / v_scale (fp32, positive,
  * (episodes, keys / block, kv_heads) contiguous; block 16, 32, 64 or 128) k and v hold e4m3 values, else bf16. lse: (episodes, heads,
  * tokens) fp32. weights: (episodes, keys) fp32, weights[e][j] = decay * weights[e][j] + the probabilities that key j < k_lens[e] got from all queries;
- * needs lse and the 8-bit cache, and 4 bytes of ws for every score; with tokens = 0 (q, out and lse may be NULL) the weights decay, and that is all. Rows of k and v behind k_lens, scales of blocks without a row, and rows of a negative document, may hold any bits. All
- * others have to be finite: a value of v that is not can reach every query that is processed beside one that sees it. ws:
- * fvla_attention_workspace_bytes of these arguments, any contents, not shared by calls that may run at the same time. out may be q. head_dim: a multiple of 8 (e4m3: 16) up to 256; up to 128 query heads per K/V head. */
+ * needs lse and the 8-bit cache, and 4 bytes of ws for every score; with tokens = 0 (q, out and lse may be NULL) the weights decay, and that is all.
+ * Rows of k and v behind k_lens, scales of blocks without a row, and rows of a negative document may hold any bits. All others have to be finite: a
+ * value of v that is not can reach queries that do not see it. ws: fvla_attention_workspace_bytes of these arguments, any contents, not shared by calls
+ * that may run at the same time. out may be q with q's strides; otherwise it overlaps neither q, k nor v. head_dim: a multiple of 8 (e4m3: 16) up to
+ * 256; up to 128 query heads per K/V head. */
 struct fvla_attention {
     const void *q, *k, *v, *k_scale, *v_scale;
     void *out, *lse, *weights, *ws;

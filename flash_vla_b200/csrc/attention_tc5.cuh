@@ -77,12 +77,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) 
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
-__device__ __forceinline__ float fast_exp2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // 128 consecutive TMEM columns of this thread's lane: four 32-column loads issued back to back, one wait.
 __device__ __forceinline__ void ld_row128(uint32_t taddr, float (&v)[128]) {
     uint32_t r[128];

@@ -59,14 +59,6 @@ static inline cudaStream_t S(void* s) { return reinterpret_cast<cudaStream_t>(s)
 static inline const bf16* B(const void* p) { return reinterpret_cast<const bf16*>(p); }
 static inline bf16* Bm(void* p) { return reinterpret_cast<bf16*>(p); }
 
-#define FVLA_REQUIRE(cond, ...)            \
-    do {                                   \
-        if (!(cond)) {                     \
-            set_error(__VA_ARGS__);        \
-            return FVLA_ERR_ARG;           \
-        }                                  \
-    } while (0)
-
 static int rownorm(const void* x, int x_is_f32, const void* w, const void* b, void* out, float* f32,
                    void* fbf, int M, int K, int mode, cudaStream_t st) {
     FVLA_REQUIRE(M > 0 && K > 0 && K % 8 == 0 && K <= 8 * 32 * RN_MAX, "rownorm: bad shape M=%d K=%d (K %% 8 == 0, K <= %d)", M, K, 8 * 32 * RN_MAX);

@@ -17,6 +17,11 @@ using bf16 = __nv_bfloat16;
 constexpr float kGeluC0 = 1.5957691216057308f;   // 2 * sqrt(2 / pi)
 constexpr float kGeluC1 = 0.044715f;
 constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 // tanh-GELU. The reference kernels write it as v * sigmoid(C0 * v * (1 + C1 v^2))
 // (kernels/base.py:77-78); sigmoid(t) = (1 + tanh(t / 2)) / 2, and tanh.approx is one special-function
@@ -168,6 +173,15 @@ void set_error(const char* fmt, ...);
 int check_launch(const char* what);
 // Health word of the current device, written by kernels (0 = healthy).
 int* device_status_ptr();
+
+// Argument checks of the C entries.
+#define FVLA_REQUIRE(cond, ...)            \
+    do {                                   \
+        if (!(cond)) {                     \
+            set_error(__VA_ARGS__);        \
+            return FVLA_ERR_ARG;           \
+        }                                  \
+    } while (0)
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

@@ -6,9 +6,9 @@
 // The keys are the 128-row operand of both products, so that every thread of the softmax has one key and all rows of it:
 //   S^T (128 keys x rows) = K Q^T,      O^T (128 dims x rows, one or two halves) += V^T P^T
 // K and V tiles go from TMA straight to the tensor cores, also the 8-bit ones (kind::f8f6f4): nothing is converted. Instead the few rows are split
-// into e4m3 terms, each a row of the other operand. A bf16 q brought to 2^7..2^8 by its row's power of two is the sum of two terms of 4 bits
-// (the second times 2^5; what falls below the subnormals is under 2^-22 of the row's largest element), a probability the sum of three (times 2^4 and
-// 2^8: 12 bits). Probabilities stand against the running maximum at 2^4, which leaves 2^-22 of it above the last term's half step.
+// into e4m3 terms, each a row of the other operand. A bf16 q brought to 2^7..2^8 by its row's power of two is the sum of two terms of 4 bits, the second
+// times 2^5 (exactly, but for elements below e4m3's smallest normal number, 2^-13 of the largest: 2^-4 of half its smallest step, 2^-21 of the largest). A
+// probability is the sum of three (times 2^4 and 2^8): with the maximum at 2^4 it is off by at most 2^-12 of itself or 2^-22 of the row's largest.
 // The scale of V moves into their exponent, and the row sum takes it back; where a share has very small or large scales (a block of zeros has 2^-120, and
 // its inverse would end fp32's range), the row sum is taken from the scores themselves against a maximum of its own. What a share leaves is its maximum, its
 // sums and the log2 of its row sum.

@@ -87,11 +87,6 @@ __global__ void __launch_bounds__(128) document_ranges_kernel(const int* __restr
     if (lane == 0) range[i] = make_int2(low, high);
 }
 
-__device__ __forceinline__ float fast_exp2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ float fast_rcp(float x) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

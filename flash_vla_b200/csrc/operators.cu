@@ -7,14 +7,6 @@ namespace fvla {
 
 static inline cudaStream_t S(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
-#define FVLA_REQUIRE(cond, ...)            \
-    do {                                   \
-        if (!(cond)) {                     \
-            set_error(__VA_ARGS__);        \
-            return FVLA_ERR_ARG;           \
-        }                                  \
-    } while (0)
-
 template <typename... KArgs, typename... Args>
 static int launch(const char* what, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
     const cudaError_t e = launch_pdl(kern, grid, block, smem, st, args...);

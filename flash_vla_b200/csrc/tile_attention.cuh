@@ -5,18 +5,21 @@
 //   warps 1, 2  one lane of each issues S = Q K^T into one of BUFFERS TMEM score buffers, and O += P V (TMEM). (An issue takes 50 to 100 clocks with
 //               its waits; one lane for both was the bottleneck at head dim 128: 301 us against 281.)
 //   warps 4-11  softmax: two groups of 128 threads, thread = row, which take the blocks in turn. P goes back to TMEM over the scores, as the A operand
-//               of P V (of bf16 keys of head dim 256, whose two score buffers have to be free early, through shared memory: 113 us against 127). All that one block needs from the one before is the running maximum: the other group
-//               hands it on (per warp, 32 rows) before it begins its exponentials, and those of one block run beside the other's
-//               loads and maxima. The accumulator is rescaled only where the maximum has grown by more than a threshold.
-// 4 096 keys, 32 query heads of 128, or 8 of 256 over 4 K/V heads: 270 us (1 018 TFLOP/s) and 112 us (1 231 TFLOP/s). A block of 128 keys takes 2 200 to
-// 2 500 clocks: at head dim 128 the softmax's instructions (128 exponentials of a row at 16 clocks a warp among them), at 256 the arrival of 128 KB of
-// keys and values through 128 KB of rings. A CTA's two ends, 7 000 and 5 000 clocks, are the rest of short walks.
-// The 8-bit cache runs in 8 bits (kind::f8f6f4), its values straight from TMA: a bf16 row of Q, brought to 2^7..2^8 by its own power of two, is the sum
-// of an e4m3 term and an e5m2 term (what rounding to 4 bits leaves of 8 has at most 3; below 2^-16, 2^-23 of the largest, is lost), a probability the sum
-// of two e4m3 terms and an e5m2 term. Probabilities stand against the running maximum at 2^6 and are rescaled when it has grown by 2^2: the terms leave 2^-4 of
-// a value and 2^-4 of the rest, or half of e4m3's smallest step, 2^-10, and then 2^-3 of that. So a probability is off by at most 2^-11 of itself or 2^-19 of the row's largest. The scale of K multiplies the scores in fp32; the
-// scale of V moves into the exponent of P (w = log2 p + log2 V_scale, P = 2^(w - max w)), and the row sum takes it back, or, where a share has very
-// small or large scales (a block of zeros has 2^-120, and its inverse would end fp32's range), is taken from the scores themselves against a maximum of their own.
+//               of P V; with bf16 keys of head dim 256, whose two score buffers have to be free early, through shared memory (113 us against 127). All
+//               that one block needs from the one before is the running maximum: the other group hands it on (per warp, 32 rows) before it begins
+//               its exponentials, and those of one block run beside the other's loads and maxima. The accumulator is rescaled only
+//               where the maximum has grown by more than a threshold.
+// 4 096 keys, 32 query heads of 128, or 8 of 256 over 4 K/V heads, without a mask: 266 us (1 033 TFLOP/s) and 111 us (1 243 TFLOP/s). A block of 128 keys
+// takes 2 200 to 2 500 clocks: at head dim 128 the softmax's instructions (128 exponentials of a row at 16 clocks a warp among them), at 256 the arrival of
+// 128 KB of keys and values through 128 KB of rings. A CTA's two ends, 7 000 and 5 000 clocks, are the rest of short walks.
+// The 8-bit cache runs in 8 bits (kind::f8f6f4; 256 tokens of eight episodes over 4 096 rows of 256: 137 us, 375 TFLOP/s), its values straight from TMA. A
+// bf16 row of Q, brought to 2^7..2^8 by its own power of two, is the sum of an e4m3 term and an e5m2 term: what rounding to 4 bits leaves of 8 has at most 3.
+// (Elements below e4m3's smallest normal number, 2^-13 of the largest, are off by 2^-3 of half its smallest step, 2^-20 of the largest.) A probability is the
+// sum of two e4m3 terms and an e5m2 term. Probabilities stand against the running maximum at 2^6 and are rescaled when it has grown by 2^2: the first two
+// terms leave 2^-8 of a value, or half of e4m3's smallest step, 2^-10, and the third 2^-3 of that. So a probability is off by at most 2^-11 of itself or 2^-19
+// of the row's largest. The scale of K multiplies the scores in fp32; the scale of V moves into the exponent of P (w = log2 p + log2 V_scale, P =
+// 2^(w - max w)), and the row sum takes it back, or, where a share has very small or large scales (a block of zeros has 2^-120, and its inverse would end
+// fp32's range), is taken from the scores themselves against a maximum of their own.
 #pragma once
 
 namespace fvla {
